@@ -325,7 +325,7 @@ def _plain_plan(st):
     rank = start[:, None] + col - held[:, None]
     table = torch.where(m, stack[(avail - 1 - rank).clamp(0, cap)].to(torch.int32), table)
     at = torch.arange(cap, device=DEV)
-    pool = torch.where((at >= free) & (at < left), stack[:cap].to(torch.int32), pool)
+    pool = torch.where((at >= free) & (at < avail), stack[:cap].to(torch.int32), pool)
     kv = torch.where(ok, ctx + add, ctx.new_zeros(()))
     # the rows of the step: position and slot of every new token
     t = torch.arange(rows, device=DEV)
@@ -475,6 +475,7 @@ def _exact_plan(st):
     cu, kv = [0], []
     pos, slots = np.zeros(rows, np.int32), np.full(rows, -1, np.int64)
     bad, wanted, avail = 0, 0, len(stack)
+    pool[free:avail] = stack[free:]                       # given back, whether or not this step takes them again
     for i in range(n):
         a = max(new[i], 0)
         t0 = cu[-1]
@@ -498,8 +499,6 @@ def _exact_plan(st):
         p = np.arange(ctx[i], ctx[i] + a)
         pos[t0:t0 + a] = p
         slots[t0:t0 + a] = table[i, p // ps].astype(np.int64) * ps + p % ps
-    if len(stack) > free:
-        pool[free:len(stack)] = stack[free:]
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
     return {"table": torch.from_numpy(table).to(DEV), "pool": torch.from_numpy(pool).to(DEV), "left": i32([len(stack)]),
             "cu": i32([min(c, rows) for c in cu]), "kv": i32(kv), "pos": torch.from_numpy(pos).to(DEV),
