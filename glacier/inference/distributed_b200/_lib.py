@@ -17,6 +17,7 @@ STATUS_NAMES = {
     -5: "GLC_ERR_DISPOSED", -6: "GLC_ERR_NCCL", -7: "GLC_ERR_TIMEOUT", -8: "GLC_ERR_STATE",
 }
 GLC_GGUF_Q4_K = 12
+GLC_GGUF_F32, GLC_GGUF_F16 = 0, 1
 GLC_WIRE_FP32, GLC_WIRE_FP16, GLC_WIRE_INT8, GLC_WIRE_FP8_E4M3 = 0, 1, 2, 3
 GLC_FWD_RMSNORM, GLC_FWD_RESIDUAL, GLC_FWD_DECODE, GLC_FWD_BATCHED, GLC_FWD_UNFUSED = 1, 2, 4, 8, 16
 
@@ -73,6 +74,14 @@ class GemvJob(C.Structure):
 GLC_GEMV_SET, GLC_GEMV_ADD, GLC_GEMV_GATE_UP = 0, 1, 2
 
 
+class KvPagesDesc(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+        ("row_stride", C.c_int64), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+    ]
+
+
 class FusedHeader(C.Structure):
     _fields_ = [
         ("sequence_id", C.c_uint64), ("token_index", C.c_int32), ("layer_index", C.c_int32),
@@ -83,6 +92,7 @@ class FusedHeader(C.Structure):
 
 vp = C.c_void_p
 i32 = C.c_int32
+i64 = C.c_int64
 _SIGNATURES = {
     "glc_abi_version": (C.c_int, []),
     "glc_last_error": (C.c_char_p, []),
@@ -111,6 +121,15 @@ _SIGNATURES = {
     "glc_attn_workspace_bytes": (C.c_int, [i32, i32, i32, C.POINTER(C.c_uint64)]),
     "glc_attn_decode_dev": (C.c_int, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, C.c_float, vp, vp,
                                       C.c_uint64, vp]),
+    "glc_kv_plan_dev": (C.c_int, [vp, vp, i32, i32, vp, i32, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp]),
+    "glc_rope_append_dev": (C.c_int, [vp, i64, vp, vp, i64, i32, i32, i32, vp, vp, C.c_float, vp, vp, i32, vp, vp,
+                                      vp]),
+    "glc_attn_prompt_dev": (C.c_int, [vp, i32, i64, vp, vp, i64, vp, i32, i32, i32, i32, i32, C.c_float, vp, i64,
+                                      vp]),
+    "glc_attn_paged_workspace_bytes": (C.c_int, [i32, i32, i32, i32, i32, C.POINTER(C.c_uint64)]),
+    "glc_attn_paged_dev": (C.c_int, [vp, i32, i64, vp, vp, i32, vp, vp, i32, i32, i32, i32, C.c_float, vp, i64, vp,
+                                     C.c_uint64, vp]),
+    "glc_paged_poll_error": (C.c_int, []),
     "glc_router_topk_dev": (C.c_int, [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]),
     "glc_dispatch_plan_dev": (C.c_int, [vp, i32, i32, vp, vp, vp, vp, vp]),
     "glc_dispatch_plan_noalloc_dev": (C.c_int, [vp, i32, i32, vp, vp, vp, vp, vp]),

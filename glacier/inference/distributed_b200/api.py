@@ -274,6 +274,78 @@ def attn_decode_dev(q_ptr: int, k_new_ptr: int, v_new_ptr: int, k_cache_ptr: int
                                     head_dim, max_len, pos, rope_theta, out_ptr, work_ptr, work_bytes, stream))
 
 
+GGUF_F32, GGUF_F16 = _lib.GLC_GGUF_F32, _lib.GLC_GGUF_F16
+
+
+class KvPages:
+    """The fp16 key and value pages of one layer (glc_kv_pages), on the caller's
+    device memory.  Default strides: [page][KV head][row][128]; strides are in
+    elements."""
+
+    def __init__(self, k_ptr: int, v_ptr: int, n_pages: int, page_size: int, n_kv_heads: int, *,
+                 page_stride: int | None = None, head_stride: int | None = None, row_stride: int | None = None,
+                 head_dim: int = 128):
+        row = head_dim if row_stride is None else row_stride
+        head = page_size * row if head_stride is None else head_stride
+        page = n_kv_heads * head if page_stride is None else page_stride
+        self.desc = _lib.KvPagesDesc(k_ptr, v_ptr, page, head, row, n_pages, page_size, n_kv_heads, head_dim)
+        self._ref = C.byref(self.desc)
+
+
+def kv_plan_dev(ctx_lens_ptr: int, new_lens_ptr: int, B: int, page_size: int, block_table_ptr: int, max_pages: int,
+                free_list_ptr: int, capacity: int, free_count_ptr: int, free_count_out_ptr: int, T: int,
+                cu_new_ptr: int, kv_lens_ptr: int, positions_ptr: int, slots_ptr: int, status_ptr: int,
+                stream: int | None = None) -> None:
+    """Page plan of a step (glc_kv_plan_dev): pages of finished requests back on
+    the free list, pages for the new tokens, first rows, cache lengths,
+    positions and slots."""
+    check(lib().glc_kv_plan_dev(ctx_lens_ptr, new_lens_ptr, B, page_size, block_table_ptr, max_pages, free_list_ptr,
+                                capacity, free_count_ptr, free_count_out_ptr, T, cu_new_ptr, kv_lens_ptr,
+                                positions_ptr, slots_ptr, status_ptr, stream))
+
+
+def rope_append_dev(q_ptr: int | None, q_stride: int, k_ptr: int, v_ptr: int, kv_stride: int, T: int, n_heads: int,
+                    n_kv_heads: int, positions_ptr: int, slots_ptr: int | None, rope_theta: float,
+                    cache: KvPages | None, q_out_ptr: int | None, q_out_type: int = GGUF_F32,
+                    k_out_ptr: int | None = None, v_out_ptr: int | None = None, stream: int | None = None) -> None:
+    """RoPE on T rows of queries and keys and the store of the rotated keys and
+    the values in their slots (glc_rope_append_dev)."""
+    check(lib().glc_rope_append_dev(q_ptr, q_stride, k_ptr, v_ptr, kv_stride, T, n_heads, n_kv_heads, positions_ptr,
+                                    slots_ptr, rope_theta, None if cache is None else cache._ref, q_out_ptr,
+                                    q_out_type, k_out_ptr, v_out_ptr, stream))
+
+
+def attn_prompt_dev(q_ptr: int, q_type: int, q_stride: int, k_ptr: int, v_ptr: int, kv_stride: int,
+                    cu_seqlens_ptr: int, B: int, T: int, n_heads: int, n_kv_heads: int, out_ptr: int,
+                    out_stride: int, scale: float = 0.0, head_dim: int = 128, stream: int | None = None) -> None:
+    """Causal attention over B packed prompts (glc_attn_prompt_dev)."""
+    check(lib().glc_attn_prompt_dev(q_ptr, q_type, q_stride, k_ptr, v_ptr, kv_stride, cu_seqlens_ptr, B, T, n_heads,
+                                    n_kv_heads, head_dim, scale, out_ptr, out_stride, stream))
+
+
+def attn_paged_workspace_bytes(n_heads: int, n_kv_heads: int, B: int, T: int, max_new: int) -> int:
+    n = C.c_uint64(0)
+    check(lib().glc_attn_paged_workspace_bytes(n_heads, n_kv_heads, B, T, max_new, C.byref(n)))
+    return int(n.value)
+
+
+def attn_paged_dev(q_ptr: int, q_type: int, q_stride: int, cache: KvPages, block_table_ptr: int, max_pages: int,
+                   cu_new_ptr: int, kv_lens_ptr: int, B: int, T: int, max_new: int, n_heads: int, out_ptr: int,
+                   out_stride: int, work_ptr: int, work_bytes: int, scale: float = 0.0,
+                   stream: int | None = None) -> None:
+    """Attention of the new tokens of B sequences over the paged cache
+    (glc_attn_paged_dev): chunks of prompts and single decode tokens."""
+    check(lib().glc_attn_paged_dev(q_ptr, q_type, q_stride, cache._ref, block_table_ptr, max_pages, cu_new_ptr,
+                                   kv_lens_ptr, B, T, max_new, n_heads, scale, out_ptr, out_stride, work_ptr,
+                                   work_bytes, stream))
+
+
+def paged_poll_error() -> None:
+    """Raises GlcError when a paged entry point met a page id, slot or length out
+    of range on the device, or a bounded device-side wait gave up."""
+    check(lib().glc_paged_poll_error())
+
+
 def dispatch_plan_dev(ids_ptr, P, E, counts_ptr, offsets_ptr, perm_ptr, inv_ptr, stream=None):
     check(lib().glc_dispatch_plan_dev(ids_ptr, P, E, counts_ptr, offsets_ptr, perm_ptr, inv_ptr, stream))
 

@@ -68,15 +68,6 @@ struct AttnSmem {
     float cs_c[kHd / 2], cs_s[kHd / 2];
 };
 
-// RoPE of pair i (0..63) at position pos: cos and sin of pos * theta^(-2i/128)
-// (the frequency formed on the host in double), the angle formed and reduced
-// to [-pi, pi] in double, then sincosf.
-__device__ __forceinline__ void rope_cs(int pos, double inv_freq, float& c, float& s) {
-    double ang = (double)pos * inv_freq;
-    ang -= 6.283185307179586 * rint(ang * 0.15915494309189535);
-    sincosf((float)ang, &s, &c);
-}
-
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }

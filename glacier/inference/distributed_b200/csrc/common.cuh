@@ -278,6 +278,15 @@ __device__ __forceinline__ float tree8(const float* s) {
     return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
+// RoPE of pair i (0..63) at position pos: cos and sin of pos * theta^(-2i/128)
+// (the frequency formed on the host in double), the angle formed and reduced
+// to [-pi, pi] in double, then sincosf.
+__device__ __forceinline__ void rope_cs(int pos, double inv_freq, float& c, float& s) {
+    double ang = (double)pos * inv_freq;
+    ang -= 6.283185307179586 * rint(ang * 0.15915494309189535);
+    sincosf((float)ang, &s, &c);
+}
+
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }

@@ -1,0 +1,35 @@
+// paged.cuh -- what the paged-cache entry points share: argument errors with a
+// formatted message, the device error word, the checks of a glc_kv_pages and
+// the TMA descriptors of its pages.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../../../include/glacier_b200.h"
+#include "kernels.h"
+
+namespace glc {
+
+// Records the formatted message for glc_last_error() and returns `code`.
+int paged_fail(int code, const char* fmt, ...);
+
+// Device error word of the current device (GLC_OK and *err set, or the status
+// of the failure).  A fixed device word of the library: nothing is allocated.
+int paged_error_word(int** err);
+
+// GLC_OK when `device_ptr` is memory the current device owns or can be handed
+// without faulting (managed and pinned host memory included).
+int paged_check_device(const void* device_ptr, const char* what);
+
+// The shape, strides and alignment rules of a page set.
+int paged_check_pages(const glc_kv_pages* c);
+
+// A descriptor of 128-wide fp16 rows as [pages][heads][2 halves][rows][64]:
+// a box is `box_rows` rows of `box_halves` 64-element halves of one head of
+// one page, 128-byte swizzled.  Rows and pages past the end read as zeros.
+int paged_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_stride, int64_t heads,
+                     int64_t head_stride, int64_t pages, int64_t page_stride, int box_rows, int box_halves);
+
+}  // namespace glc

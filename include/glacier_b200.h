@@ -47,6 +47,9 @@ extern "C" {
 
 /* GGUF tensor types accepted for expert weights (GGUF type ids). */
 #define GLC_GGUF_Q4_K 12
+/* GGUF type ids of the query and output rows of the batched attention. */
+#define GLC_GGUF_F32 0
+#define GLC_GGUF_F16 1
 
 /* wire precision modes (WirePrecisionMode, Protocol/FusedActivationHeader.cs:12-18) */
 #define GLC_WIRE_FP32 0
@@ -254,6 +257,109 @@ int glc_attn_workspace_bytes(int32_t n_heads, int32_t n_kv_heads, int32_t max_le
 int glc_attn_decode_dev(const float* q, const float* k_new, const float* v_new, void* k_cache, void* v_cache,
                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_len, int32_t pos,
                         float rope_theta, float* out, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ---- paged fp16 K/V cache and the attention of a batch of sequences (the
+ *      attention half of IClusterStageModel.ForwardBatchStage,
+ *      IClusterStageModel.cs:24; the reference keeps one contiguous cache per
+ *      stage model and runs a batch's tokens one position after another).
+ *      A step: glc_kv_plan_dev gives the step's new tokens their pages,
+ *      glc_rope_append_dev rotates q and k and stores the new keys and values,
+ *      glc_attn_paged_dev attends over the pages (or glc_attn_prompt_dev over
+ *      packed keys and values of whole prompts).  Device pointers; no handle:
+ *      the calls run on the current device and the stream as given, allocate
+ *      nothing and can be captured into a graph (the first call on a device
+ *      looks up the error word's address: make it before a capture).  Pointers
+ *      of another device are refused.  Lengths live on the device; what
+ *      the host passes are row counts and bounds. ---- */
+
+/* Pages of one layer: row r of KV head h of page p is the 128 halves at
+ * k + p*page_stride + h*head_stride + r*row_stride (strides in elements,
+ * multiples of 8), so both [page][head][row][128] and [page][row][head][128]
+ * work, and k and v may share pages.  16-byte aligned. */
+typedef struct glc_kv_pages {
+    void* k;
+    void* v;
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t row_stride;
+    int32_t n_pages;
+    int32_t page_size;   /* rows of a page: 16, 32, 64, 128 or 256 */
+    int32_t n_kv_heads;
+    int32_t head_dim;    /* 128 */
+} glc_kv_pages;
+
+/* Page plan of a step.  Request i holds ctx_lens[i] cached tokens in the pages
+ * block_table[i][0 .. ceil(ctx/page_size)) and brings new_lens[i] new ones;
+ * new_lens[i] < 0: it is finished and its pages are pushed on the free list,
+ * in request order.  Then, in request order, each request takes the pages its
+ * new tokens need from the end of the free list, which holds free_count pages
+ * (device word) of a room of `capacity`.  A request is served when its rows
+ * end within T, its pages fit max_pages, and the pages needed by it and the
+ * requests before it are there.  Outputs: its table entries; free_list and
+ * free_count_out; cu_new [B+1], the first row of each request's new tokens
+ * (clamped to T); kv_lens [B] = ctx + new, 0 for finished and unserved
+ * requests (attention gives those zero rows); positions and slots [T] of
+ * every new row (slot = page * page_size + row; slot -1, position 0 for the
+ * rows of unserved requests and behind the last one); status = requests not
+ * served.  kv_lens and free_count_out must not alias the inputs.  The same
+ * inputs give the same outputs again, so a step can be planned twice. */
+int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens, int32_t B, int32_t page_size,
+                    int32_t* block_table, int32_t max_pages, int32_t* free_list, int32_t capacity,
+                    const int32_t* free_count, int32_t* free_count_out, int32_t T, int32_t* cu_new,
+                    int32_t* kv_lens, int32_t* positions, int64_t* slots, int32_t* status, void* stream);
+
+/* RoPE (rotate-half pairs (i, i+64), frequencies theta^(-2i/128), angles in
+ * double) of T rows of queries and keys at positions[t], and the store of the
+ * rotated keys and the values as fp16 in their slots.  q [T] rows of
+ * n_heads x 128 q_stride elements apart, k and v rows of n_kv_heads x 128
+ * kv_stride apart (fp32, rows 16-byte aligned: a fused QKV row works).
+ * q_out [T][n_heads][128] in q_out_type (GLC_GGUF_F32 or GLC_GGUF_F16; may be
+ * q itself for dense fp32 rows; n_heads 0: keys and values only).  cache NULL:
+ * nothing is stored; slots < 0 are skipped, slots past the cache are skipped
+ * and recorded (glc_paged_poll_error).  k_out / v_out: the same fp16 rows
+ * packed [T][n_kv_heads][128], or NULL. */
+int glc_rope_append_dev(const float* q, int64_t q_stride, const float* k, const float* v, int64_t kv_stride,
+                        int32_t T, int32_t n_heads, int32_t n_kv_heads, const int32_t* positions,
+                        const int64_t* slots, float rope_theta, const glc_kv_pages* cache, void* q_out,
+                        int32_t q_out_type, void* k_out, void* v_out, void* stream);
+
+/* Causal attention over packed prompts: rows cu_seqlens[b] .. cu_seqlens[b+1]
+ * (device, ascending, within T) are sequence b; its query i sees its keys
+ * 0 .. i.  q, out: T rows of n_heads x 128 in q_type (GLC_GGUF_F32 or
+ * GLC_GGUF_F16), q_stride / out_stride elements apart; k, v: fp16 rows of
+ * n_kv_heads x 128, kv_stride apart.  out = softmax(scale q.K^T) V, query head
+ * h reading KV head h / (n_heads / n_kv_heads), at most 16 query heads per KV
+ * head; scale 0 means 1/sqrt(128).  Scores, softmax and sums in fp32; fp32
+ * queries and their softmax weights keep ~22 bits, fp16 queries' weights are
+ * rounded to fp16.  Rows behind the last sequence are not touched.  Values of
+ * a sequence's rows must be finite. */
+int glc_attn_prompt_dev(const void* q, int32_t q_type, int64_t q_stride, const void* k, const void* v,
+                        int64_t kv_stride, const int32_t* cu_seqlens, int32_t B, int32_t T, int32_t n_heads,
+                        int32_t n_kv_heads, int32_t head_dim, float scale, void* out, int64_t out_stride,
+                        void* stream);
+
+/* Attention of the new tokens of B sequences over a paged cache that already
+ * holds them (a chunk of a prompt, or one decode token): sequence b's n new
+ * rows are cu_new[b] .. cu_new[b+1], its cache holds kv_lens[b] rows in pages
+ * block_table[b][0 ..], and its query i sees keys j <= kv_len - n + i (a query
+ * that sees none gets zeros).  max_new: the most new tokens of any sequence.
+ * The rest as glc_attn_prompt_dev; rows of a page past kv_len are not read as
+ * numbers.  A page id outside the cache, a kv_len past the table or a sequence
+ * longer than max_new is recorded (glc_paged_poll_error) and that sequence's
+ * rows are unspecified.  workspace: glc_attn_paged_workspace_bytes device
+ * bytes, 16-byte aligned, any contents; calls that may overlap need their own. */
+int glc_attn_paged_workspace_bytes(int32_t n_heads, int32_t n_kv_heads, int32_t B, int32_t T, int32_t max_new,
+                                   uint64_t* bytes);
+int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_stride, const glc_kv_pages* cache,
+                       const int32_t* block_table, int32_t max_pages, const int32_t* cu_new, const int32_t* kv_lens,
+                       int32_t B, int32_t T, int32_t max_new, int32_t n_heads, float scale, void* out,
+                       int64_t out_stride, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Reads and clears the device error word of the paged entry points on the
+ * current device (synchronises the device): GLC_ERR_INVALID_ARG when a page
+ * id, slot or length on the device was out of range, GLC_ERR_TIMEOUT when a
+ * bounded device-side wait gave up, else GLC_OK. */
+int glc_paged_poll_error(void);
 
 /* ---- router alone (for tests and for callers that route elsewhere) ---- */
 int glc_router_topk_dev(const float* x, const float* router_w, int32_t T, int32_t D, int32_t E,
