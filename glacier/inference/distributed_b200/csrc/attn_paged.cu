@@ -41,6 +41,8 @@ constexpr int kRowThreads = (kRowWarps + 1) * 32;
 constexpr int kRows = 16;                      // query rows of a tile
 constexpr float kPShift = 10.f;                // exponentials are stored as 2^10 e^(s - m): see below
 
+constexpr float kMinFactor = 1.2e-38f;         // a factor of zero would turn a masked -inf into NaN
+
 // p = 2^(s - m) lies in [0, 1]; stored as 2^10 p its fp16 form stays normal down
 // to 2^-24 of the row's largest weight.  The factor cancels in o / l.
 
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             // largest value to [2^12, 2^13): the low halves stay normal far below it
             const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
             const float up = exp2f((float)max(-126, min(126, e)));
-            f[hh] = p.scale_log2 / up;
+            f[hh] = fmaxf(p.scale_log2 / up, kMinFactor);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
@@ -301,11 +303,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const uint32_t kb = smem_u32(S.ring[st][0]) + warp_off, vb = smem_u32(S.ring[st][1]) + warp_off;
         const int j0 = it * kTile + k0;                // first key of the warp's 16
         if (j0 < kv_end) {
-            float s[2][4];
+            float s[2][4], sl[2][4];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+                for (int e = 0; e < 4; ++e) s[t][e] = sl[t][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
                 uint32_t b[4];
@@ -314,9 +316,15 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 mma_f16(s[0], qh[ks], b[0], b[1]);
                 mma_f16(s[1], qh[ks], b[2], b[3]);
                 if constexpr (F32) {
-                    mma_f16(s[0], ql[ks], b[0], b[1]);
-                    mma_f16(s[1], ql[ks], b[2], b[3]);
+                    mma_f16(sl[0], ql[ks], b[0], b[1]);
+                    mma_f16(sl[1], ql[ks], b[2], b[3]);
                 }
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][e] += sl[t][e];
             }
             uint32_t ph[4], pl[4];
 #pragma unroll
@@ -369,11 +377,22 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                     b[2] &= k0m;
                     b[3] &= k1m;
                 }
-                mma_f16(o[2 * t], ph, b[0], b[1]);
-                mma_f16(o[2 * t + 1], ph, b[2], b[3]);
                 if constexpr (F32) {
-                    mma_f16(o[2 * t], pl, b[0], b[1]);
-                    mma_f16(o[2 * t + 1], pl, b[2], b[3]);
+                    // the tensor core cuts its sums: the 16 keys' products are
+                    // added to the running output by fp32 additions
+                    float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(a0, pl, b[0], b[1]);
+                    mma_f16(a1, pl, b[2], b[3]);
+                    mma_f16(a0, ph, b[0], b[1]);
+                    mma_f16(a1, ph, b[2], b[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[2 * t][e] += a0[e];
+                        o[2 * t + 1][e] += a1[e];
+                    }
+                } else {
+                    mma_f16(o[2 * t], ph, b[0], b[1]);
+                    mma_f16(o[2 * t + 1], ph, b[2], b[3]);
                 }
             }
         }
@@ -446,6 +465,500 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     }
 }
 
+// ------------------------------------------------- tensor-memory tiles (prompts)
+// attn_tiles_kernel: 256 query rows of one KV head per CTA, as two row tiles A
+// and B of 128 (floor(128 / G) tokens times their G heads) that share every K
+// and V tile of 128 keys.  Per key tile and row tile, with one thread of a warp
+// issuing for both:
+//   S = Q K^T   tcgen05.mma, Q and K from shared memory, S in tensor memory;
+//   P = 2^(S f - m)  one warpgroup per row tile, one row per thread: no
+//               exchange between threads; P overwrites S in tensor memory;
+//   PV          tcgen05.mma, P from tensor memory, V from shared memory, into a
+//               tile of its own that the row's thread adds to its fp32 output
+//               in registers: o = o 2^(m_old - m) + PV.
+// While one row tile's warpgroup works on its softmax the tensor core runs the
+// other's products.  Keeping o out of the tensor-memory accumulator costs a
+// 128-column read per tile, and keeps the rounding of the sum over the keys
+// that of fp32 additions: the tensor core's own accumulation cuts the sum at
+// every 16 keys, which over 32,000 keys costs fp32 queries a decimal digit.
+// fp32 queries: S and PV take two products each (halves of q and of p, low
+// halves first).  Warps 0-7: softmax; warp 8: TMA; warp 9: MMA issue.
+constexpr int kTcThreads = 12 * 32;
+constexpr int kTcRows = 128;
+constexpr uint32_t kTcCols = 512;        // S_A, S_B, PV_A, PV_B
+constexpr int kMaxStages = 5;
+
+struct TilesSmem {
+    float f[2][kTcRows];                  // score factor of each row
+    uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2], p_full[2], o_full[2], q_full, v_clean, drain;
+    uint32_t tmem;
+    int seq, tile, found;
+};
+
+template <bool F32>
+struct TilesLayout {
+    static constexpr int kQBytes = 2 * (F32 ? 2 : 1) * kTileBytes;   // [row tile][half of q][2 x 64 dims][128 rows]
+    static constexpr int kStages = F32 ? 3 : 5;
+    static constexpr int kBytes = kQBytes + kStages * kTileBytes + (int)sizeof(TilesSmem) + 1024;
+};
+
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_arrive(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]^T and D[tmem] (+)= A[tmem] B[smem], fp16 operands, fp32 accumulators
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// SWIZZLE_128B matrix descriptors.  K-major (Q, K: 64 dims a row of 128 bytes):
+// 8-row groups 1024 bytes apart.  MN-major (V: the dims run along a row, the
+// keys down the rows): 64-dim blocks 16 KB apart, 8-key groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | (((uint64_t)(kTileBytes / 2) >> 4) << 16) | ((1024ull >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);   // f32 += f16 x f16, M = N = 128
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);                                     // B MN-major
+
+#define TMEM_LD32(taddr, r)                                                                                        \
+    asm volatile(                                                                                                  \
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"         \
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                                     \
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),           \
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),     \
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),   \
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])    \
+        : "r"(taddr)                                                                                               \
+        : "memory")
+#define TMEM_ST16(taddr, r)                                                                                        \
+    asm volatile(                                                                                                  \
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"    \
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),       \
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])              \
+        : "memory")
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Like find_tile, counted from the batch's end: the last tiles of a sequence
+// see the most keys, so they start first and the short ones fill the gaps.
+__device__ __forceinline__ bool find_tile_back(const AttnBatch& p, int x, int& seq, int& tile) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int b0 = p.B - 1; b0 >= 0; b0 -= 32) {
+        const int b = b0 - lane;
+        int nt = 0;
+        if (b >= 0) {
+            int first, n;
+            seq_rows(p, b, first, n);
+            nt = (n + p.tokens_per_tile - 1) / p.tokens_per_tile;
+        }
+        int end = nt;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, end, off);
+            if (lane >= off) end += o;
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, before + end > x);
+        if (m) {
+            const int l = __ffs(m) - 1;
+            seq = b0 - l;
+            tile = before + __shfl_sync(0xffffffffu, end, l) - 1 - x;
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, end, 31);
+    }
+    return false;
+}
+
+// A row's 32 scores of one chunk, in log2 units before the maximum is taken off;
+// keys at or past lim count as -inf.
+template <bool MASK>
+__device__ __forceinline__ float masked(uint32_t s, int j, int lim) {
+    return MASK && j >= lim ? -INFINITY : __uint_as_float(s);
+}
+
+// Softmax of one row against one key tile.  Two passes over the scores in tensor
+// memory (a row's 128 scores next to its 128 outputs would not fit the
+// registers): the maximum, then the exponentials, whose fp16 form overwrites
+// the chunk it came from.  Returns the rescale of what came before.
+template <bool F32, bool MASK>
+__device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, float& m, float& l) {
+    uint32_t r[32];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        TMEM_LD32(trow + 32 * c, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, masked<MASK>(r[e], 32 * c + e, lim));
+    }
+    const float mn = fmaxf(m, mx * f);
+    const float mu = mn == -INFINITY ? 0.f : mn - kPShift;
+    const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+    m = mn;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        TMEM_LD32(trow + 32 * c, r);
+        tmem_wait_ld();
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+            const float a = ex2(fmaf(masked<MASK>(r[e], 32 * c + e, lim), f, -mu));
+            const float b = ex2(fmaf(masked<MASK>(r[e + 1], 32 * c + e + 1, lim), f, -mu));
+            sum[e & 2] += a;
+            sum[(e & 2) + 1] += b;
+            if constexpr (F32) split2(a, b, hi[e >> 1], lo[e >> 1]);
+            else hi[e >> 1] = pack2(a, b);
+        }
+        if constexpr (F32) {   // chunk c's columns: 16 of high halves, 16 of low halves
+            TMEM_ST16(trow + 32 * c, hi);
+            TMEM_ST16(trow + 32 * c + 16, lo);
+        } else {
+            TMEM_ST16(trow + 16 * c, hi);
+        }
+    }
+    l = fmaf(l, corr, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    return corr;
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attn_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                      const __grid_constant__ AttnBatch p) {
+    using L = TilesLayout<F32>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* qs = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint8_t* ring = qs + L::kQBytes;
+    TilesSmem& S = *reinterpret_cast<TilesSmem*>(ring + L::kStages * kTileBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = blockIdx.x % p.n_kv;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kStages; ++i) {
+            mbar_init(&S.kv_full[i], 1);
+            mbar_init(&S.kv_empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&S.s_full[t], 1);
+            mbar_init(&S.p_full[t], 4);
+            mbar_init(&S.o_full[t], 1);
+        }
+        mbar_init(&S.q_full, 8);
+        mbar_init(&S.v_clean, 1);
+        mbar_init(&S.drain, 1);
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        int seq = 0, tile = 0;
+        const bool ok = find_tile_back(p, blockIdx.x / p.n_kv, seq, tile);
+        if (lane == 0) {
+            S.seq = seq;
+            S.tile = tile;
+            S.found = ok;
+        }
+    }
+    __syncthreads();
+    if (!S.found) return;
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem)),
+                     "r"(kTcCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = S.tmem;
+
+    const int seq = S.seq, tpt = p.tokens_per_tile >> 1;   // tokens per row tile
+    int first, n;
+    seq_rows(p, seq, first, n);
+    const int tok0 = S.tile * p.tokens_per_tile;
+    int kv_len = n;
+    if (p.kv_lens) {
+        const long long room = (long long)p.max_pages << p.ps_log2;
+        kv_len = p.kv_lens[seq];
+        if ((kv_len < 0 || kv_len > room || n > p.max_new) && threadIdx.x == 0) atomicExch(p.err, kDevBadArg);
+        kv_len = kv_len < 0 ? 0 : (kv_len > room ? (int)room : kv_len);
+    }
+    // row tile t: tokens [tok0 + t tpt, +ntok[t]), keys [0, end[t])
+    int ntok[2], nt[2], kv_end = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        ntok[t] = max(0, min(tpt, n - tok0 - t * tpt));
+        const int end = ntok[t] ? max(0, min(kv_len, kv_len - n + tok0 + t * tpt + ntok[t])) : 0;
+        nt[t] = (end + kTile - 1) / kTile;
+        kv_end = max(kv_end, end);
+    }
+    const int ntiles = max(nt[0], nt[1]);
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) {
+            // --------------------------------------------------- K and V tiles
+            const int ps = 1 << p.ps_log2, nbox = kTile / p.box_rows, halves = nbox == 1 ? 1 : 2;
+            const int box = lane / halves, half = lane - box * halves;
+            bool ok = true;
+            int it = 0;
+            for (int j = 0; j < ntiles && ok; ++j) {
+                const int r0 = j * kTile + box * p.box_rows;
+                const bool mine = box < nbox && r0 < kv_end;
+                const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+                const uint32_t bytes = (uint32_t)(boxes * p.box_rows * (nbox == 1 ? 256 : 128));
+                int page = 0, row = first + r0;
+                if (mine && p.table) {
+                    page = p.table[(long long)seq * p.max_pages + (r0 >> p.ps_log2)];
+                    row = r0 & (ps - 1);
+                    if ((unsigned)page >= (unsigned)p.n_pages) {  // reads as zeros
+                        atomicExch(p.err, kDevBadArg);
+                        page = p.n_pages;
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m, ++it) {
+                    const int st = it % L::kStages;
+                    ok = mbar_wait_backoff(&S.kv_empty[st], ((uint32_t)(it / L::kStages) & 1u) ^ 1u, p.err,
+                                           kDevTimeoutEmpty, 32);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&S.kv_full[st], bytes);
+                    __syncwarp();
+                    uint8_t* dst = ring + st * kTileBytes;
+                    if (mine)
+                        tma_load_kv(dst + half * (kTileBytes / 2) + box * p.box_rows * 128, m ? &tv : &tk, half, row, g,
+                                    page, &S.kv_full[st]);
+                    __syncwarp();
+                    // values past the last key may be anything, NaN included: zeros
+                    // before the tensor core reads them
+                    if (m == 1 && j == ntiles - 1 && kv_end < (j + 1) * kTile) {
+                        ok = mbar_wait(&S.kv_full[st], (uint32_t)(it / L::kStages) & 1u, p.err, kDevTimeoutFull);
+                        for (int r = kv_end - j * kTile + (lane >> 3); r < kTile; r += 4)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                *reinterpret_cast<uint4*>(dst + h * (kTileBytes / 2) + r * 128 + (lane & 7) * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&S.v_clean);
+                    }
+                }
+            }
+            if (lane == 0) drain_issued_stages(S.kv_full, L::kStages, it, kWaitLimitNs);
+        } else if (warp == 9 && lane == 0 && ntiles > 0) {
+            // ------------------------------------------------------------- MMA
+            auto wait_kv = [&](int it) {
+                return mbar_wait(&S.kv_full[it % L::kStages], (uint32_t)(it / L::kStages) & 1u, p.err, kDevTimeoutFull);
+            };
+            auto qk = [&](int t, int it) {   // S_t = Q_t K^T
+                const uint32_t kb = smem_u32(ring + (it % L::kStages) * kTileBytes);
+                const uint32_t qb = smem_u32(qs + t * (F32 ? 2 : 1) * kTileBytes);
+#pragma unroll
+                for (int part = F32 ? 1 : 0; part >= 0; --part)
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t off = (uint32_t)(ks >> 2) * (kTileBytes / 2) + (uint32_t)(ks & 3) * 32u;
+                        mma_ss(tmem + 128u * t, desc_k(qb + part * kTileBytes + off), desc_k(kb + off), kIdescS,
+                               (ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
+                    }
+                tc_arrive(&S.s_full[t]);
+            };
+            auto pv = [&](int t, int it) {   // PV_t = P_t V
+                const uint32_t vb = smem_u32(ring + (it % L::kStages) * kTileBytes);
+#pragma unroll
+                for (int part = F32 ? 1 : 0; part >= 0; --part)
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t col = F32 ? 32u * (ks >> 1) + 8u * (ks & 1) + 16u * part : 8u * ks;
+                        mma_ts(tmem + 256u + 128u * t, tmem + 128u * t + col, desc_mn(vb + (uint32_t)ks * 2048u), kIdescO,
+                               (ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
+                    }
+                tc_arrive(&S.o_full[t]);
+            };
+            bool ok = mbar_wait(&S.q_full, 0, p.err, kDevTimeoutFull) && wait_kv(0);
+            tc_after();
+            if (ok) {
+                for (int t = 0; t < 2; ++t)
+                    if (nt[t] > 0) qk(t, 0);
+                tc_arrive(&S.kv_empty[0]);
+            }
+            for (int j = 0; j < ntiles && ok; ++j) {
+                const int iv = 2 * j + 1, ik = 2 * j + 2;
+                ok = wait_kv(iv);
+                if (ok && j == ntiles - 1 && kv_end < ntiles * kTile) ok = mbar_wait(&S.v_clean, 0, p.err, kDevTimeoutFull);
+                if (ok && j + 1 < ntiles) ok = wait_kv(ik);
+                for (int t = 0; t < 2 && ok; ++t) {
+                    if (j >= nt[t]) continue;
+                    ok = mbar_wait(&S.p_full[t], (uint32_t)j & 1u, p.err, kDevTimeoutFull);
+                    if (!ok) break;
+                    tc_after();
+                    pv(t, iv);
+                    if (j + 1 < nt[t]) qk(t, ik);
+                }
+                if (!ok) break;
+                tc_arrive(&S.kv_empty[iv % L::kStages]);
+                if (j + 1 < ntiles) tc_arrive(&S.kv_empty[ik % L::kStages]);
+            }
+            // every product is done before the CTA frees its tensor memory
+            tc_arrive(&S.drain);
+            mbar_wait(&S.drain, 0, nullptr, 0, kWaitLimitNs);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int t = warp >> 2, wrow = 32 * (warp & 3);
+        const int rows = ntok[t] * p.G;
+        // ------------------------------------------------------------- queries
+        // a warp's 32 rows to shared memory, 64 dims a 128-byte swizzled row
+        uint8_t* qt = qs + t * (F32 ? 2 : 1) * kTileBytes;
+        const int64_t tok_first = first + tok0 + t * tpt;
+        if constexpr (F32) {
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += 8) {
+                float4 a[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = wrow + r0 + i, tok = r / p.G, h = r - tok * p.G;
+                    a[i] = r < rows ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) +
+                                                                            (tok_first + tok) * p.q_stride +
+                                                                            (int64_t)(g * p.G + h) * kHd) +
+                                            lane)
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = wrow + r0 + i;
+                    float mx = fmaxf(fmaxf(fabsf(a[i].x), fabsf(a[i].y)), fmaxf(fabsf(a[i].z), fabsf(a[i].w)));
+#pragma unroll
+                    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                    const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
+                    const float up = exp2f((float)max(-126, min(126, e)));
+                    if (lane == 0) S.f[t][r] = fmaxf(p.scale_log2 / up, kMinFactor);
+                    uint2 hi, lo;
+                    split2(a[i].x * up, a[i].y * up, hi.x, lo.x);
+                    split2(a[i].z * up, a[i].w * up, hi.y, lo.y);
+                    const int c = lane >> 1;
+                    uint8_t* d = qt + (c >> 3) * (kTileBytes / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                    *reinterpret_cast<uint2*>(d) = hi;
+                    *reinterpret_cast<uint2*>(d + kTileBytes) = lo;
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                const int r = wrow + 2 * i + (lane >> 4), c = lane & 15, tok = r / p.G, h = r - tok * p.G;
+                uint4 a = make_uint4(0u, 0u, 0u, 0u);
+                if (r < rows)
+                    a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + (tok_first + tok) * p.q_stride +
+                                                             (int64_t)(g * p.G + h) * kHd) +
+                              c);
+                *reinterpret_cast<uint4*>(qt + (c >> 3) * (kTileBytes / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = a;
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.q_full);
+
+        // ------------------------------------------------------------- softmax
+        const int row = wrow + lane, tok = row / p.G;
+        const bool live = row < rows;
+        const int lim = live ? max(0, min(kv_len, kv_len - n + tok0 + t * tpt + tok + 1)) : 0;
+        const int lim0 = max(0, kv_len - n + tok0 + t * tpt + 1);   // keys the tile's first row sees
+        const float f = F32 ? S.f[t][row] : p.scale_log2;
+        const uint32_t trow = tmem + 128u * t + ((uint32_t)wrow << 16);
+        float o[kHd], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int d = 0; d < kHd; ++d) o[d] = 0.f;
+        bool ok = true;
+        for (int j = 0; j < nt[t] && ok; ++j) {
+            const uint32_t ph = (uint32_t)j & 1u;
+            ok = mbar_wait(&S.s_full[t], ph, p.err, kDevTimeoutFull);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_after();
+            const float corr = (j + 1) * kTile > lim0 ? softmax_row<F32, true>(trow, lim - j * kTile, f, m, l)
+                                                      : softmax_row<F32, false>(trow, 0, f, m, l);
+            tmem_wait_st();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.p_full[t]);
+            ok = mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_after();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t r[32];
+                TMEM_LD32(trow + 256u + 32 * c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[32 * c + e] = fmaf(o[32 * c + e], corr, __uint_as_float(r[e]));
+            }
+            tc_before();
+        }
+        if (live && ok) {
+            const float inv = lim > 0 ? 1.f / l : 0.f;
+            const int h = row - tok * p.G;
+            const int64_t off = (tok_first + tok) * p.out_stride + (int64_t)(g * p.G + h) * kHd;
+            if constexpr (F32) {
+                float* d = static_cast<float*>(p.out) + off;
+#pragma unroll
+                for (int e = 0; e < kHd; e += 4)
+                    *reinterpret_cast<float4*>(d + e) =
+                        lim > 0 ? make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+            } else {
+                __half* d = static_cast<__half*>(p.out) + off;
+#pragma unroll
+                for (int e = 0; e < kHd; e += 8) {
+                    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                    if (lim > 0) {
+                        u.x = pack2(o[e] * inv, o[e + 1] * inv);
+                        u.y = pack2(o[e + 2] * inv, o[e + 3] * inv);
+                        u.z = pack2(o[e + 4] * inv, o[e + 5] * inv);
+                        u.w = pack2(o[e + 6] * inv, o[e + 7] * inv);
+                    }
+                    *reinterpret_cast<uint4*>(d + e) = u;
+                }
+            }
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcCols) : "memory");
+    }
+}
+
+template <bool F32>
+int attn_tiles_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p, cudaStream_t st) {
+    p.tokens_per_tile = 2 * (kTcRows / p.G);
+    constexpr int smem = TilesLayout<F32>::kBytes;
+    static_assert(smem <= 232448, "shared memory of a CTA");
+    cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
+    const long long tiles = (long long)p.T / p.tokens_per_tile + std::min(p.B, p.T);
+    if (tiles * p.n_kv > 0x7fffffffLL) return paged_fail(GLC_ERR_UNSUPPORTED, "%d rows are too many for one call", p.T);
+    attn_tiles_kernel<F32><<<(unsigned)(tiles * p.n_kv), kTcThreads, smem, st>>>(tk, tv, p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
+    return GLC_OK;
+}
+
 int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, bool f32, cudaStream_t st) {
     const int smem = (int)sizeof(RowsSmemAll) + 1024;
     const void* fn = f32 ? (const void*)attn_rows_kernel<true> : (const void*)attn_rows_kernel<false>;
@@ -461,6 +974,16 @@ int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBat
     e = cudaGetLastError();
     if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
     return GLC_OK;
+}
+
+// Tiles where a sequence may have more rows of a KV head than one 16-row tile
+// holds, the row kernel where none has.
+bool takes_tiles(int G, int max_new) { return (long long)max_new * G > kRows; }
+
+int attn_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, bool f32, int max_new,
+                cudaStream_t st) {
+    if (!takes_tiles(p.G, max_new)) return attn_rows_launch(tk, tv, p, f32, st);
+    return f32 ? attn_tiles_launch<true>(tk, tv, p, st) : attn_tiles_launch<false>(tk, tv, p, st);
 }
 
 // What both attentions ask of their queries, outputs and heads.
@@ -525,7 +1048,7 @@ extern "C" int glc_attn_prompt_dev(const void* q, int32_t q_type, int64_t q_stri
     CUtensorMap tk, tv;
     if (int rc = glc::paged_tensor_map(&tk, k, T, kv_stride, n_kv_heads, 128, 1, kv_stride, p.box_rows, 2)) return rc;
     if (int rc = glc::paged_tensor_map(&tv, v, T, kv_stride, n_kv_heads, 128, 1, kv_stride, p.box_rows, 2)) return rc;
-    return glc::attn_rows_launch(tk, tv, p, q_type == GLC_GGUF_F32, (cudaStream_t)stream);
+    return glc::attn_launch(tk, tv, p, q_type == GLC_GGUF_F32, T, (cudaStream_t)stream);
 }
 
 extern "C" int glc_attn_paged_workspace_bytes(int32_t n_heads, int32_t n_kv_heads, int32_t B, int32_t T,
@@ -568,12 +1091,15 @@ extern "C" int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_strid
     p.n_pages = cache->n_pages;
     while ((1 << p.ps_log2) < cache->page_size) ++p.ps_log2;
     p.box_rows = std::min(cache->page_size, glc::kTile);
+    // a tile's K and V lie as two blocks of 64 dims: a box that covers part of the
+    // tile's keys is one block's, one that covers them all takes both
+    const int halves = glc::takes_tiles(p.G, max_new) && p.box_rows < glc::kTile ? 1 : 2;
     CUtensorMap tk, tv;
     if (int rc = glc::paged_tensor_map(&tk, cache->k, cache->page_size, cache->row_stride, cache->n_kv_heads,
-                                       cache->head_stride, cache->n_pages, cache->page_stride, p.box_rows, 2))
+                                       cache->head_stride, cache->n_pages, cache->page_stride, p.box_rows, halves))
         return rc;
     if (int rc = glc::paged_tensor_map(&tv, cache->v, cache->page_size, cache->row_stride, cache->n_kv_heads,
-                                       cache->head_stride, cache->n_pages, cache->page_stride, p.box_rows, 2))
+                                       cache->head_stride, cache->n_pages, cache->page_stride, p.box_rows, halves))
         return rc;
-    return glc::attn_rows_launch(tk, tv, p, q_type == GLC_GGUF_F32, (cudaStream_t)stream);
+    return glc::attn_launch(tk, tv, p, q_type == GLC_GGUF_F32, max_new, (cudaStream_t)stream);
 }
