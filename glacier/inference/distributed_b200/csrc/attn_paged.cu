@@ -89,6 +89,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// One instruction; the division's subroutine call costs the callers' registers.
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -490,7 +496,7 @@ constexpr int kMaxStages = 5;
 
 struct TilesSmem {
     float f[2][kTcRows];                  // score factor of each row
-    uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2], p_full[2], o_full[2], q_full, v_clean, drain;
+    uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2], p_full[2][2], o_full[2], q_full, v_clean, drain;
     uint32_t tmem;
     int seq, tile, found;
 };
@@ -508,28 +514,35 @@ __device__ __forceinline__ void tc_arrive(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
+// SWIZZLE_128B matrix descriptors, the low word only: start address and the
+// leading offset; kDescHi holds 1024 bytes between groups of 8 rows (or keys),
+// the version and the swizzle.  K-major (Q, K: 64 dims a row of 128 bytes) has
+// no leading offset; MN-major (V: the dims run along a row, the keys down the
+// rows) has 16 KB between its blocks of 64 dims.  The 64-bit descriptors are put
+// together inside the instruction's block: kept as values, the issuing thread's
+// 64 loop-invariant descriptors spilled to local memory (10x the kernel's time
+// with 227 KB of shared memory, which leaves no first-level cache).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) {
+    return ((addr >> 4) & 0x3FFFu) | (((uint32_t)(kTileBytes / 2) >> 4) << 16);
+}
 // D[tmem] (+)= A[smem] B[smem]^T and D[tmem] (+)= A[tmem] B[smem], fp16 operands, fp32 accumulators
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc),
+        "r"(kDescHi)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc),
+        "r"(kDescHi)
         : "memory");
-}
-// SWIZZLE_128B matrix descriptors.  K-major (Q, K: 64 dims a row of 128 bytes):
-// 8-row groups 1024 bytes apart.  MN-major (V: the dims run along a row, the
-// keys down the rows): 64-dim blocks 16 KB apart, 8-key groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | (((uint64_t)(kTileBytes / 2) >> 4) << 16) | ((1024ull >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
 }
 constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);   // f32 += f16 x f16, M = N = 128
 constexpr uint32_t kIdescO = kIdescS | (1u << 16);                                     // B MN-major
@@ -544,12 +557,23 @@ constexpr uint32_t kIdescO = kIdescS | (1u << 16);                              
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])    \
         : "r"(taddr)                                                                                               \
         : "memory")
+#define TMEM_LD16(taddr, r)                                                                                        \
+    asm volatile(                                                                                                  \
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"     \
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),           \
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])      \
+        : "r"(taddr)                                                                                               \
+        : "memory")
 #define TMEM_ST16(taddr, r)                                                                                        \
     asm volatile(                                                                                                  \
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"    \
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),       \
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])              \
         : "memory")
+#define TMEM_ST8(taddr, r)                                                                                         \
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),  \
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])                        \
+                 : "memory")
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -584,56 +608,199 @@ __device__ __forceinline__ bool find_tile_back(const AttnBatch& p, int x, int& s
     return false;
 }
 
-// A row's 32 scores of one chunk, in log2 units before the maximum is taken off;
-// keys at or past lim count as -inf.
-template <bool MASK>
-__device__ __forceinline__ float masked(uint32_t s, int j, int lim) {
-    return MASK && j >= lim ? -INFINITY : __uint_as_float(s);
+// Pairs of fp32 values in one 64-bit register: half the issue slots of scalar
+// arithmetic.  Volatile on purpose: the compiler otherwise sinks a chunk's
+// arithmetic below the next chunk's tensor-memory load, keeps several chunks
+// alive next to the row's 128 outputs, and spills.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+    return d;
+}
+// o = o * c + (a, b)
+__device__ __forceinline__ void fma_pair(uint64_t& o, uint64_t c, uint32_t a, uint32_t b) {
+    asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, %0, %3, t;\n\t}"
+                 : "+l"(o)
+                 : "r"(a), "r"(b), "l"(c));
+}
+__device__ __forceinline__ void mul_pair(uint32_t& a, uint32_t& b, uint64_t c) {
+    asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tmul.rn.f32x2 t, t, %2;\n\tmov.b64 {%0, %1}, t;\n\t}"
+                 : "+r"(a), "+r"(b)
+                 : "l"(c));
+}
+// 16 bytes of output: the pairs times c
+__device__ __forceinline__ void store_f32(uint4* d, uint64_t a, uint64_t b, uint64_t c) {
+    asm volatile(
+        "{\n\t.reg .b64 t, u;\n\tmul.rn.f32x2 t, %1, %3;\n\tmul.rn.f32x2 u, %2, %3;\n\tst.global.v2.b64 [%0], {t, u};\n\t}" ::
+            "l"(d),
+        "l"(a), "l"(b), "l"(c)
+        : "memory");
+}
+// 2^((a, b) * f - mu)
+__device__ __forceinline__ void exp_pair(uint32_t a, uint32_t b, uint64_t f, uint64_t mu, float& x, float& y) {
+    asm volatile(
+        "{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tfma.rn.f32x2 t, t, %4, %5;\n\tmov.b64 {%0, %1}, t;\n\t"
+        "ex2.approx.ftz.f32 %0, %0;\n\tex2.approx.ftz.f32 %1, %1;\n\t}"
+        : "=f"(x), "=f"(y)
+        : "r"(a), "r"(b), "l"(f), "l"(mu));
+}
+__device__ __forceinline__ void add_pair(uint64_t& s, float a, float b) {
+    asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(s) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void max3(float& m, uint32_t a, uint32_t b) {
+    asm volatile("max.f32 %0, %0, %1, %2;" : "+f"(m) : "r"(a), "r"(b));
 }
 
-// Softmax of one row against one key tile.  Two passes over the scores in tensor
-// memory (a row's 128 scores next to its 128 outputs would not fit the
-// registers): the maximum, then the exponentials, whose fp16 form overwrites
-// the chunk it came from.  Returns the rescale of what came before.
-template <bool F32, bool MASK>
-__device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, float& m, float& l) {
-    uint32_t r[32];
-    float mx = -INFINITY;
+// 16 scores of a row: MASK takes keys at or past lim out
+template <bool MASK>
+__device__ __forceinline__ void mask16(uint32_t (&r)[16], int lim) {
+    if (MASK) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        TMEM_LD32(trow + 32 * c, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, masked<MASK>(r[e], 32 * c + e, lim));
+        for (int e = 0; e < 16; ++e)
+            if (e >= lim) r[e] = 0xff800000u;
     }
-    const float mn = fmaxf(m, mx * f);
+}
+__device__ __forceinline__ void max16(const uint32_t (&r)[16], float& m0, float& m1) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+        max3(m0, r[e], r[e + 1]);
+        max3(m1, r[e + 2], r[e + 3]);
+    }
+}
+// The weights of 16 scores over the scores' columns: 8 columns of high halves,
+// then 8 of low halves
+__device__ __forceinline__ void exp16(const uint32_t (&r)[16], uint32_t col, uint64_t f, uint64_t mu, uint64_t& s0,
+                                      uint64_t& s1) {
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        float a, b;
+        exp_pair(r[e], r[e + 1], f, mu, a, b);
+        add_pair((e & 2) ? s1 : s0, a, b);
+        split2(a, b, hi[e >> 1], lo[e >> 1]);
+    }
+    TMEM_ST8(col, hi);
+    TMEM_ST8(col + 8, lo);
+}
+
+// One arrival per warp: its rows' weights of 64 keys are in tensor memory.
+__device__ __forceinline__ void weights_ready(uint64_t* bar) {
+    tmem_wait_st();
+    tc_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// fp32 queries: softmax of one row against one key tile.  Two passes over the
+// scores in tensor memory (a row's 128 scores next to its 128 outputs would not
+// fit the registers): the maximum, then the exponentials.  Both loop over 32
+// scores as two loads of 16, the next in flight while one is worked on, and stay
+// rolled: unrolled, all the loads move to the top and their values spill.  MASK:
+// keys at or past lim count as -inf.  Returns the rescale of what came before.
+template <bool MASK>
+__device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, float& m, float& l, uint64_t* p_full) {
+    uint32_t a[16], b[16];
+    float mx0 = -INFINITY, mx1 = -INFINITY;
+    TMEM_LD16(trow, a);
+    tmem_wait_ld();
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        TMEM_LD16(trow + 32 * c + 16, b);
+        mask16<MASK>(a, lim - 32 * c);
+        max16(a, mx0, mx1);
+        tmem_wait_ld();
+        TMEM_LD16(trow + ((32 * c + 32) & 127), a);   // after the last chunk: the first again, for the second pass
+        mask16<MASK>(b, lim - 32 * c - 16);
+        max16(b, mx0, mx1);
+        tmem_wait_ld();
+    }
+    const float mn = fmaxf(m, fmaxf(mx0, mx1) * f);
     const float mu = mn == -INFINITY ? 0.f : mn - kPShift;
     const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
     m = mn;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+    const uint64_t f2 = pair(f, f), mu2 = pair(-mu, -mu);
+    uint64_t s0 = 0, s1 = 0;
+#pragma unroll 1
     for (int c = 0; c < 4; ++c) {
-        TMEM_LD32(trow + 32 * c, r);
+        TMEM_LD16(trow + 32 * c + 16, b);
+        mask16<MASK>(a, lim - 32 * c);
+        exp16(a, trow + 32 * c, f2, mu2, s0, s1);
         tmem_wait_ld();
-        uint32_t hi[16], lo[16];
+        if (c < 3) TMEM_LD16(trow + 32 * c + 32, a);
+        mask16<MASK>(b, lim - 32 * c - 16);
+        exp16(b, trow + 32 * c + 16, f2, mu2, s0, s1);
+        tmem_wait_ld();
+        if (c & 1) weights_ready(p_full + (c >> 1));
+    }
+    const float2 u = unpair(s0), v = unpair(s1);
+    l = fmaf(l, corr, (u.x + u.y) + (v.x + v.y));
+    return corr;
+}
+
+// fp16 queries: the row's 128 scores in registers, its outputs in tensor memory.
+// The maximum in use may lag the row's by kLazy before the outputs are rescaled
+// (the weights then reach 2^(kPShift + kLazy), inside fp16): after the first
+// tiles that hardly happens.
+constexpr float kLazy = 5.f;
+template <bool MASK>
+__device__ __forceinline__ void softmax_row_f16(uint32_t trow, int lim, float f, bool first, float& m, float& l,
+                                                uint64_t* p_full) {
+    uint32_t s[kTile];
+    TMEM_LD32(trow, s);
+    TMEM_LD32(trow + 32, (s + 32));
+    TMEM_LD32(trow + 64, (s + 64));
+    TMEM_LD32(trow + 96, (s + 96));
+    tmem_wait_ld();
+    if (MASK) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-            const float a = ex2(fmaf(masked<MASK>(r[e], 32 * c + e, lim), f, -mu));
-            const float b = ex2(fmaf(masked<MASK>(r[e + 1], 32 * c + e + 1, lim), f, -mu));
-            sum[e & 2] += a;
-            sum[(e & 2) + 1] += b;
-            if constexpr (F32) split2(a, b, hi[e >> 1], lo[e >> 1]);
-            else hi[e >> 1] = pack2(a, b);
-        }
-        if constexpr (F32) {   // chunk c's columns: 16 of high halves, 16 of low halves
-            TMEM_ST16(trow + 32 * c, hi);
-            TMEM_ST16(trow + 32 * c + 16, lo);
-        } else {
-            TMEM_ST16(trow + 16 * c, hi);
+        for (int e = 0; e < kTile; ++e)
+            if (e >= lim) s[e] = 0xff800000u;
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < kTile; e += 2) max3(mx[(e >> 1) & 3], s[e], s[e + 1]);
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+    if (__any_sync(0xffffffffu, top > m + kLazy)) {
+        const float mn = fmaxf(m, top);
+        const float corr = mn == -INFINITY ? 1.f : ex2(m - mn);
+        m = mn;
+        l *= corr;
+        if (!first) {   // S of this tile is there, so the product before it is done
+            const uint64_t corr2 = pair(corr, corr);
+#pragma unroll 1
+            for (int c = 0; c < kHd; c += 16) {
+                uint32_t r[16];
+                TMEM_LD16(trow + 256u + c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) mul_pair(r[e], r[e + 1], corr2);
+                TMEM_ST16(trow + 256u + c, r);
+            }
         }
     }
-    l = fmaf(l, corr, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-    return corr;
+    const float mu = m == -INFINITY ? 0.f : m - kPShift;
+    const uint64_t f2 = pair(f, f), mu2 = pair(-mu, -mu);
+    uint64_t s0 = 0, s1 = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+            float a, b;
+            exp_pair(s[32 * c + e], s[32 * c + e + 1], f2, mu2, a, b);
+            add_pair((e & 2) ? s1 : s0, a, b);
+            w[e >> 1] = pack2(a, b);
+        }
+        TMEM_ST16(trow + 16 * c, w);
+        if (c & 1) weights_ready(p_full + (c >> 1));
+    }
+    const float2 u = unpair(s0), v = unpair(s1);
+    l += (u.x + u.y) + (v.x + v.y);
 }
 
 template <bool F32>
@@ -655,7 +822,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&S.s_full[t], 1);
-            mbar_init(&S.p_full[t], 4);
+            mbar_init(&S.p_full[t][0], 4);
+            mbar_init(&S.p_full[t][1], 4);
             mbar_init(&S.o_full[t], 1);
         }
         mbar_init(&S.q_full, 8);
@@ -708,7 +876,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int ntiles = max(nt[0], nt[1]);
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == 8) {
             // --------------------------------------------------- K and V tiles
             const int ps = 1 << p.ps_log2, nbox = kTile / p.box_rows, halves = nbox == 1 ? 1 : 2;
@@ -765,29 +933,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 return mbar_wait(&S.kv_full[it % L::kStages], (uint32_t)(it / L::kStages) & 1u, p.err, kDevTimeoutFull);
             };
             auto qk = [&](int t, int it) {   // S_t = Q_t K^T
-                const uint32_t kb = smem_u32(ring + (it % L::kStages) * kTileBytes);
-                const uint32_t qb = smem_u32(qs + t * (F32 ? 2 : 1) * kTileBytes);
+                const uint32_t kb = desc_k(smem_u32(ring + (it % L::kStages) * kTileBytes));
+                const uint32_t qb = desc_k(smem_u32(qs + t * (F32 ? 2 : 1) * kTileBytes));
 #pragma unroll
                 for (int part = F32 ? 1 : 0; part >= 0; --part)
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
-                        const uint32_t off = (uint32_t)(ks >> 2) * (kTileBytes / 2) + (uint32_t)(ks & 3) * 32u;
-                        mma_ss(tmem + 128u * t, desc_k(qb + part * kTileBytes + off), desc_k(kb + off), kIdescS,
+                        const uint32_t off = ((uint32_t)(ks >> 2) * (kTileBytes / 2) + (uint32_t)(ks & 3) * 32u) >> 4;
+                        mma_ss(tmem + 128u * t, qb + (uint32_t)(part * (kTileBytes >> 4)) + off, kb + off, kIdescS,
                                (ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
                     }
                 tc_arrive(&S.s_full[t]);
             };
-            auto pv = [&](int t, int it) {   // PV_t = P_t V
-                const uint32_t vb = smem_u32(ring + (it % L::kStages) * kTileBytes);
+            auto pv = [&](int t, int it, int half, bool fresh) {   // PV_t (+)= P_t V over 64 of the tile's keys
+                const uint32_t vb = desc_mn(smem_u32(ring + (it % L::kStages) * kTileBytes)) + (uint32_t)half * (8192u >> 4);
 #pragma unroll
                 for (int part = F32 ? 1 : 0; part >= 0; --part)
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint32_t col = F32 ? 32u * (ks >> 1) + 8u * (ks & 1) + 16u * part : 8u * ks;
-                        mma_ts(tmem + 256u + 128u * t, tmem + 128u * t + col, desc_mn(vb + (uint32_t)ks * 2048u), kIdescO,
-                               (ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint32_t col = (uint32_t)(4 * half + ks) * (F32 ? 16u : 8u) + 8u * part;
+                        mma_ts(tmem + 256u + 128u * t, tmem + 128u * t + col, vb + (uint32_t)ks * (2048u >> 4), kIdescO,
+                               (fresh && ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
                     }
-                tc_arrive(&S.o_full[t]);
             };
             bool ok = mbar_wait(&S.q_full, 0, p.err, kDevTimeoutFull) && wait_kv(0);
             tc_after();
@@ -803,10 +970,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (ok && j + 1 < ntiles) ok = wait_kv(ik);
                 for (int t = 0; t < 2 && ok; ++t) {
                     if (j >= nt[t]) continue;
-                    ok = mbar_wait(&S.p_full[t], (uint32_t)j & 1u, p.err, kDevTimeoutFull);
+                    for (int half = 0; half < 2 && ok; ++half) {
+                        ok = mbar_wait(&S.p_full[t][half], (uint32_t)j & 1u, p.err, kDevTimeoutFull);
+                        if (!ok) break;
+                        tc_after();
+                        pv(t, iv, half, half == 0 && (F32 || j == 0));
+                    }
                     if (!ok) break;
-                    tc_after();
-                    pv(t, iv);
+                    if (F32 || j + 1 == nt[t]) tc_arrive(&S.o_full[t]);
                     if (j + 1 < nt[t]) qk(t, ik);
                 }
                 if (!ok) break;
@@ -818,7 +989,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_wait(&S.drain, 0, nullptr, 0, kWaitLimitNs);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int t = warp >> 2, wrow = 32 * (warp & 3);
         const int rows = ntok[t] * p.G;
         // ------------------------------------------------------------- queries
@@ -879,59 +1050,85 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int lim0 = max(0, kv_len - n + tok0 + t * tpt + 1);   // keys the tile's first row sees
         const float f = F32 ? S.f[t][row] : p.scale_log2;
         const uint32_t trow = tmem + 128u * t + ((uint32_t)wrow << 16);
-        float o[kHd], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int d = 0; d < kHd; ++d) o[d] = 0.f;
+        const int64_t out_off = (tok_first + tok) * p.out_stride + (int64_t)(g * p.G + row - tok * p.G) * kHd;
+        float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = 0; j < nt[t] && ok; ++j) {
-            const uint32_t ph = (uint32_t)j & 1u;
-            ok = mbar_wait(&S.s_full[t], ph, p.err, kDevTimeoutFull);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_after();
-            const float corr = (j + 1) * kTile > lim0 ? softmax_row<F32, true>(trow, lim - j * kTile, f, m, l)
-                                                      : softmax_row<F32, false>(trow, 0, f, m, l);
-            tmem_wait_st();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&S.p_full[t]);
-            ok = mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_after();
+        if constexpr (F32) {
+            uint64_t o[kHd / 2];   // the row's outputs in pairs
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t r[32];
-                TMEM_LD32(trow + 256u + 32 * c, r);
-                tmem_wait_ld();
+            for (int d = 0; d < kHd / 2; ++d) o[d] = 0;
+            for (int j = 0; j < nt[t]; ++j) {
+                const uint32_t ph = (uint32_t)j & 1u;
+                ok = mbar_wait(&S.s_full[t], ph, p.err, kDevTimeoutFull);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_after();
+                const float corr = (j + 1) * kTile > lim0 ? softmax_row<true>(trow, lim - j * kTile, f, m, l, S.p_full[t])
+                                                          : softmax_row<false>(trow, 0, f, m, l, S.p_full[t]);
+                ok = mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_after();
+                const uint64_t corr2 = pair(corr, corr);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[32 * c + e] = fmaf(o[32 * c + e], corr, __uint_as_float(r[e]));
+                for (int c = 0; c < 4; ++c) {
+                    // the barrier once more: a branch that keeps the later loads from
+                    // moving to the top, where their values would spill
+                    if (c == 2 && !mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull)) ok = false;
+                    uint32_t r[32];
+                    TMEM_LD32(trow + 256u + 32 * c, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) fma_pair(o[16 * c + e], corr2, r[2 * e], r[2 * e + 1]);
+                }
+                tc_before();
             }
-            tc_before();
-        }
-        if (live && ok) {
-            const float inv = lim > 0 ? 1.f / l : 0.f;
-            const int h = row - tok * p.G;
-            const int64_t off = (tok_first + tok) * p.out_stride + (int64_t)(g * p.G + h) * kHd;
-            if constexpr (F32) {
-                float* d = static_cast<float*>(p.out) + off;
+            if (live && ok) {
+                uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + out_off);
+                if (lim > 0) {
+                    const float rl = rcp(l);
+                    const uint64_t inv = pair(rl, rl);
 #pragma unroll
-                for (int e = 0; e < kHd; e += 4)
-                    *reinterpret_cast<float4*>(d + e) =
-                        lim > 0 ? make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
-            } else {
-                __half* d = static_cast<__half*>(p.out) + off;
+                    for (int e = 0; e < kHd / 2; e += 2) store_f32(d + e / 2, o[e], o[e + 1], inv);
+                } else {   // no key seen
 #pragma unroll
-                for (int e = 0; e < kHd; e += 8) {
-                    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                    if (lim > 0) {
-                        u.x = pack2(o[e] * inv, o[e + 1] * inv);
-                        u.y = pack2(o[e + 2] * inv, o[e + 3] * inv);
-                        u.z = pack2(o[e + 4] * inv, o[e + 5] * inv);
-                        u.w = pack2(o[e + 6] * inv, o[e + 7] * inv);
+                    for (int e = 0; e < kHd / 4; ++e) d[e] = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+        } else {
+            for (int j = 0; j < nt[t]; ++j) {
+                ok = mbar_wait(&S.s_full[t], (uint32_t)j & 1u, p.err, kDevTimeoutFull);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_after();
+                if ((j + 1) * kTile > lim0) softmax_row_f16<true>(trow, lim - j * kTile, f, j == 0, m, l, S.p_full[t]);
+                else softmax_row_f16<false>(trow, 0, f, j == 0, m, l, S.p_full[t]);
+            }
+            if (ok && nt[t] > 0) {
+                ok = mbar_wait(&S.o_full[t], 0, p.err, kDevTimeoutFull);
+                ok = __all_sync(0xffffffffu, ok);
+                tc_after();
+            }
+            if (ok) {
+                const float rl = rcp(l);
+                uint4* d = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + out_off);
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    if (nt[t] > 0) TMEM_LD32(trow + 256u + 32 * c, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                        if (lim > 0) {
+                            u.x = pack2(__uint_as_float(r[e]) * rl, __uint_as_float(r[e + 1]) * rl);
+                            u.y = pack2(__uint_as_float(r[e + 2]) * rl, __uint_as_float(r[e + 3]) * rl);
+                            u.z = pack2(__uint_as_float(r[e + 4]) * rl, __uint_as_float(r[e + 5]) * rl);
+                            u.w = pack2(__uint_as_float(r[e + 6]) * rl, __uint_as_float(r[e + 7]) * rl);
+                        }
+                        if (live) d[4 * c + (e >> 3)] = u;
                     }
-                    *reinterpret_cast<uint4*>(d + e) = u;
+                    __syncwarp();
                 }
             }
         }
