@@ -474,8 +474,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 // ------------------------------------------------- tensor-memory tiles (prompts)
 // attn_tiles_kernel: 256 query rows of one KV head per CTA, as two row tiles A
 // and B of 128 (floor(128 / G) tokens times their G heads) that share every K
-// and V tile of 128 keys.  Per key tile and row tile, with one thread of a warp
-// issuing for both:
+// and V tile of 128 keys.  Per key tile and row tile:
 //   S = Q K^T   tcgen05.mma, Q and K from shared memory, S in tensor memory;
 //   P = 2^(S f - m)  one warpgroup per row tile, one row per thread: no
 //               exchange between threads; P overwrites S in tensor memory;
@@ -488,7 +487,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 // that of fp32 additions: the tensor core's own accumulation cuts the sum at
 // every 16 keys, which over 32,000 keys costs fp32 queries a decimal digit.
 // fp32 queries: S and PV take two products each (halves of q and of p, low
-// halves first).  Warps 0-7: softmax; warp 8: TMA; warp 9: MMA issue.
+// halves first).  Warps 0-7: softmax; warp 8: TMA; warps 9 and 10: MMA issue.
 constexpr int kTcThreads = 12 * 32;
 constexpr int kTcRows = 128;
 constexpr uint32_t kTcCols = 512;        // S_A, S_B, PV_A, PV_B
@@ -496,7 +495,8 @@ constexpr int kMaxStages = 5;
 
 struct TilesSmem {
     float f[2][kTcRows];                  // score factor of each row
-    uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2], p_full[2][2], o_full[2], q_full, v_clean, drain;
+    uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2], p_full[2][2], o_full[2], turn[2], q_full, v_clean,
+        drain[2];
     uint32_t tmem;
     int seq, tile, found;
 };
@@ -688,6 +688,24 @@ __device__ __forceinline__ void exp16(const uint32_t (&r)[16], uint32_t col, uin
     TMEM_ST8(col + 8, lo);
 }
 
+// The two warpgroups take turns at the exponentials: one row tile's run while the
+// other's products do.  Left alone the two fall into step, and the tensor core
+// and the exponential unit wait for each other (4.2k cycles a key tile against
+// 2.9k in turns, fp16 queries).  Warpgroup 0 starts; a turn is passed on before
+// the last quarter of the exponentials.
+struct Turn {
+    uint64_t *mine, *other;   // null: this tile has no partner
+    uint32_t phase;
+    bool wait;
+    int* err;
+    __device__ __forceinline__ bool take() const {
+        return !wait || mbar_wait(mine, phase, err, kDevTimeoutFull);
+    }
+    __device__ __forceinline__ void pass() const {
+        if (other && (threadIdx.x & 31) == 0) mbar_arrive(other);
+    }
+};
+
 // One arrival per warp: its rows' weights of 64 keys are in tensor memory.
 __device__ __forceinline__ void weights_ready(uint64_t* bar) {
     tmem_wait_st();
@@ -703,7 +721,8 @@ __device__ __forceinline__ void weights_ready(uint64_t* bar) {
 // rolled: unrolled, all the loads move to the top and their values spill.  MASK:
 // keys at or past lim count as -inf.  Returns the rescale of what came before.
 template <bool MASK>
-__device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, float& m, float& l, uint64_t* p_full) {
+__device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, float& m, float& l, uint64_t* p_full,
+                                             const Turn& turn, bool& ok) {
     uint32_t a[16], b[16];
     float mx0 = -INFINITY, mx1 = -INFINITY;
     TMEM_LD16(trow, a);
@@ -725,8 +744,10 @@ __device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, fl
     m = mn;
     const uint64_t f2 = pair(f, f), mu2 = pair(-mu, -mu);
     uint64_t s0 = 0, s1 = 0;
+    ok = turn.take();
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
+        if (c == 3) turn.pass();
         TMEM_LD16(trow + 32 * c + 16, b);
         mask16<MASK>(a, lim - 32 * c);
         exp16(a, trow + 32 * c, f2, mu2, s0, s1);
@@ -749,7 +770,7 @@ __device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, fl
 constexpr float kLazy = 5.f;
 template <bool MASK>
 __device__ __forceinline__ void softmax_row_f16(uint32_t trow, int lim, float f, bool first, float& m, float& l,
-                                                uint64_t* p_full) {
+                                                uint64_t* p_full, const Turn& turn, bool& ok) {
     uint32_t s[kTile];
     TMEM_LD32(trow, s);
     TMEM_LD32(trow + 32, (s + 32));
@@ -786,8 +807,10 @@ __device__ __forceinline__ void softmax_row_f16(uint32_t trow, int lim, float f,
     const float mu = m == -INFINITY ? 0.f : m - kPShift;
     const uint64_t f2 = pair(f, f), mu2 = pair(-mu, -mu);
     uint64_t s0 = 0, s1 = 0;
+    ok = turn.take();
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
+        if (c == 3) turn.pass();
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
@@ -818,17 +841,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(&S.kv_full[i], 1);
-            mbar_init(&S.kv_empty[i], 1);
+            mbar_init(&S.kv_empty[i], 2);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&S.s_full[t], 1);
             mbar_init(&S.p_full[t][0], 4);
             mbar_init(&S.p_full[t][1], 4);
             mbar_init(&S.o_full[t], 1);
+            mbar_init(&S.turn[t], 4);
         }
         mbar_init(&S.q_full, 8);
         mbar_init(&S.v_clean, 1);
-        mbar_init(&S.drain, 1);
+        mbar_init(&S.drain[0], 1);
+        mbar_init(&S.drain[1], 1);
         fence_mbar_init();
     }
     if (warp == 0) {
@@ -927,66 +952,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             }
             if (lane == 0) drain_issued_stages(S.kv_full, L::kStages, it, kWaitLimitNs);
-        } else if (warp == 9 && lane == 0 && ntiles > 0) {
+        } else if (warp <= 10 && lane == 0 && ntiles > 0) {
             // ------------------------------------------------------------- MMA
+            // One issuer per row tile: an issuing thread's waits queue behind its
+            // own products (~200 cycles each, measured), and the other issuer's
+            // products run meanwhile.
+            const int t = warp - 9;
+            const uint32_t qb = desc_k(smem_u32(qs + t * (F32 ? 2 : 1) * kTileBytes));
+            const uint32_t s_col = tmem + 128u * t, o_col = tmem + 256u + 128u * t;
             auto wait_kv = [&](int it) {
                 return mbar_wait(&S.kv_full[it % L::kStages], (uint32_t)(it / L::kStages) & 1u, p.err, kDevTimeoutFull);
             };
-            auto qk = [&](int t, int it) {   // S_t = Q_t K^T
+            auto qk = [&](int it) {   // S = Q K^T
                 const uint32_t kb = desc_k(smem_u32(ring + (it % L::kStages) * kTileBytes));
-                const uint32_t qb = desc_k(smem_u32(qs + t * (F32 ? 2 : 1) * kTileBytes));
 #pragma unroll
                 for (int part = F32 ? 1 : 0; part >= 0; --part)
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
                         const uint32_t off = ((uint32_t)(ks >> 2) * (kTileBytes / 2) + (uint32_t)(ks & 3) * 32u) >> 4;
-                        mma_ss(tmem + 128u * t, qb + (uint32_t)(part * (kTileBytes >> 4)) + off, kb + off, kIdescS,
+                        mma_ss(s_col, qb + (uint32_t)(part * (kTileBytes >> 4)) + off, kb + off, kIdescS,
                                (ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
                     }
                 tc_arrive(&S.s_full[t]);
             };
-            auto pv = [&](int t, int it, int half, bool fresh) {   // PV_t (+)= P_t V over 64 of the tile's keys
+            auto pv = [&](int it, int half, bool fresh) {   // PV (+)= P V over 64 of the tile's keys
                 const uint32_t vb = desc_mn(smem_u32(ring + (it % L::kStages) * kTileBytes)) + (uint32_t)half * (8192u >> 4);
 #pragma unroll
                 for (int part = F32 ? 1 : 0; part >= 0; --part)
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
                         const uint32_t col = (uint32_t)(4 * half + ks) * (F32 ? 16u : 8u) + 8u * part;
-                        mma_ts(tmem + 256u + 128u * t, tmem + 128u * t + col, vb + (uint32_t)ks * (2048u >> 4), kIdescO,
+                        mma_ts(o_col, s_col + col, vb + (uint32_t)ks * (2048u >> 4), kIdescO,
                                (fresh && ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
                     }
             };
+            const int mine = nt[t];
             bool ok = mbar_wait(&S.q_full, 0, p.err, kDevTimeoutFull) && wait_kv(0);
             tc_after();
             if (ok) {
-                for (int t = 0; t < 2; ++t)
-                    if (nt[t] > 0) qk(t, 0);
+                if (mine > 0) qk(0);
                 tc_arrive(&S.kv_empty[0]);
             }
             for (int j = 0; j < ntiles && ok; ++j) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2;
                 ok = wait_kv(iv);
                 if (ok && j == ntiles - 1 && kv_end < ntiles * kTile) ok = mbar_wait(&S.v_clean, 0, p.err, kDevTimeoutFull);
+                // the next keys too, while the weights are on their way
                 if (ok && j + 1 < ntiles) ok = wait_kv(ik);
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (j >= nt[t]) continue;
-                    for (int half = 0; half < 2 && ok; ++half) {
-                        ok = mbar_wait(&S.p_full[t][half], (uint32_t)j & 1u, p.err, kDevTimeoutFull);
+                if (j < mine) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        ok = ok && mbar_wait(&S.p_full[t][half], (uint32_t)j & 1u, p.err, kDevTimeoutFull);
                         if (!ok) break;
                         tc_after();
-                        pv(t, iv, half, half == 0 && (F32 || j == 0));
+                        pv(iv, half, half == 0 && (F32 || j == 0));
                     }
-                    if (!ok) break;
-                    if (F32 || j + 1 == nt[t]) tc_arrive(&S.o_full[t]);
-                    if (j + 1 < nt[t]) qk(t, ik);
+                    if (ok && (F32 || j + 1 == mine)) tc_arrive(&S.o_full[t]);
                 }
                 if (!ok) break;
+                if (j + 1 < mine) qk(ik);
                 tc_arrive(&S.kv_empty[iv % L::kStages]);
                 if (j + 1 < ntiles) tc_arrive(&S.kv_empty[ik % L::kStages]);
             }
             // every product is done before the CTA frees its tensor memory
-            tc_arrive(&S.drain);
-            mbar_wait(&S.drain, 0, nullptr, 0, kWaitLimitNs);
+            tc_arrive(&S.drain[t]);
+            mbar_wait(&S.drain[t], 0, nullptr, 0, kWaitLimitNs);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -998,10 +1028,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t tok_first = first + tok0 + t * tpt;
         if constexpr (F32) {
 #pragma unroll 1
-            for (int r0 = 0; r0 < 32; r0 += 8) {
-                float4 a[8];
+            for (int r0 = 0; r0 < 32; r0 += 16) {
+                float4 a[16];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 16; ++i) {
                     const int r = wrow + r0 + i, tok = r / p.G, h = r - tok * p.G;
                     a[i] = r < rows ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) +
                                                                             (tok_first + tok) * p.q_stride +
@@ -1010,7 +1040,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                     : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 16; ++i) {
                     const int r = wrow + r0 + i;
                     float mx = fmaxf(fmaxf(fabsf(a[i].x), fabsf(a[i].y)), fmaxf(fabsf(a[i].z), fabsf(a[i].w)));
 #pragma unroll
@@ -1028,15 +1058,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             }
         } else {
-#pragma unroll 4
+            const int c = lane & 15;
+            uint4 a[16];
+#pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int r = wrow + 2 * i + (lane >> 4), c = lane & 15, tok = r / p.G, h = r - tok * p.G;
-                uint4 a = make_uint4(0u, 0u, 0u, 0u);
+                const int r = wrow + 2 * i + (lane >> 4), tok = r / p.G, h = r - tok * p.G;
+                a[i] = make_uint4(0u, 0u, 0u, 0u);
                 if (r < rows)
-                    a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + (tok_first + tok) * p.q_stride +
-                                                             (int64_t)(g * p.G + h) * kHd) +
-                              c);
-                *reinterpret_cast<uint4*>(qt + (c >> 3) * (kTileBytes / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = a;
+                    a[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) +
+                                                                (tok_first + tok) * p.q_stride +
+                                                                (int64_t)(g * p.G + h) * kHd) +
+                                 c);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int r = wrow + 2 * i + (lane >> 4);
+                *reinterpret_cast<uint4*>(qt + (c >> 3) * (kTileBytes / 2) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = a[i];
             }
         }
         fence_proxy_async_smem();
@@ -1053,6 +1090,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t out_off = (tok_first + tok) * p.out_stride + (int64_t)(g * p.G + row - tok * p.G) * kHd;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
+        const int both = min(nt[0], nt[1]);
+        auto turn_of = [&](int j) {   // warpgroup 0 waits for 1's turn at the tile before, 1 for 0's at this one
+            return Turn{&S.turn[t], j < both ? &S.turn[t ^ 1] : nullptr, (uint32_t)(j - 1 + t) & 1u,
+                        j < both && j + t > 0, p.err};
+        };
         if constexpr (F32) {
             uint64_t o[kHd / 2];   // the row's outputs in pairs
 #pragma unroll
@@ -1063,9 +1105,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_after();
-                const float corr = (j + 1) * kTile > lim0 ? softmax_row<true>(trow, lim - j * kTile, f, m, l, S.p_full[t])
-                                                          : softmax_row<false>(trow, 0, f, m, l, S.p_full[t]);
-                ok = mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
+                const Turn turn = turn_of(j);
+                const float corr = (j + 1) * kTile > lim0
+                                       ? softmax_row<true>(trow, lim - j * kTile, f, m, l, S.p_full[t], turn, ok)
+                                       : softmax_row<false>(trow, 0, f, m, l, S.p_full[t], turn, ok);
+                ok = ok && mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_after();
@@ -1101,8 +1145,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_after();
-                if ((j + 1) * kTile > lim0) softmax_row_f16<true>(trow, lim - j * kTile, f, j == 0, m, l, S.p_full[t]);
-                else softmax_row_f16<false>(trow, 0, f, j == 0, m, l, S.p_full[t]);
+                const Turn turn = turn_of(j);
+                if ((j + 1) * kTile > lim0)
+                    softmax_row_f16<true>(trow, lim - j * kTile, f, j == 0, m, l, S.p_full[t], turn, ok);
+                else softmax_row_f16<false>(trow, 0, f, j == 0, m, l, S.p_full[t], turn, ok);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
             }
             if (ok && nt[t] > 0) {
                 ok = mbar_wait(&S.o_full[t], 0, p.err, kDevTimeoutFull);
