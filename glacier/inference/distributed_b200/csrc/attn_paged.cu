@@ -8,15 +8,17 @@
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j,  zero where no key is seen.
 // Query head h reads KV head h / G (G = n_heads / n_kv_heads).
 //
-// Row kernel (attn_rows_kernel): a tile is up to 16 query rows of one KV head --
-// floor(16 / G) tokens times their G heads -- so every K and V row is read once
-// for all the heads that share it.  Eight warps take 16 of a stage's 128 keys
-// each and keep their own running maximum, sum and output in registers (one
-// pass, no exchange between warps until the tile's end, where the eight
-// partials are merged in warp order); a ninth warp streams the pages with TMA
+// Two kernels, by the rows a sequence brings to a KV head (its new tokens times
+// their G heads): up to 16 take attn_rows_kernel, which lives by the bytes of K
+// and V; more take attn_tiles_kernel on 128-row tensor-memory tiles.
+//
+// attn_rows_kernel: up to 16 query rows of one KV head, so every K and V row is
+// read once for all the heads that share it.  Eight warps take 16 of a stage's
+// 128 keys each and keep their own running maximum, sum and output in registers
+// (one pass, no exchange between warps until a unit's end, where the eight
+// partials are joined in warp order); a ninth warp streams the pages with TMA
 // into a ring of three 64 KB stages.  Products run as mma.sync m16n8k16 with
-// fp32 accumulators: 16 rows cannot fill a 128-row tensor-memory tile, and at
-// these row counts the bytes of K and V bound the time.
+// fp32 accumulators: 16 rows cannot fill a 128-row tensor-memory tile.
 // fp32 queries are carried as two fp16 halves after a power-of-two scale per
 // row, and so are the exponentials (two products each, ~22 bits of q and p
 // against the fp16 cache values); fp16 queries take one product.
@@ -56,6 +58,7 @@ struct AttnBatch {
     int max_pages, ps_log2, n_pages, box_rows;
     int B, T, max_new, n_heads, n_kv, G, tokens_per_tile;
     float scale_log2;               // softmax scale times log2(e)
+    float* work;                    // partials
     int* err;
 };
 
@@ -113,49 +116,200 @@ __device__ __forceinline__ void seq_rows(const AttnBatch& p, int b, int& first, 
     n = min(max(p.cu[b + 1], first), p.T) - first;
 }
 
-// Sequence and tile of the x-th tile of the batch (called by one warp): the
-// tiles of a sequence are its tokens in runs of tokens_per_tile.
-__device__ __forceinline__ bool find_tile(const AttnBatch& p, int x, int& seq, int& tile) {
-    const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-        const int b = b0 + lane;
-        int nt = 0;
-        if (b < p.B) {
-            int first, n;
-            seq_rows(p, b, first, n);
-            nt = (n + p.tokens_per_tile - 1) / p.tokens_per_tile;
-        }
-        int end = nt;
+// One warp's 16 keys against the 16 query rows: scores, weights, outputs.
+template <bool F32>
+__device__ __forceinline__ void rows_step(uint32_t kb, uint32_t vb, int box_b, int lr, int lc, int vr, int vc, int gc,
+                                          int j0, int kv_len, const int (&lim)[2], const float (&f)[2],
+                                          const uint32_t (&qh)[8][4], const uint32_t (&ql)[F32 ? 8 : 1][4],
+                                          float (&o)[16][4], float (&m)[2], float (&l)[2]) {
+    float s[2][4], sl[2][4];
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, end, off);
-            if (lane >= off) end += o;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = sl[t][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+        uint32_t b[4];
+        const int c = 2 * (ks & 3) + lc;
+        ldsm4(kb + (ks >> 2) * box_b + lr * 128 + ((c ^ (lr & 7)) << 4), b);
+        mma_f16(s[0], qh[ks], b[0], b[1]);
+        mma_f16(s[1], qh[ks], b[2], b[3]);
+        if constexpr (F32) {
+            mma_f16(sl[0], ql[ks], b[0], b[1]);
+            mma_f16(sl[1], ql[ks], b[2], b[3]);
         }
-        const unsigned m = __ballot_sync(0xffffffffu, before + end > x);
-        if (m) {
-            const int l = __ffs(m) - 1;
-            seq = b0 + l;
-            tile = x - before - __shfl_sync(0xffffffffu, end - nt, l);
-            return true;
-        }
-        before += __shfl_sync(0xffffffffu, end, 31);
     }
-    return false;
+    if constexpr (F32) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] += sl[t][e];
+    }
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int j = j0 + 8 * (e >> 1) + 2 * gc + (e & 1);
+            v[e] = j < lim[hh] ? s[e >> 1][2 * hh + (e & 1)] * f[hh] : -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[hh], mx), mu = (mn == -INFINITY) ? 0.f : mn - kPShift;
+        if (mn > m[hh]) {
+            const float corr = ex2(m[hh] - mn);
+            l[hh] *= corr;
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                o[t][2 * hh] *= corr;
+                o[t][2 * hh + 1] *= corr;
+            }
+            m[hh] = mn;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ex2(v[e] - mu);
+        l[hh] += (v[0] + v[1]) + (v[2] + v[3]);
+        // P as an A fragment: register hh holds keys 2 gc, 2 gc + 1; register hh + 2 the same + 8
+        if constexpr (F32) {
+            split2(v[0], v[1], ph[hh], pl[hh]);
+            split2(v[2], v[3], ph[hh + 2], pl[hh + 2]);
+        } else {
+            ph[hh] = pack2(v[0], v[1]);
+            ph[hh + 2] = pack2(v[2], v[3]);
+        }
+    }
+    // values past the last key may be anything, NaN included: they count as zeros
+    const bool tail = j0 + 16 > kv_len;
+    const int left = kv_len - j0 - 2 * gc;     // keys left from this thread's first
+    const uint32_t k0m = (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
+    const uint32_t k1m = (left > 8 ? 0xffffu : 0u) | (left > 9 ? 0xffff0000u : 0u);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        uint32_t b[4];
+        const int c = 2 * (t & 3) + vc;
+        ldsm4_t(vb + (t >> 2) * box_b + vr * 128 + ((c ^ (vr & 7)) << 4), b);
+        if (tail) {
+            b[0] &= k0m;
+            b[1] &= k1m;
+            b[2] &= k0m;
+            b[3] &= k1m;
+        }
+        if constexpr (F32) {
+            // the tensor core cuts its sums: the 16 keys' products are
+            // added to the running output by fp32 additions
+            float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(a0, pl, b[0], b[1]);
+            mma_f16(a1, pl, b[2], b[3]);
+            mma_f16(a0, ph, b[0], b[1]);
+            mma_f16(a1, ph, b[2], b[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[2 * t][e] += a0[e];
+                o[2 * t + 1][e] += a1[e];
+            }
+        } else {
+            mma_f16(o[2 * t], ph, b[0], b[1]);
+            mma_f16(o[2 * t + 1], ph, b[2], b[3]);
+        }
+    }
 }
+
+// N outputs of a row from dimension off on, times inv (zeros where the row sees no key)
+template <bool F32, int N>
+__device__ __forceinline__ void rows_store(void* out, int64_t off, const float (&a)[N], float inv, bool none) {
+    if constexpr (F32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + off);
+#pragma unroll
+        for (int e = 0; e < N; e += 4)
+            d[e / 4] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                            : make_float4(a[e] * inv, a[e + 1] * inv, a[e + 2] * inv, a[e + 3] * inv);
+    } else {
+        uint4* d = reinterpret_cast<uint4*>(static_cast<__half*>(out) + off);
+#pragma unroll
+        for (int e = 0; e < N; e += 8)
+            d[e / 8] = none ? make_uint4(0u, 0u, 0u, 0u)
+                            : make_uint4(pack2(a[e] * inv, a[e + 1] * inv), pack2(a[e + 2] * inv, a[e + 3] * inv),
+                                         pack2(a[e + 4] * inv, a[e + 5] * inv), pack2(a[e + 6] * inv, a[e + 7] * inv));
+    }
+}
+
+// ------------------------------------------------------------ few rows (decode)
+// A unit is one KV head of one sequence; its keys come in tiles of 128.  The
+// tiles of all units, one unit after another, are cut into kRowCtas equal runs,
+// one CTA each: every SM streams the same number of bytes whatever the lengths.
+// A run holds whole units, which are finished in place, and at most two that it
+// shares with its neighbours; their partials (maximum, sum, unnormalised output)
+// go to the workspace, two places a CTA, and attn_rows_merge_kernel joins them in
+// key order.
+constexpr int kRowCtas = 148;
+
+struct RowsUnit {
+    int first, n, kv_len, tiles;
+};
+__device__ __forceinline__ RowsUnit rows_unit(const AttnBatch& p, int b) {
+    RowsUnit u;
+    seq_rows(p, b, u.first, u.n);
+    u.kv_len = u.n;
+    if (p.kv_lens) {
+        const long long room = (long long)p.max_pages << p.ps_log2;
+        u.kv_len = (int)min((long long)max(p.kv_lens[b], 0), room);
+    }
+    u.tiles = u.n > 0 ? (u.kv_len + kTile - 1) / kTile : 0;
+    return u;
+}
+
+// CTA that holds tile x of W: the last c with c * W / kRowCtas <= x.
+__device__ __forceinline__ int rows_cta(long long x, long long W) { return (int)(((x + 1) * kRowCtas - 1) / W); }
+
+// Sum over the CTA's `threads` first threads of two values (all of them call).
+__device__ __forceinline__ void sum2(long long& a, long long& b, long long (*buf)[2], int threads, int bar) {
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, off);
+        b += __shfl_xor_sync(0xffffffffu, b, off);
+    }
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+        buf[warp][0] = a;
+        buf[warp][1] = b;
+    }
+    named_bar_sync(bar, threads);
+    a = b = 0;
+    for (int w = 0; w < (threads >> 5); ++w) {
+        a += buf[w][0];
+        b += buf[w][1];
+    }
+}
+
+// A position in the flattened tiles, and how many are left of the CTA's run.
+struct RowsWalk {
+    int b, g, tile;
+    long long left;
+};
 
 struct RowsSmem {
     uint8_t ring[kStages][2][kTileBytes];
     float m[kRowWarps][kRows];
     float l[kRowWarps][kRows];
     uint64_t full[kStages], empty[kStages];
-    int seq, tile, found;
+    long long sums[kRowWarps][2];
+    RowsWalk start;
 };
 // the merge of a tile's partials: four warps' outputs at a time
 struct RowsSmemAll {
     RowsSmem s;
     float o[4][kRows][kHd];
 };
+
+constexpr size_t kRowsWorkBytes = (size_t)2 * kRowCtas * kRows * (kHd + 2) * sizeof(float);
+
+// Partials in the workspace: place 2c for a unit that began before CTA c's run,
+// 2c + 1 for one that goes on behind it.
+__device__ __forceinline__ float* part_out(const AttnBatch& p, int place) {
+    return p.work + (size_t)place * kRows * (kHd + 2);
+}
 
 template <bool F32>
 __global__ void __launch_bounds__(kRowThreads, 1)
@@ -165,8 +319,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     RowsSmemAll& A = *reinterpret_cast<RowsSmemAll*>(base);
     RowsSmem& S = A.s;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    grid_dep_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&S.full[i], 1);
@@ -174,301 +329,288 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         }
         fence_mbar_init();
     }
-    if (warp == 0) {
-        int seq = 0, tile = 0;
-        const bool ok = find_tile(p, blockIdx.x, seq, tile);
-        if (lane == 0) {
-            S.seq = seq;
-            S.tile = tile;
-            S.found = ok;
+    // where the CTA's run of tiles begins
+    if (warp < kRowWarps) {
+        long long total = 0, none = 0;
+        for (int b = threadIdx.x; b < p.B; b += kRowWarps * 32) total += rows_unit(p, b).tiles;
+        sum2(total, none, S.sums, kRowWarps * 32, 1);
+        const long long W = total * p.n_kv;
+        const long long x0 = W * blockIdx.x / kRowCtas, x1 = W * (blockIdx.x + 1) / kRowCtas;
+        if (threadIdx.x == 0) S.start.left = 0;
+        if (warp == 0 && x1 > x0) {
+            long long before = 0;   // tiles of the sequences before b0
+            for (int b0 = 0; b0 < p.B; b0 += 32) {
+                const int b = b0 + lane;
+                const long long t = b < p.B ? rows_unit(p, b).tiles : 0;
+                long long end = t;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const long long o = __shfl_up_sync(0xffffffffu, end, off);
+                    if (lane >= off) end += o;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, (before + end) * p.n_kv > x0);
+                if (hit) {
+                    if (lane == __ffs(hit) - 1) {
+                        const long long in = x0 - (before + end - t) * p.n_kv;
+                        S.start = RowsWalk{b, (int)(in / t), (int)(in % t), x1 - x0};
+                    }
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, end, 31);
+            }
         }
     }
     __syncthreads();
-    if (!S.found) return;
-    const int seq = S.seq, tok0 = S.tile * p.tokens_per_tile;
-    int first, n;
-    seq_rows(p, seq, first, n);
-    const int ntok = min(p.tokens_per_tile, n - tok0), rows = ntok * p.G;
-    int kv_len = n;
-    if (p.kv_lens) {
-        if (n > p.max_new && threadIdx.x == 0) atomicExch(p.err, kDevBadArg);
-        const long long room = (long long)p.max_pages << p.ps_log2;
-        kv_len = p.kv_lens[seq];
-        if (kv_len < 0 || kv_len > room) {
-            if (threadIdx.x == 0) atomicExch(p.err, kDevBadArg);
-            kv_len = kv_len < 0 ? 0 : (int)room;
-        }
-    }
-    const int see0 = kv_len - n + tok0 + 1;            // keys the tile's first token sees (may be <= 0)
-    const int kv_end = max(0, min(kv_len, see0 + ntok - 1));
-    const int ntiles = (kv_end + kTile - 1) / kTile;
+    RowsWalk w = S.start;
 
     if (warp == kRowWarps) {
         // ------------------------------------------------------- page stream
         const int nbox = kTile / p.box_rows, ps = 1 << p.ps_log2;
         bool ok = true;
         int it = 0;
-        for (; it < ntiles && ok; ++it) {
-            const int st = it % kStages;
-            ok = mbar_wait_backoff(&S.empty[st], ((uint32_t)(it / kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty, 32);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const int r0 = it * kTile + lane * p.box_rows;
-            const bool mine = lane < nbox && r0 < kv_end;
-            const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
-            if (lane == 0) mbar_arrive_expect_tx(&S.full[st], (uint32_t)(boxes * p.box_rows * kHd * 2 * 2));
-            int page = 0, row = first + r0;
-            if (mine && p.table) {
-                page = p.table[(long long)seq * p.max_pages + (r0 >> p.ps_log2)];
-                row = r0 & (ps - 1);
-                if ((unsigned)page >= (unsigned)p.n_pages) {  // reads as zeros
-                    atomicExch(p.err, kDevBadArg);
-                    page = p.n_pages;
+        while (w.left > 0 && ok) {
+            const RowsUnit u = rows_unit(p, w.b);
+            const int end = (int)min((long long)u.tiles, w.tile + w.left);
+            for (int j = w.tile; j < end; ++j, ++it) {
+                const int st = it % kStages;
+                const int r0 = j * kTile + lane * p.box_rows;
+                const bool mine = lane < nbox && r0 < u.kv_len;
+                const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+                int page = 0, row = u.first + r0;
+                if (mine && p.table) {
+                    page = p.table[(long long)w.b * p.max_pages + (r0 >> p.ps_log2)];
+                    row = r0 & (ps - 1);
+                    if ((unsigned)page >= (unsigned)p.n_pages) {  // reads as zeros
+                        atomicExch(p.err, kDevBadArg);
+                        page = p.n_pages;
+                    }
                 }
+                ok = mbar_wait_backoff(&S.empty[st], ((uint32_t)(it / kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty, 32);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&S.full[st], (uint32_t)(boxes * p.box_rows * kHd * 2 * 2));
+                __syncwarp();
+                if (mine) {
+                    tma_load_kv(S.ring[st][0] + lane * p.box_rows * kHd * 2, &tk, 0, row, w.g, page, &S.full[st]);
+                    tma_load_kv(S.ring[st][1] + lane * p.box_rows * kHd * 2, &tv, 0, row, w.g, page, &S.full[st]);
+                }
+                __syncwarp();
             }
-            __syncwarp();
-            if (mine) {
-                tma_load_kv(S.ring[st][0] + lane * p.box_rows * kHd * 2, &tk, 0, row, g, page, &S.full[st]);
-                tma_load_kv(S.ring[st][1] + lane * p.box_rows * kHd * 2, &tv, 0, row, g, page, &S.full[st]);
+            w.left -= end - w.tile;
+            w.tile = 0;
+            if (++w.g == p.n_kv) {
+                w.g = 0;
+                do ++w.b;
+                while (w.left > 0 && w.b < p.B && rows_unit(p, w.b).tiles == 0);
             }
-            __syncwarp();
         }
         if (lane == 0) drain_issued_stages(S.full, kStages, it, kWaitLimitNs);
-        __syncthreads();  // matches the consumers' first barrier of the merge
-        for (int i = 0; i < 4; ++i) __syncthreads();
         return;
     }
 
-    // ---------------------------------------------------------------- queries
-    // A fragments of the tile's 16 rows: thread (gr, gc) holds rows gr, gr + 8,
-    // columns 16 ks + 2 gc + {0, 1} and + 8
     const int gr = lane >> 2, gc = lane & 3;
-    uint32_t qh[8][4], ql[F32 ? 8 : 1][4];
-    float f[2];                                        // S row factor: scale * log2(e) * the row's power of two
-    int lim[2];                                        // keys seen by the thread's two rows
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-        const int r = gr + 8 * hh, tok = r / p.G, h = r - tok * p.G;
-        const bool live = r < rows;
-        lim[hh] = live ? max(0, min(kv_len, see0 + tok)) : 0;
-        f[hh] = p.scale_log2;
-        const int64_t off = (int64_t)(first + tok0 + tok) * p.q_stride + (int64_t)(g * p.G + h) * kHd + 2 * gc;
-        if constexpr (F32) {
-            float2 a[8][2];
-            float mx = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    a[ks][c] = live ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + off +
-                                                                            16 * ks + 8 * c))
-                                    : make_float2(0.f, 0.f);
-                    mx = fmaxf(mx, fmaxf(fabsf(a[ks][c].x), fabsf(a[ks][c].y)));
-                }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // largest value to [2^12, 2^13): the low halves stay normal far below it
-            const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
-            const float up = exp2f((float)max(-126, min(126, e)));
-            f[hh] = fmaxf(p.scale_log2 / up, kMinFactor);
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    split2(a[ks][c].x * up, a[ks][c].y * up, qh[ks][2 * c + hh], ql[ks][2 * c + hh]);
-        } else {
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    qh[ks][2 * c + hh] = live ? __ldg(reinterpret_cast<const uint32_t*>(
-                                                    static_cast<const __half*>(p.q) + off + 16 * ks + 8 * c))
-                                              : 0u;
-        }
-    }
-
-    float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int t = 0; t < 16; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
-
     // the warp's 16 keys of a stage: box and row inside the box are fixed
     const int k0 = 16 * warp, box_b = p.box_rows * kHd;  // bytes of a 64-element half of a box
     const uint32_t warp_off = (uint32_t)((k0 / p.box_rows) * box_b * 2 + (k0 % p.box_rows) * 128);
     // ldmatrix lane addresses (rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7))
     const int lr = (lane & 7) + ((lane >> 4) << 3), lc = (lane >> 3) & 1;          // K: matrices (keys 0-7, c), (keys 0-7, c + 1), (keys 8-15, ..)
     const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;          // V (transposed): (keys 0-7, c), (keys 8-15, c), (.., c + 1)
-
     bool ok = true;
-    for (int it = 0; it < ntiles && ok; ++it) {
-        const int st = it % kStages;
-        ok = mbar_wait(&S.full[st], (uint32_t)(it / kStages) & 1u, p.err, kDevTimeoutFull);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t kb = smem_u32(S.ring[st][0]) + warp_off, vb = smem_u32(S.ring[st][1]) + warp_off;
-        const int j0 = it * kTile + k0;                // first key of the warp's 16
-        if (j0 < kv_end) {
-            float s[2][4], sl[2][4];
+    int it = 0;
+    while (w.left > 0 && ok) {
+        const RowsUnit u = rows_unit(p, w.b);
+        const int g = w.g, tile0 = w.tile, tile1 = (int)min((long long)u.tiles, w.tile + w.left);
+        const int ntok = min(u.n, p.tokens_per_tile), rows = ntok * p.G;
+        const int see0 = u.kv_len - u.n + 1;           // keys the first token sees (may be <= 0)
+
+        // ------------------------------------------------------------ queries
+        // A fragments of the 16 rows: thread (gr, gc) holds rows gr, gr + 8,
+        // columns 16 ks + 2 gc + {0, 1} and + 8
+        uint32_t qh[8][4], ql[F32 ? 8 : 1][4];
+        float f[2];                                    // S row factor: scale * log2(e) * the row's power of two
+        int lim[2];                                    // keys seen by the thread's two rows
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[t][e] = sl[t][e] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                uint32_t b[4];
-                const int c = 2 * (ks & 3) + lc;
-                ldsm4(kb + (ks >> 2) * box_b + lr * 128 + ((c ^ (lr & 7)) << 4), b);
-                mma_f16(s[0], qh[ks], b[0], b[1]);
-                mma_f16(s[1], qh[ks], b[2], b[3]);
-                if constexpr (F32) {
-                    mma_f16(sl[0], ql[ks], b[0], b[1]);
-                    mma_f16(sl[1], ql[ks], b[2], b[3]);
-                }
-            }
+        for (int hh = 0; hh < 2; ++hh) {
+            const int r = gr + 8 * hh, tok = r / p.G, h = r - tok * p.G;
+            const bool live = r < rows;
+            lim[hh] = live ? max(0, min(u.kv_len, see0 + tok)) : 0;
+            f[hh] = p.scale_log2;
+            const int64_t off = (int64_t)(u.first + tok) * p.q_stride + (int64_t)(g * p.G + h) * kHd + 2 * gc;
             if constexpr (F32) {
+                float2 a[8][2];
+                float mx = 0.f;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[t][e] += sl[t][e];
-            }
-            uint32_t ph[4], pl[4];
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = j0 + 8 * (e >> 1) + 2 * gc + (e & 1);
-                    v[e] = j < lim[hh] ? s[e >> 1][2 * hh + (e & 1)] * f[hh] : -INFINITY;
-                }
-                float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                    for (int c = 0; c < 2; ++c) {
+                        a[ks][c] = live ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + off +
+                                                                                16 * ks + 8 * c))
+                                        : make_float2(0.f, 0.f);
+                        mx = fmaxf(mx, fmaxf(fabsf(a[ks][c].x), fabsf(a[ks][c].y)));
+                    }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m[hh], mx), mu = (mn == -INFINITY) ? 0.f : mn - kPShift;
-                if (mn > m[hh]) {
-                    const float corr = ex2(m[hh] - mn);
-                    l[hh] *= corr;
+                // largest value to [2^12, 2^13): the low halves stay normal far below it
+                const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
+                const float up = exp2f((float)max(-126, min(126, e)));
+                f[hh] = fmaxf(p.scale_log2 / up, kMinFactor);
 #pragma unroll
-                    for (int t = 0; t < 16; ++t) {
-                        o[t][2 * hh] *= corr;
-                        o[t][2 * hh + 1] *= corr;
-                    }
-                    m[hh] = mn;
-                }
+                for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = ex2(v[e] - mu);
-                l[hh] += (v[0] + v[1]) + (v[2] + v[3]);
-                // P as an A fragment: register hh holds keys 2 gc, 2 gc + 1; register hh + 2 the same + 8
-                if constexpr (F32) {
-                    split2(v[0], v[1], ph[hh], pl[hh]);
-                    split2(v[2], v[3], ph[hh + 2], pl[hh + 2]);
-                } else {
-                    ph[hh] = pack2(v[0], v[1]);
-                    ph[hh + 2] = pack2(v[2], v[3]);
-                }
-            }
-            // values past the last key may be anything, NaN included: they count as zeros
-            const bool tail = j0 + 16 > kv_end;
-            const int left = kv_end - j0 - 2 * gc;     // keys left from this thread's first
-            const uint32_t k0m = (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
-            const uint32_t k1m = (left > 8 ? 0xffffu : 0u) | (left > 9 ? 0xffff0000u : 0u);
+                    for (int c = 0; c < 2; ++c)
+                        split2(a[ks][c].x * up, a[ks][c].y * up, qh[ks][2 * c + hh], ql[ks][2 * c + hh]);
+            } else {
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                uint32_t b[4];
-                const int c = 2 * (t & 3) + vc;
-                ldsm4_t(vb + (t >> 2) * box_b + vr * 128 + ((c ^ (vr & 7)) << 4), b);
-                if (tail) {
-                    b[0] &= k0m;
-                    b[1] &= k1m;
-                    b[2] &= k0m;
-                    b[3] &= k1m;
-                }
-                if constexpr (F32) {
-                    // the tensor core cuts its sums: the 16 keys' products are
-                    // added to the running output by fp32 additions
-                    float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_f16(a0, pl, b[0], b[1]);
-                    mma_f16(a1, pl, b[2], b[3]);
-                    mma_f16(a0, ph, b[0], b[1]);
-                    mma_f16(a1, ph, b[2], b[3]);
+                for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        o[2 * t][e] += a0[e];
-                        o[2 * t + 1][e] += a1[e];
-                    }
-                } else {
-                    mma_f16(o[2 * t], ph, b[0], b[1]);
-                    mma_f16(o[2 * t + 1], ph, b[2], b[3]);
-                }
+                    for (int c = 0; c < 2; ++c)
+                        qh[ks][2 * c + hh] = live ? __ldg(reinterpret_cast<const uint32_t*>(
+                                                        static_cast<const __half*>(p.q) + off + 16 * ks + 8 * c))
+                                                  : 0u;
             }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.empty[st]);
-    }
 
-    // ------------------------------------------------------------------ merge
+        float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-        l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
-        l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
-        if (gc == 0) {
-            S.m[warp][gr + 8 * hh] = m[hh];
-            S.l[warp][gr + 8 * hh] = l[hh];
+        for (int t = 0; t < 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+
+        for (int j = tile0; j < tile1 && ok; ++j, ++it) {
+            const int st = it % kStages;
+            ok = mbar_wait(&S.full[st], (uint32_t)(it / kStages) & 1u, p.err, kDevTimeoutFull);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t kb = smem_u32(S.ring[st][0]) + warp_off, vb = smem_u32(S.ring[st][1]) + warp_off;
+            const int j0 = j * kTile + k0;             // first key of the warp's 16
+            if (j0 < u.kv_len)
+                rows_step<F32>(kb, vb, box_b, lr, lc, vr, vc, gc, j0, u.kv_len, lim, f, qh, ql, o, m, l);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.empty[st]);
         }
-    }
-    __syncthreads();
-    float corr[2];
+
+        // -------------------------------------------------------------- merge
+        // the eight warps' partials, in warp order
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) M = fmaxf(M, S.m[w][gr + 8 * hh]);
-        corr[hh] = m[hh] == -INFINITY ? 0.f : ex2(m[hh] - M);
-    }
-    constexpr int kPer = kRows * kHd / (kRowWarps * 32);  // outputs per thread: row tid / 16, dims 8 (tid % 16) ..
-    const int orow = threadIdx.x >> 4, od = (threadIdx.x & 15) * kPer;
-    float acc[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        if ((warp >> 2) == half) {
-#pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                const int d = 8 * t + 2 * gc;
-                *reinterpret_cast<float2*>(&A.o[warp & 3][gr][d]) = make_float2(o[t][0] * corr[0], o[t][1] * corr[0]);
-                *reinterpret_cast<float2*>(&A.o[warp & 3][gr + 8][d]) = make_float2(o[t][2] * corr[1], o[t][3] * corr[1]);
+        for (int hh = 0; hh < 2; ++hh) {
+            l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
+            l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
+            if (gc == 0) {
+                S.m[warp][gr + 8 * hh] = m[hh];
+                S.l[warp][gr + 8 * hh] = l[hh];
             }
         }
-        __syncthreads();
+        named_bar_sync(1, kRowWarps * 32);
+        float corr[2];
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int hh = 0; hh < 2; ++hh) {
+            float M = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) acc[e] += A.o[w][orow][od + e];
-        __syncthreads();
-    }
-    if (orow < rows) {
-        float M = -INFINITY, L = 0.f;
+            for (int x = 0; x < kRowWarps; ++x) M = fmaxf(M, S.m[x][gr + 8 * hh]);
+            corr[hh] = m[hh] == -INFINITY ? 0.f : ex2(m[hh] - M);
+        }
+        constexpr int kPer = kRows * kHd / (kRowWarps * 32);  // outputs per thread: row tid / 16, dims 8 (tid % 16) ..
+        const int orow = threadIdx.x >> 4, od = (threadIdx.x & 15) * kPer;
+        float acc[kPer];
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) M = fmaxf(M, S.m[w][orow]);
+        for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w)
-            L += S.m[w][orow] == -INFINITY ? 0.f : S.l[w][orow] * ex2(S.m[w][orow] - M);
-        const int tok = orow / p.G, h = orow - tok * p.G;
-        // no key seen: zeros.  A NaN score leaves m at -inf or l at NaN: the row's sum says which
-        const bool none = max(0, min(kv_len, see0 + tok)) == 0;
-        const float inv = none ? 0.f : 1.f / L;
-        const int64_t off = (int64_t)(first + tok0 + tok) * p.out_stride + (int64_t)(g * p.G + h) * kHd + od;
-        if constexpr (F32) {
-            float* d = static_cast<float*>(p.out) + off;
+        for (int half = 0; half < 2; ++half) {
+            if ((warp >> 2) == half) {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) d[e] = none ? 0.f : acc[e] * inv;
-        } else {
-            __half* d = static_cast<__half*>(p.out) + off;
+                for (int t = 0; t < 16; ++t) {
+                    const int d = 8 * t + 2 * gc;
+                    *reinterpret_cast<float2*>(&A.o[warp & 3][gr][d]) =
+                        make_float2(o[t][0] * corr[0], o[t][1] * corr[0]);
+                    *reinterpret_cast<float2*>(&A.o[warp & 3][gr + 8][d]) =
+                        make_float2(o[t][2] * corr[1], o[t][3] * corr[1]);
+                }
+            }
+            named_bar_sync(1, kRowWarps * 32);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) d[e] = __float2half_rn(none ? 0.f : acc[e] * inv);
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) acc[e] += A.o[x][orow][od + e];
+            named_bar_sync(1, kRowWarps * 32);
+        }
+        if (orow < rows) {
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int x = 0; x < kRowWarps; ++x) M = fmaxf(M, S.m[x][orow]);
+#pragma unroll
+            for (int x = 0; x < kRowWarps; ++x)
+                L += S.m[x][orow] == -INFINITY ? 0.f : S.l[x][orow] * ex2(S.m[x][orow] - M);
+            if (tile0 == 0 && tile1 == u.tiles) {
+                const int tok = orow / p.G, h = orow - tok * p.G;
+                const bool none = max(0, min(u.kv_len, see0 + tok)) == 0;
+                const int64_t off = (int64_t)(u.first + tok) * p.out_stride + (int64_t)(g * p.G + h) * kHd + od;
+                rows_store<F32, kPer>(p.out, off, acc, none ? 0.f : rcp(L), none);
+            } else {
+                float* d = part_out(p, 2 * blockIdx.x + (tile0 > 0 ? 0 : 1));
+                if (od == 0) {
+                    d[kRows * kHd + 2 * orow] = M;
+                    d[kRows * kHd + 2 * orow + 1] = L;
+                }
+                float4* x = reinterpret_cast<float4*>(d + orow * kHd + od);
+                x[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                x[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            }
+        }
+        named_bar_sync(1, kRowWarps * 32);   // the next unit overwrites S.m and S.l
+        w.left -= tile1 - tile0;
+        w.tile = 0;
+        if (++w.g == p.n_kv) {
+            w.g = 0;
+            do ++w.b;
+            while (w.left > 0 && w.b < p.B && rows_unit(p, w.b).tiles == 0);
         }
     }
+}
+
+// Joins the partials of a unit that several CTAs shared, in key order, and
+// writes the zeros of one without keys.  One CTA per unit; the sums over the
+// sequences are formed while the row kernel still runs.
+template <bool F32>
+__global__ void __launch_bounds__(256) attn_rows_merge_kernel(const __grid_constant__ AttnBatch p) {
+    __shared__ long long sums[8][2];
+    const int b = blockIdx.x / p.n_kv, g = blockIdx.x - b * p.n_kv;
+    long long total = 0, before = 0;
+    for (int i = threadIdx.x; i < p.B; i += 256) {
+        const int t = rows_unit(p, i).tiles;
+        total += t;
+        if (i < b) before += t;
+    }
+    sum2(total, before, sums, 256, 1);
+    const RowsUnit u = rows_unit(p, b);
+    if (p.kv_lens && g == 0 && threadIdx.x == 0 && (u.n > p.max_new || p.kv_lens[b] != u.kv_len))
+        atomicExch(p.err, kDevBadArg);
+    const int row = threadIdx.x >> 4, od = (threadIdx.x & 15) * 8;
+    const int ntok = min(u.n, p.tokens_per_tile), rows = ntok * p.G;
+    if (row >= rows) return;
+    const long long W = total * p.n_kv, x0 = before * p.n_kv + (long long)g * u.tiles;
+    const int c0 = u.tiles ? rows_cta(x0, W) : 0, c1 = u.tiles ? rows_cta(x0 + u.tiles - 1, W) : 0;
+    if (u.tiles && c0 == c1) return;   // finished by its one CTA
+    const int tok = row / p.G, h = row - tok * p.G;
+    const int64_t off = (int64_t)(u.first + tok) * p.out_stride + (int64_t)(g * p.G + h) * kHd + od;
+    const bool none = max(0, min(u.kv_len, u.kv_len - u.n + 1 + tok)) == 0;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, M = -INFINITY, L = 0.f;
+    grid_dep_wait();
+    for (int c = c0; u.tiles && c <= c1; ++c) {
+        // a CTA with an empty run wrote nothing
+        if (W * c / kRowCtas == W * (c + 1) / kRowCtas) continue;
+        const float* d = part_out(p, 2 * c + (c == c0 ? 1 : 0));
+        const float m = d[kRows * kHd + 2 * row], l = d[kRows * kHd + 2 * row + 1];
+        const float4 x = *reinterpret_cast<const float4*>(d + row * kHd + od);
+        const float4 y = *reinterpret_cast<const float4*>(d + row * kHd + od + 4);
+        const float mn = fmaxf(M, m);
+        const float fo = M == -INFINITY ? 0.f : ex2(M - mn), fn = m == -INFINITY ? 0.f : ex2(m - mn);
+        M = mn;
+        L = fmaf(L, fo, l * fn);
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], fo, v[e] * fn);
+    }
+    rows_store<F32, 8>(p.out, off, acc, none ? 0.f : rcp(L), none);
 }
 
 // ------------------------------------------------- tensor-memory tiles (prompts)
@@ -577,8 +719,10 @@ constexpr uint32_t kIdescO = kIdescS | (1u << 16);                              
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Like find_tile, counted from the batch's end: the last tiles of a sequence
-// see the most keys, so they start first and the short ones fill the gaps.
+// Sequence and tile of the x-th tile of the batch, counted from its end (called
+// by one warp): the tiles of a sequence are its tokens in runs of
+// tokens_per_tile.  The last ones see the most keys, so they start first and
+// the short ones fill the gaps.
 __device__ __forceinline__ bool find_tile_back(const AttnBatch& p, int x, int& seq, int& tile) {
     const int lane = threadIdx.x & 31;
     int before = 0;
@@ -1204,19 +1348,29 @@ int attn_tiles_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p,
     return GLC_OK;
 }
 
-int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, bool f32, cudaStream_t st) {
-    const int smem = (int)sizeof(RowsSmemAll) + 1024;
-    const void* fn = f32 ? (const void*)attn_rows_kernel<true> : (const void*)attn_rows_kernel<false>;
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
-    const long long tiles = (long long)p.T / p.tokens_per_tile + std::min(p.B, p.T);
-    if (tiles > 0x7fffffffLL) return paged_fail(GLC_ERR_UNSUPPORTED, "%d rows are too many for one call", p.T);
-    const dim3 grid((unsigned)tiles, (unsigned)p.n_kv);
-    if (f32)
-        attn_rows_kernel<true><<<grid, kRowThreads, smem, st>>>(tk, tv, p);
-    else
-        attn_rows_kernel<false><<<grid, kRowThreads, smem, st>>>(tk, tv, p);
-    e = cudaGetLastError();
+template <bool F32>
+int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, cudaStream_t st) {
+    constexpr int smem = (int)sizeof(RowsSmemAll) + 1024;
+    static_assert(smem <= 232448, "shared memory of a CTA");
+    if ((long long)p.B * p.n_kv > 0x7fffffffLL)
+        return paged_fail(GLC_ERR_UNSUPPORTED, "%d sequences are too many for one call", p.B);
+    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) {
+        attn_rows_kernel<F32><<<kRowCtas, kRowThreads, smem, st>>>(tk, tv, p);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(p.B * p.n_kv));
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, attn_rows_merge_kernel<F32>, p);
+    }
     if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
     return GLC_OK;
 }
@@ -1227,7 +1381,7 @@ bool takes_tiles(int G, int max_new) { return (long long)max_new * G > kRows; }
 
 int attn_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, bool f32, int max_new,
                 cudaStream_t st) {
-    if (!takes_tiles(p.G, max_new)) return attn_rows_launch(tk, tv, p, f32, st);
+    if (!takes_tiles(p.G, max_new)) return f32 ? attn_rows_launch<true>(tk, tv, p, st) : attn_rows_launch<false>(tk, tv, p, st);
     return f32 ? attn_tiles_launch<true>(tk, tv, p, st) : attn_tiles_launch<false>(tk, tv, p, st);
 }
 
@@ -1303,7 +1457,7 @@ extern "C" int glc_attn_paged_workspace_bytes(int32_t n_heads, int32_t n_kv_head
         max_new < 0)
         return paged_fail(GLC_ERR_INVALID_ARG, "bad attention shape (%d heads, %d KV heads, %d sequences, %d rows)",
                           n_heads, n_kv_heads, B, T);
-    *bytes = 256;
+    *bytes = glc::kRowsWorkBytes;
     return GLC_OK;
 }
 
@@ -1329,6 +1483,7 @@ extern "C" int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_strid
     if (int rc = glc::paged_check_device(cache->k, "the cache")) return rc;
     glc::AttnBatch p = glc::make_batch(q, q_stride, out, out_stride, cu_new, B, T, n_heads, cache->n_kv_heads, scale);
     if (int rc = glc::paged_error_word(&p.err)) return rc;
+    p.work = static_cast<float*>(workspace);
     p.kv_lens = kv_lens;
     p.table = block_table;
     p.max_pages = max_pages;
