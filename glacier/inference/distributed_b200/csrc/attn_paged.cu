@@ -13,11 +13,11 @@
 // and V; more take attn_tiles_kernel on 128-row tensor-memory tiles.
 //
 // attn_rows_kernel: up to 16 query rows of one KV head, so every K and V row is
-// read once for all the heads that share it.  Eight warps take 16 of a stage's
+// read once for all the heads that share it.  Eight warps take 16 of a tile's
 // 128 keys each and keep their own running maximum, sum and output in registers
 // (one pass, no exchange between warps until a unit's end, where the eight
 // partials are joined in warp order); a ninth warp streams the pages with TMA
-// into a ring of three 64 KB stages.  Products run as mma.sync m16n8k16 with
+// into a ring of six 32 KB slots.  Products run as mma.sync m16n8k16 with
 // fp32 accumulators: 16 rows cannot fill a 128-row tensor-memory tile.
 // fp32 queries are carried as two fp16 halves after a power-of-two scale per
 // row, and so are the exponentials (two products each, ~22 bits of q and p
@@ -25,6 +25,8 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <cmath>
 
 #include "common.cuh"
@@ -35,9 +37,8 @@ namespace glc {
 namespace {
 
 constexpr int kHd = 128;
-constexpr int kTile = 128;                     // keys per stage
-constexpr int kStages = 3;
-constexpr int kTileBytes = kTile * kHd * 2;    // one matrix of a stage
+constexpr int kTile = 128;                     // keys per tile
+constexpr int kTileBytes = kTile * kHd * 2;    // K or V of a tile
 constexpr int kRowWarps = 8;
 constexpr int kRowThreads = (kRowWarps + 1) * 32;
 constexpr int kRows = 16;                      // query rows of a tile
@@ -58,7 +59,8 @@ struct AttnBatch {
     int max_pages, ps_log2, n_pages, box_rows;
     int B, T, max_new, n_heads, n_kv, G, tokens_per_tile;
     float scale_log2;               // softmax scale times log2(e)
-    float* work;                    // partials
+    float* work;                    // partials of the row kernel
+    unsigned long long nonce;       // value of a set flag in this call
     int* err;
 };
 
@@ -110,129 +112,18 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
     lo = pack2(a - f.x, b - f.y);
 }
 
+// Power of two that takes a query row's largest value to [2^12, 2^13), where the
+// low halves stay normal far below it, and the score factor that undoes it.
+__device__ __forceinline__ void row_scale(float mx, float scale_log2, float& up, float& f) {
+    const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
+    up = exp2f((float)max(-126, min(126, e)));
+    f = fmaxf(scale_log2 / up, kMinFactor);
+}
+
 // Rows of sequence b, held inside [0, T] whatever cu holds.
 __device__ __forceinline__ void seq_rows(const AttnBatch& p, int b, int& first, int& n) {
     first = min(max(p.cu[b], 0), p.T);
     n = min(max(p.cu[b + 1], first), p.T) - first;
-}
-
-// One warp's 16 keys against the 16 query rows: scores, weights, outputs.
-template <bool F32>
-__device__ __forceinline__ void rows_step(uint32_t kb, uint32_t vb, int box_b, int lr, int lc, int vr, int vc, int gc,
-                                          int j0, int kv_len, const int (&lim)[2], const float (&f)[2],
-                                          const uint32_t (&qh)[8][4], const uint32_t (&ql)[F32 ? 8 : 1][4],
-                                          float (&o)[16][4], float (&m)[2], float (&l)[2]) {
-    float s[2][4], sl[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[t][e] = sl[t][e] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-        uint32_t b[4];
-        const int c = 2 * (ks & 3) + lc;
-        ldsm4(kb + (ks >> 2) * box_b + lr * 128 + ((c ^ (lr & 7)) << 4), b);
-        mma_f16(s[0], qh[ks], b[0], b[1]);
-        mma_f16(s[1], qh[ks], b[2], b[3]);
-        if constexpr (F32) {
-            mma_f16(sl[0], ql[ks], b[0], b[1]);
-            mma_f16(sl[1], ql[ks], b[2], b[3]);
-        }
-    }
-    if constexpr (F32) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] += sl[t][e];
-    }
-    uint32_t ph[4], pl[4];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int j = j0 + 8 * (e >> 1) + 2 * gc + (e & 1);
-            v[e] = j < lim[hh] ? s[e >> 1][2 * hh + (e & 1)] * f[hh] : -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[hh], mx), mu = (mn == -INFINITY) ? 0.f : mn - kPShift;
-        if (mn > m[hh]) {
-            const float corr = ex2(m[hh] - mn);
-            l[hh] *= corr;
-#pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                o[t][2 * hh] *= corr;
-                o[t][2 * hh + 1] *= corr;
-            }
-            m[hh] = mn;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = ex2(v[e] - mu);
-        l[hh] += (v[0] + v[1]) + (v[2] + v[3]);
-        // P as an A fragment: register hh holds keys 2 gc, 2 gc + 1; register hh + 2 the same + 8
-        if constexpr (F32) {
-            split2(v[0], v[1], ph[hh], pl[hh]);
-            split2(v[2], v[3], ph[hh + 2], pl[hh + 2]);
-        } else {
-            ph[hh] = pack2(v[0], v[1]);
-            ph[hh + 2] = pack2(v[2], v[3]);
-        }
-    }
-    // values past the last key may be anything, NaN included: they count as zeros
-    const bool tail = j0 + 16 > kv_len;
-    const int left = kv_len - j0 - 2 * gc;     // keys left from this thread's first
-    const uint32_t k0m = (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
-    const uint32_t k1m = (left > 8 ? 0xffffu : 0u) | (left > 9 ? 0xffff0000u : 0u);
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        uint32_t b[4];
-        const int c = 2 * (t & 3) + vc;
-        ldsm4_t(vb + (t >> 2) * box_b + vr * 128 + ((c ^ (vr & 7)) << 4), b);
-        if (tail) {
-            b[0] &= k0m;
-            b[1] &= k1m;
-            b[2] &= k0m;
-            b[3] &= k1m;
-        }
-        if constexpr (F32) {
-            // the tensor core cuts its sums: the 16 keys' products are
-            // added to the running output by fp32 additions
-            float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(a0, pl, b[0], b[1]);
-            mma_f16(a1, pl, b[2], b[3]);
-            mma_f16(a0, ph, b[0], b[1]);
-            mma_f16(a1, ph, b[2], b[3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[2 * t][e] += a0[e];
-                o[2 * t + 1][e] += a1[e];
-            }
-        } else {
-            mma_f16(o[2 * t], ph, b[0], b[1]);
-            mma_f16(o[2 * t + 1], ph, b[2], b[3]);
-        }
-    }
-}
-
-// N outputs of a row from dimension off on, times inv (zeros where the row sees no key)
-template <bool F32, int N>
-__device__ __forceinline__ void rows_store(void* out, int64_t off, const float (&a)[N], float inv, bool none) {
-    if constexpr (F32) {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + off);
-#pragma unroll
-        for (int e = 0; e < N; e += 4)
-            d[e / 4] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                            : make_float4(a[e] * inv, a[e + 1] * inv, a[e + 2] * inv, a[e + 3] * inv);
-    } else {
-        uint4* d = reinterpret_cast<uint4*>(static_cast<__half*>(out) + off);
-#pragma unroll
-        for (int e = 0; e < N; e += 8)
-            d[e / 8] = none ? make_uint4(0u, 0u, 0u, 0u)
-                            : make_uint4(pack2(a[e] * inv, a[e + 1] * inv), pack2(a[e + 2] * inv, a[e + 3] * inv),
-                                         pack2(a[e + 4] * inv, a[e + 5] * inv), pack2(a[e + 6] * inv, a[e + 7] * inv));
-    }
 }
 
 // ------------------------------------------------------------ few rows (decode)
@@ -240,15 +131,34 @@ __device__ __forceinline__ void rows_store(void* out, int64_t off, const float (
 // tiles of all units, one unit after another, are cut into kRowCtas equal runs,
 // one CTA each: every SM streams the same number of bytes whatever the lengths.
 // A run holds whole units, which are finished in place, and at most two that it
-// shares with its neighbours; their partials (maximum, sum, unnormalised output)
-// go to the workspace, two places a CTA, and attn_rows_merge_kernel joins them in
-// key order.
+// shares with its neighbours.  Their partials (maximum, sum, unnormalised output)
+// go to the workspace, two places a CTA, each with a flag; the CTA that finds all
+// flags of a unit set joins them in key order.  Two may find that at once: they
+// write the same values.  No CTA waits for another.
 constexpr int kRowCtas = 148;
+constexpr int kRowSlots = 6;                   // 32 KB each: K and V tiles in turn
+constexpr int kUnitCache = 256;                // sequences whose lengths are kept in shared memory
+constexpr int kPartFloats = kRows * (kHd + 2); // a partial: outputs, then (maximum, sum) of each row
+constexpr size_t kRowsWorkBytes = (size_t)2 * kRowCtas * (kPartFloats * sizeof(float) + sizeof(unsigned long long));
 
 struct RowsUnit {
     int first, n, kv_len, tiles;
 };
-__device__ __forceinline__ RowsUnit rows_unit(const AttnBatch& p, int b) {
+
+struct RowsSmem {
+    uint8_t ring[kRowSlots][kTileBytes];
+    uint4 q[2][8][32];                         // A fragments of the unit's rows: high and low halves, 8 steps of 16 dims
+    float o[kRowWarps][8][64];                 // joins the warps' outputs, 8 rows x 64 dims at a time
+    float m[kRowWarps][kRows], l[kRowWarps][kRows], qmax[kRowWarps][kRows];
+    int first[kUnitCache], n[kUnitCache], kv[kUnitCache];
+    uint64_t full[kRowSlots], empty[kRowSlots];
+    long long sums[kRowWarps];
+    long long W, x0;                           // tiles in all, first tile of the CTA's run
+    int b, g, tile, left;                      // where that is
+    int last;
+};
+
+__device__ __forceinline__ RowsUnit load_unit(const AttnBatch& p, int b) {
     RowsUnit u;
     seq_rows(p, b, u.first, u.n);
     u.kv_len = u.n;
@@ -259,56 +169,51 @@ __device__ __forceinline__ RowsUnit rows_unit(const AttnBatch& p, int b) {
     u.tiles = u.n > 0 ? (u.kv_len + kTile - 1) / kTile : 0;
     return u;
 }
-
-// CTA that holds tile x of W: the last c with c * W / kRowCtas <= x.
-__device__ __forceinline__ int rows_cta(long long x, long long W) { return (int)(((x + 1) * kRowCtas - 1) / W); }
-
-// Sum over the CTA's `threads` first threads of two values (all of them call).
-__device__ __forceinline__ void sum2(long long& a, long long& b, long long (*buf)[2], int threads, int bar) {
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, off);
-        b += __shfl_xor_sync(0xffffffffu, b, off);
-    }
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
-        buf[warp][0] = a;
-        buf[warp][1] = b;
-    }
-    named_bar_sync(bar, threads);
-    a = b = 0;
-    for (int w = 0; w < (threads >> 5); ++w) {
-        a += buf[w][0];
-        b += buf[w][1];
-    }
+__device__ __forceinline__ RowsUnit get_unit(const AttnBatch& p, const RowsSmem& S, int b) {
+    if (p.B > kUnitCache) return load_unit(p, b);
+    RowsUnit u;
+    u.first = S.first[b];
+    u.n = S.n[b];
+    u.kv_len = S.kv[b];
+    u.tiles = u.n > 0 ? (u.kv_len + kTile - 1) / kTile : 0;
+    return u;
 }
 
 // A position in the flattened tiles, and how many are left of the CTA's run.
 struct RowsWalk {
-    int b, g, tile;
-    long long left;
+    int b, g, tile, left;
+    __device__ __forceinline__ int end(const RowsUnit& u) const { return min(u.tiles, tile + left); }
+    __device__ __forceinline__ void next(const AttnBatch& p, const RowsSmem& S, const RowsUnit& u) {
+        left -= end(u) - tile;
+        tile = 0;
+        if (left > 0 && ++g == p.n_kv) {
+            g = 0;
+            do ++b;
+            while (b + 1 < p.B && get_unit(p, S, b).tiles == 0);
+        }
+    }
 };
 
-struct RowsSmem {
-    uint8_t ring[kStages][2][kTileBytes];
-    float m[kRowWarps][kRows];
-    float l[kRowWarps][kRows];
-    uint64_t full[kStages], empty[kStages];
-    long long sums[kRowWarps][2];
-    RowsWalk start;
-};
-// the merge of a tile's partials: four warps' outputs at a time
-struct RowsSmemAll {
-    RowsSmem s;
-    float o[4][kRows][kHd];
-};
+// CTA that holds tile x of W: the last c with c * W / kRowCtas <= x.
+__device__ __forceinline__ int rows_cta(long long x, long long W) { return (int)(((x + 1) * kRowCtas - 1) / W); }
+__device__ __forceinline__ bool rows_cta_empty(int c, long long W) {
+    return W * c / kRowCtas == W * (c + 1) / kRowCtas;
+}
+// Partials: place 2c for a unit that began before CTA c's run, 2c + 1 for one
+// that goes on behind it.
+__device__ __forceinline__ float* part_at(const AttnBatch& p, int place) { return p.work + (size_t)place * kPartFloats; }
+__device__ __forceinline__ unsigned long long* part_flag(const AttnBatch& p, int place) {
+    return reinterpret_cast<unsigned long long*>(p.work + (size_t)2 * kRowCtas * kPartFloats) + place;
+}
 
-constexpr size_t kRowsWorkBytes = (size_t)2 * kRowCtas * kRows * (kHd + 2) * sizeof(float);
-
-// Partials in the workspace: place 2c for a unit that began before CTA c's run,
-// 2c + 1 for one that goes on behind it.
-__device__ __forceinline__ float* part_out(const AttnBatch& p, int place) {
-    return p.work + (size_t)place * kRows * (kHd + 2);
+// Two outputs of a row, times inv (zeros where the row sees no key)
+template <bool F32>
+__device__ __forceinline__ void store_pair(void* out, int64_t off, float2 a, float inv, bool none) {
+    if constexpr (F32)
+        *reinterpret_cast<float2*>(static_cast<float*>(out) + off) =
+            none ? make_float2(0.f, 0.f) : make_float2(a.x * inv, a.y * inv);
+    else
+        *reinterpret_cast<uint32_t*>(static_cast<__half*>(out) + off) = none ? 0u : pack2(a.x * inv, a.y * inv);
 }
 
 template <bool F32>
@@ -316,52 +221,68 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     attn_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                      const __grid_constant__ AttnBatch p) {
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    RowsSmemAll& A = *reinterpret_cast<RowsSmemAll*>(base);
-    RowsSmem& S = A.s;
+    RowsSmem& S = *reinterpret_cast<RowsSmem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kConsumers = kRowWarps * 32;
 
-    grid_dep_launch_dependents();
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) {
+    if (threadIdx.x == kConsumers) {
+        for (int i = 0; i < kRowSlots; ++i) {
             mbar_init(&S.full[i], 1);
             mbar_init(&S.empty[i], kRowWarps);
         }
         fence_mbar_init();
     }
-    // where the CTA's run of tiles begins
+    // where the CTA's run of tiles begins: sums over the sequences, 256 at a time
     if (warp < kRowWarps) {
-        long long total = 0, none = 0;
-        for (int b = threadIdx.x; b < p.B; b += kRowWarps * 32) total += rows_unit(p, b).tiles;
-        sum2(total, none, S.sums, kRowWarps * 32, 1);
-        const long long W = total * p.n_kv;
-        const long long x0 = W * blockIdx.x / kRowCtas, x1 = W * (blockIdx.x + 1) / kRowCtas;
-        if (threadIdx.x == 0) S.start.left = 0;
-        if (warp == 0 && x1 > x0) {
-            long long before = 0;   // tiles of the sequences before b0
-            for (int b0 = 0; b0 < p.B; b0 += 32) {
-                const int b = b0 + lane;
-                const long long t = b < p.B ? rows_unit(p, b).tiles : 0;
-                long long end = t;
+        const int tid = threadIdx.x;
+        RowsUnit u = tid < p.B ? load_unit(p, tid) : RowsUnit{0, 0, 0, 0};
+        if (p.B <= kUnitCache && tid < p.B) {
+            S.first[tid] = u.first;
+            S.n[tid] = u.n;
+            S.kv[tid] = u.kv_len;
+        }
+        if (tid == 0) S.left = 0;
+        long long total = u.tiles;
+        for (int b = tid + kConsumers; b < p.B; b += kConsumers) total += load_unit(p, b).tiles;
 #pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const long long o = __shfl_up_sync(0xffffffffu, end, off);
-                    if (lane >= off) end += o;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, (before + end) * p.n_kv > x0);
-                if (hit) {
-                    if (lane == __ffs(hit) - 1) {
-                        const long long in = x0 - (before + end - t) * p.n_kv;
-                        S.start = RowsWalk{b, (int)(in / t), (int)(in % t), x1 - x0};
-                    }
-                    break;
-                }
-                before += __shfl_sync(0xffffffffu, end, 31);
+        for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+        if (lane == 0) S.sums[warp] = total;
+        named_bar_sync(1, kConsumers);
+        long long W = 0;
+        for (int x = 0; x < kRowWarps; ++x) W += S.sums[x];
+        W *= p.n_kv;
+        const long long x0 = W * blockIdx.x / kRowCtas, x1 = W * (blockIdx.x + 1) / kRowCtas;
+        long long before = 0;
+        for (int b0 = 0; b0 < p.B && x1 > x0 && before * p.n_kv <= x0; b0 += kConsumers) {
+            if (b0) u = b0 + tid < p.B ? load_unit(p, b0 + tid) : RowsUnit{0, 0, 0, 0};
+            long long end = u.tiles;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const long long o = __shfl_up_sync(0xffffffffu, end, off);
+                if (lane >= off) end += o;
             }
+            named_bar_sync(1, kConsumers);
+            if (lane == 31) S.sums[warp] = end;
+            named_bar_sync(1, kConsumers);
+            long long all = 0;
+            for (int x = 0; x < kRowWarps; ++x) {
+                if (x == warp) end += all + before;
+                all += S.sums[x];
+            }
+            const long long in = x0 - (end - u.tiles) * p.n_kv;   // tiles into this thread's sequence
+            if (in >= 0 && in < (long long)u.tiles * p.n_kv) {
+                S.b = b0 + tid;
+                S.g = (int)(in / u.tiles);
+                S.tile = (int)(in % u.tiles);
+                S.left = (int)min(x1 - x0, (long long)0x7fffffff);
+                S.x0 = x0;
+                S.W = W;
+            }
+            before += all;
         }
     }
     __syncthreads();
-    RowsWalk w = S.start;
+    RowsWalk w{S.b, S.g, S.tile, S.left};
 
     if (warp == kRowWarps) {
         // ------------------------------------------------------- page stream
@@ -369,10 +290,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         bool ok = true;
         int it = 0;
         while (w.left > 0 && ok) {
-            const RowsUnit u = rows_unit(p, w.b);
-            const int end = (int)min((long long)u.tiles, w.tile + w.left);
-            for (int j = w.tile; j < end; ++j, ++it) {
-                const int st = it % kStages;
+            const RowsUnit u = get_unit(p, S, w.b);
+            const int end = w.end(u);
+            for (int j = w.tile; j < end && ok; ++j) {
                 const int r0 = j * kTile + lane * p.box_rows;
                 const bool mine = lane < nbox && r0 < u.kv_len;
                 const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
@@ -385,89 +305,104 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                         page = p.n_pages;
                     }
                 }
-                ok = mbar_wait_backoff(&S.empty[st], ((uint32_t)(it / kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty, 32);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) mbar_arrive_expect_tx(&S.full[st], (uint32_t)(boxes * p.box_rows * kHd * 2 * 2));
-                __syncwarp();
-                if (mine) {
-                    tma_load_kv(S.ring[st][0] + lane * p.box_rows * kHd * 2, &tk, 0, row, w.g, page, &S.full[st]);
-                    tma_load_kv(S.ring[st][1] + lane * p.box_rows * kHd * 2, &tv, 0, row, w.g, page, &S.full[st]);
+#pragma unroll
+                for (int m = 0; m < 2; ++m, ++it) {
+                    const int st = it % kRowSlots;
+                    ok = mbar_wait(&S.empty[st], ((uint32_t)(it / kRowSlots) & 1u) ^ 1u, p.err, kDevTimeoutEmpty);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&S.full[st], (uint32_t)(boxes * p.box_rows * kHd * 2));
+                    __syncwarp();
+                    if (mine)
+                        tma_load_kv(S.ring[st] + lane * p.box_rows * kHd * 2, m ? &tv : &tk, 0, row, w.g, page,
+                                    &S.full[st]);
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-            w.left -= end - w.tile;
-            w.tile = 0;
-            if (++w.g == p.n_kv) {
-                w.g = 0;
-                do ++w.b;
-                while (w.left > 0 && w.b < p.B && rows_unit(p, w.b).tiles == 0);
-            }
+            w.next(p, S, u);
         }
-        if (lane == 0) drain_issued_stages(S.full, kStages, it, kWaitLimitNs);
+        if (lane == 0) drain_issued_stages(S.full, kRowSlots, it, kWaitLimitNs);
         return;
     }
 
+    // sequences without keys (zero rows) and lengths out of range: CTA b % kRowCtas sees to b
+    for (int b = blockIdx.x; b < p.B; b += kRowCtas) {
+        const RowsUnit u = get_unit(p, S, b);
+        if (p.kv_lens && threadIdx.x == 0 && (u.n > p.max_new || p.kv_lens[b] != u.kv_len)) atomicExch(p.err, kDevBadArg);
+        if (u.n > 0 && u.tiles == 0)
+            for (int i = threadIdx.x; i < min(u.n, p.tokens_per_tile) * p.n_heads * (kHd / 2); i += kConsumers) {
+                const int tok = i / (p.n_heads * (kHd / 2)), d = i - tok * p.n_heads * (kHd / 2);
+                store_pair<F32>(p.out, (int64_t)(u.first + tok) * p.out_stride + 2 * d, make_float2(0.f, 0.f), 0.f, true);
+            }
+    }
+
     const int gr = lane >> 2, gc = lane & 3;
-    // the warp's 16 keys of a stage: box and row inside the box are fixed
+    // the warp's 16 keys of a tile: box and row inside the box are fixed
     const int k0 = 16 * warp, box_b = p.box_rows * kHd;  // bytes of a 64-element half of a box
     const uint32_t warp_off = (uint32_t)((k0 / p.box_rows) * box_b * 2 + (k0 % p.box_rows) * 128);
     // ldmatrix lane addresses (rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7))
     const int lr = (lane & 7) + ((lane >> 4) << 3), lc = (lane >> 3) & 1;          // K: matrices (keys 0-7, c), (keys 0-7, c + 1), (keys 8-15, ..)
     const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;          // V (transposed): (keys 0-7, c), (keys 8-15, c), (.., c + 1)
+    long long x = S.x0;                            // flattened position
     bool ok = true;
     int it = 0;
-    while (w.left > 0 && ok) {
-        const RowsUnit u = rows_unit(p, w.b);
-        const int g = w.g, tile0 = w.tile, tile1 = (int)min((long long)u.tiles, w.tile + w.left);
+    while (w.left > 0) {
+        const RowsUnit u = get_unit(p, S, w.b);
+        const int g = w.g, tile0 = w.tile, tile1 = w.end(u);
         const int ntok = min(u.n, p.tokens_per_tile), rows = ntok * p.G;
         const int see0 = u.kv_len - u.n + 1;           // keys the first token sees (may be <= 0)
 
         // ------------------------------------------------------------ queries
-        // A fragments of the 16 rows: thread (gr, gc) holds rows gr, gr + 8,
-        // columns 16 ks + 2 gc + {0, 1} and + 8
-        uint32_t qh[8][4], ql[F32 ? 8 : 1][4];
-        float f[2];                                    // S row factor: scale * log2(e) * the row's power of two
+        // warp ks brings step ks of the A fragments: thread (gr, gc) holds rows
+        // gr, gr + 8, columns 16 ks + 2 gc + {0, 1} and + 8
+        float f[2];                                    // score factor: scale * log2(e) * the row's power of two
         int lim[2];                                    // keys seen by the thread's two rows
+        {
+            uint32_t hi[4], lo[4];
+            float2 a[2][2];
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-            const int r = gr + 8 * hh, tok = r / p.G, h = r - tok * p.G;
-            const bool live = r < rows;
-            lim[hh] = live ? max(0, min(u.kv_len, see0 + tok)) : 0;
-            f[hh] = p.scale_log2;
-            const int64_t off = (int64_t)(u.first + tok) * p.q_stride + (int64_t)(g * p.G + h) * kHd + 2 * gc;
-            if constexpr (F32) {
-                float2 a[8][2];
-                float mx = 0.f;
+            for (int hh = 0; hh < 2; ++hh) {
+                const int r = gr + 8 * hh, tok = r / p.G, h = r - tok * p.G;
+                const bool live = r < rows;
+                lim[hh] = live ? max(0, min(u.kv_len, see0 + tok)) : 0;
+                f[hh] = p.scale_log2;
+                const int64_t off =
+                    (int64_t)(u.first + tok) * p.q_stride + (int64_t)(g * p.G + h) * kHd + 16 * warp + 2 * gc;
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        a[ks][c] = live ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + off +
-                                                                                16 * ks + 8 * c))
+                for (int c = 0; c < 2; ++c) {
+                    if constexpr (F32)
+                        a[hh][c] = live ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + off + 8 * c))
                                         : make_float2(0.f, 0.f);
-                        mx = fmaxf(mx, fmaxf(fabsf(a[ks][c].x), fabsf(a[ks][c].y)));
-                    }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                // largest value to [2^12, 2^13): the low halves stay normal far below it
-                const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
-                const float up = exp2f((float)max(-126, min(126, e)));
-                f[hh] = fmaxf(p.scale_log2 / up, kMinFactor);
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        split2(a[ks][c].x * up, a[ks][c].y * up, qh[ks][2 * c + hh], ql[ks][2 * c + hh]);
-            } else {
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        qh[ks][2 * c + hh] = live ? __ldg(reinterpret_cast<const uint32_t*>(
-                                                        static_cast<const __half*>(p.q) + off + 16 * ks + 8 * c))
-                                                  : 0u;
+                    else
+                        hi[2 * c + hh] = live ? __ldg(reinterpret_cast<const uint32_t*>(static_cast<const __half*>(p.q) +
+                                                                                        off + 8 * c))
+                                              : 0u;
+                }
             }
+            if constexpr (F32) {
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    float mx = fmaxf(fmaxf(fabsf(a[hh][0].x), fabsf(a[hh][0].y)), fmaxf(fabsf(a[hh][1].x), fabsf(a[hh][1].y)));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    if (gc == 0) S.qmax[warp][gr + 8 * hh] = mx;
+                }
+                named_bar_sync(1, kConsumers);
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    float mx = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kRowWarps; ++i) mx = fmaxf(mx, S.qmax[i][gr + 8 * hh]);
+                    float up;
+                    row_scale(mx, p.scale_log2, up, f[hh]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        split2(a[hh][c].x * up, a[hh][c].y * up, hi[2 * c + hh], lo[2 * c + hh]);
+                }
+                S.q[1][warp][lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            S.q[0][warp][lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            named_bar_sync(1, kConsumers);
         }
 
         float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -476,21 +411,128 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
 
-        for (int j = tile0; j < tile1 && ok; ++j, ++it) {
-            const int st = it % kStages;
-            ok = mbar_wait(&S.full[st], (uint32_t)(it / kStages) & 1u, p.err, kDevTimeoutFull);
+        for (int j = tile0; j < tile1 && ok; ++j, it += 2) {
+            const int j0 = j * kTile + k0;             // first key of the warp's 16
+            const bool any = j0 < u.kv_len;
+            uint32_t ph[4], pl[4];
+            // ------------------------------------------------ scores, weights
+            int st = it % kRowSlots;
+            ok = mbar_wait(&S.full[st], (uint32_t)(it / kRowSlots) & 1u, p.err, kDevTimeoutFull);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const uint32_t kb = smem_u32(S.ring[st][0]) + warp_off, vb = smem_u32(S.ring[st][1]) + warp_off;
-            const int j0 = j * kTile + k0;             // first key of the warp's 16
-            if (j0 < u.kv_len)
-                rows_step<F32>(kb, vb, box_b, lr, lc, vr, vc, gc, j0, u.kv_len, lim, f, qh, ql, o, m, l);
+            if (any) {
+                const uint32_t kb = smem_u32(S.ring[st]) + warp_off;
+                float s[2][4], sl[2][4];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][e] = sl[t][e] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    uint32_t b[4];
+                    const int c = 2 * (ks & 3) + lc;
+                    ldsm4(kb + (ks >> 2) * box_b + lr * 128 + ((c ^ (lr & 7)) << 4), b);
+                    const uint4 q = S.q[0][ks][lane];
+                    const uint32_t qa[4] = {q.x, q.y, q.z, q.w};
+                    mma_f16(s[0], qa, b[0], b[1]);
+                    mma_f16(s[1], qa, b[2], b[3]);
+                    if constexpr (F32) {
+                        const uint4 r = S.q[1][ks][lane];
+                        const uint32_t ra[4] = {r.x, r.y, r.z, r.w};
+                        mma_f16(sl[0], ra, b[0], b[1]);
+                        mma_f16(sl[1], ra, b[2], b[3]);
+                    }
+                }
+                if constexpr (F32) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[t][e] += sl[t][e];
+                }
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int k = j0 + 8 * (e >> 1) + 2 * gc + (e & 1);
+                        v[e] = k < lim[hh] ? s[e >> 1][2 * hh + (e & 1)] * f[hh] : -INFINITY;
+                    }
+                    float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float mn = fmaxf(m[hh], mx), mu = (mn == -INFINITY) ? 0.f : mn - kPShift;
+                    if (mn > m[hh]) {
+                        const float corr = ex2(m[hh] - mn);
+                        l[hh] *= corr;
+#pragma unroll
+                        for (int t = 0; t < 16; ++t) {
+                            o[t][2 * hh] *= corr;
+                            o[t][2 * hh + 1] *= corr;
+                        }
+                        m[hh] = mn;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = ex2(v[e] - mu);
+                    l[hh] += (v[0] + v[1]) + (v[2] + v[3]);
+                    // P as an A fragment: register hh holds keys 2 gc, 2 gc + 1; register hh + 2 the same + 8
+                    if constexpr (F32) {
+                        split2(v[0], v[1], ph[hh], pl[hh]);
+                        split2(v[2], v[3], ph[hh + 2], pl[hh + 2]);
+                    } else {
+                        ph[hh] = pack2(v[0], v[1]);
+                        ph[hh + 2] = pack2(v[2], v[3]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.empty[st]);
+            // -------------------------------------------------------- outputs
+            st = (it + 1) % kRowSlots;
+            ok = mbar_wait(&S.full[st], (uint32_t)((it + 1) / kRowSlots) & 1u, p.err, kDevTimeoutFull);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (any) {
+                const uint32_t vb = smem_u32(S.ring[st]) + warp_off;
+                // values past the last key may be anything, NaN included: they count as zeros
+                const bool tail = j0 + 16 > u.kv_len;
+                const int left = u.kv_len - j0 - 2 * gc;   // keys left from this thread's first
+                const uint32_t k0m = (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
+                const uint32_t k1m = (left > 8 ? 0xffffu : 0u) | (left > 9 ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                    uint32_t b[4];
+                    const int c = 2 * (t & 3) + vc;
+                    ldsm4_t(vb + (t >> 2) * box_b + vr * 128 + ((c ^ (vr & 7)) << 4), b);
+                    if (tail) {
+                        b[0] &= k0m;
+                        b[1] &= k1m;
+                        b[2] &= k0m;
+                        b[3] &= k1m;
+                    }
+                    if constexpr (F32) {
+                        // the tensor core cuts its sums: the 16 keys' products are
+                        // added to the running output by fp32 additions
+                        float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma_f16(a0, pl, b[0], b[1]);
+                        mma_f16(a1, pl, b[2], b[3]);
+                        mma_f16(a0, ph, b[0], b[1]);
+                        mma_f16(a1, ph, b[2], b[3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[2 * t][e] += a0[e];
+                            o[2 * t + 1][e] += a1[e];
+                        }
+                    } else {
+                        mma_f16(o[2 * t], ph, b[0], b[1]);
+                        mma_f16(o[2 * t + 1], ph, b[2], b[3]);
+                    }
+                }
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.empty[st]);
         }
 
-        // -------------------------------------------------------------- merge
-        // the eight warps' partials, in warp order
+        // ------------------------------------- the warps' partials, in warp order
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
             l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
@@ -500,117 +542,112 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 S.l[warp][gr + 8 * hh] = l[hh];
             }
         }
-        named_bar_sync(1, kRowWarps * 32);
-        float corr[2];
+        named_bar_sync(1, kConsumers);
+        const bool whole = tile0 == 0 && tile1 == u.tiles;
+        const int place = 2 * blockIdx.x + (tile0 > 0 ? 0 : 1);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
+            if (8 * hh >= rows) break;
             float M = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < kRowWarps; ++x) M = fmaxf(M, S.m[x][gr + 8 * hh]);
-            corr[hh] = m[hh] == -INFINITY ? 0.f : ex2(m[hh] - M);
-        }
-        constexpr int kPer = kRows * kHd / (kRowWarps * 32);  // outputs per thread: row tid / 16, dims 8 (tid % 16) ..
-        const int orow = threadIdx.x >> 4, od = (threadIdx.x & 15) * kPer;
-        float acc[kPer];
+            for (int i = 0; i < kRowWarps; ++i) M = fmaxf(M, S.m[i][gr + 8 * hh]);
+            const float corr = m[hh] == -INFINITY ? 0.f : ex2(m[hh] - M);
+            const int row = warp + 8 * hh;             // the thread's row when it joins
+            float MR = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+            for (int i = 0; i < kRowWarps; ++i) MR = fmaxf(MR, S.m[i][row]);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if ((warp >> 2) == half) {
+            for (int i = 0; i < kRowWarps; ++i) L += S.m[i][row] == -INFINITY ? 0.f : S.l[i][row] * ex2(S.m[i][row] - MR);
+            const int tok = row / p.G;
+            const bool none = max(0, min(u.kv_len, see0 + tok)) == 0;
+            const float inv = none ? 0.f : rcp(L);
+            const int64_t off = (int64_t)(u.first + tok) * p.out_stride + (int64_t)(g * p.G + row - tok * p.G) * kHd;
+            if (!whole && row < rows && lane == 0)
+                *reinterpret_cast<float2*>(part_at(p, place) + kRows * kHd + 2 * row) = make_float2(MR, L);
 #pragma unroll
-                for (int t = 0; t < 16; ++t) {
-                    const int d = 8 * t + 2 * gc;
-                    *reinterpret_cast<float2*>(&A.o[warp & 3][gr][d]) =
-                        make_float2(o[t][0] * corr[0], o[t][1] * corr[0]);
-                    *reinterpret_cast<float2*>(&A.o[warp & 3][gr + 8][d]) =
-                        make_float2(o[t][2] * corr[1], o[t][3] * corr[1]);
+            for (int dh = 0; dh < 2; ++dh) {
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+                    *reinterpret_cast<float2*>(&S.o[warp][gr][8 * t + 2 * gc]) =
+                        make_float2(o[8 * dh + t][2 * hh] * corr, o[8 * dh + t][2 * hh + 1] * corr);
+                named_bar_sync(1, kConsumers);
+                float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < kRowWarps; ++i) {
+                    const float2 y = *reinterpret_cast<const float2*>(&S.o[i][warp][2 * lane]);
+                    acc.x += y.x;
+                    acc.y += y.y;
                 }
-            }
-            named_bar_sync(1, kRowWarps * 32);
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) acc[e] += A.o[x][orow][od + e];
-            named_bar_sync(1, kRowWarps * 32);
-        }
-        if (orow < rows) {
-            float M = -INFINITY, L = 0.f;
-#pragma unroll
-            for (int x = 0; x < kRowWarps; ++x) M = fmaxf(M, S.m[x][orow]);
-#pragma unroll
-            for (int x = 0; x < kRowWarps; ++x)
-                L += S.m[x][orow] == -INFINITY ? 0.f : S.l[x][orow] * ex2(S.m[x][orow] - M);
-            if (tile0 == 0 && tile1 == u.tiles) {
-                const int tok = orow / p.G, h = orow - tok * p.G;
-                const bool none = max(0, min(u.kv_len, see0 + tok)) == 0;
-                const int64_t off = (int64_t)(u.first + tok) * p.out_stride + (int64_t)(g * p.G + h) * kHd + od;
-                rows_store<F32, kPer>(p.out, off, acc, none ? 0.f : rcp(L), none);
-            } else {
-                float* d = part_out(p, 2 * blockIdx.x + (tile0 > 0 ? 0 : 1));
-                if (od == 0) {
-                    d[kRows * kHd + 2 * orow] = M;
-                    d[kRows * kHd + 2 * orow + 1] = L;
+                if (row < rows) {
+                    const int d = 64 * dh + 2 * lane;
+                    if (whole) store_pair<F32>(p.out, off + d, acc, inv, none);
+                    else *reinterpret_cast<float2*>(part_at(p, place) + row * kHd + d) = acc;
                 }
-                float4* x = reinterpret_cast<float4*>(d + orow * kHd + od);
-                x[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                x[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                named_bar_sync(1, kConsumers);
             }
         }
-        named_bar_sync(1, kRowWarps * 32);   // the next unit overwrites S.m and S.l
-        w.left -= tile1 - tile0;
-        w.tile = 0;
-        if (++w.g == p.n_kv) {
-            w.g = 0;
-            do ++w.b;
-            while (w.left > 0 && w.b < p.B && rows_unit(p, w.b).tiles == 0);
-        }
-    }
-}
-
-// Joins the partials of a unit that several CTAs shared, in key order, and
-// writes the zeros of one without keys.  One CTA per unit; the sums over the
-// sequences are formed while the row kernel still runs.
-template <bool F32>
-__global__ void __launch_bounds__(256) attn_rows_merge_kernel(const __grid_constant__ AttnBatch p) {
-    __shared__ long long sums[8][2];
-    const int b = blockIdx.x / p.n_kv, g = blockIdx.x - b * p.n_kv;
-    long long total = 0, before = 0;
-    for (int i = threadIdx.x; i < p.B; i += 256) {
-        const int t = rows_unit(p, i).tiles;
-        total += t;
-        if (i < b) before += t;
-    }
-    sum2(total, before, sums, 256, 1);
-    const RowsUnit u = rows_unit(p, b);
-    if (p.kv_lens && g == 0 && threadIdx.x == 0 && (u.n > p.max_new || p.kv_lens[b] != u.kv_len))
-        atomicExch(p.err, kDevBadArg);
-    const int row = threadIdx.x >> 4, od = (threadIdx.x & 15) * 8;
-    const int ntok = min(u.n, p.tokens_per_tile), rows = ntok * p.G;
-    if (row >= rows) return;
-    const long long W = total * p.n_kv, x0 = before * p.n_kv + (long long)g * u.tiles;
-    const int c0 = u.tiles ? rows_cta(x0, W) : 0, c1 = u.tiles ? rows_cta(x0 + u.tiles - 1, W) : 0;
-    if (u.tiles && c0 == c1) return;   // finished by its one CTA
-    const int tok = row / p.G, h = row - tok * p.G;
-    const int64_t off = (int64_t)(u.first + tok) * p.out_stride + (int64_t)(g * p.G + h) * kHd + od;
-    const bool none = max(0, min(u.kv_len, u.kv_len - u.n + 1 + tok)) == 0;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, M = -INFINITY, L = 0.f;
-    grid_dep_wait();
-    for (int c = c0; u.tiles && c <= c1; ++c) {
-        // a CTA with an empty run wrote nothing
-        if (W * c / kRowCtas == W * (c + 1) / kRowCtas) continue;
-        const float* d = part_out(p, 2 * c + (c == c0 ? 1 : 0));
-        const float m = d[kRows * kHd + 2 * row], l = d[kRows * kHd + 2 * row + 1];
-        const float4 x = *reinterpret_cast<const float4*>(d + row * kHd + od);
-        const float4 y = *reinterpret_cast<const float4*>(d + row * kHd + od + 4);
-        const float mn = fmaxf(M, m);
-        const float fo = M == -INFINITY ? 0.f : ex2(M - mn), fn = m == -INFINITY ? 0.f : ex2(m - mn);
-        M = mn;
-        L = fmaf(L, fo, l * fn);
-        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        // --------------------------------------- a shared unit: the last one joins
+        if (!whole) {
+            const long long u0 = x - tile0;
+            const int c0 = rows_cta(u0, S.W), c1 = rows_cta(u0 + u.tiles - 1, S.W);
+            __threadfence();
+            named_bar_sync(1, kConsumers);
+            if (warp == 0) {
+                if (lane == 0) {
+                    atomicExch(part_flag(p, place), p.nonce);
+                    __threadfence();   // the flag before the others are read
+                }
+                __syncwarp();
+                bool set = true;
+                for (int c = c0 + lane; c <= c1; c += 32)
+                    if (!rows_cta_empty(c, S.W))
+                        set = set && *reinterpret_cast<volatile unsigned long long*>(part_flag(p, 2 * c + (c == c0))) == p.nonce;
+                set = __all_sync(0xffffffffu, set);
+                if (lane == 0) S.last = set && ok;
+                __threadfence();
+            }
+            named_bar_sync(1, kConsumers);
+            if (S.last) {
+#pragma unroll 1
+                for (int row = warp; row < rows; row += kRowWarps) {
+                    // the maximum first: then the parts' outputs come in any number at once
+                    float M = -INFINITY;
+                    for (int c = c0 + lane; c <= c1; c += 32)
+                        if (!rows_cta_empty(c, S.W))
+                            M = fmaxf(M, __ldcg(part_at(p, 2 * c + (c == c0)) + kRows * kHd + 2 * row));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], fo, v[e] * fn);
+                    for (int d = 16; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float L = 0.f;
+#pragma unroll 4
+                    for (int c = c0; c <= c1; ++c) {
+                        if (rows_cta_empty(c, S.W)) continue;
+                        const float* d = part_at(p, 2 * c + (c == c0));
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(d + kRows * kHd + 2 * row));
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(d + row * kHd) + lane);
+                        const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+                        L = fmaf(ml.y, k, L);
+                        acc.x = fmaf(y.x, k, acc.x);
+                        acc.y = fmaf(y.y, k, acc.y);
+                        acc.z = fmaf(y.z, k, acc.z);
+                        acc.w = fmaf(y.w, k, acc.w);
+                    }
+                    const int tok = row / p.G;
+                    const bool none = max(0, min(u.kv_len, see0 + tok)) == 0;
+                    const float inv = none ? 0.f : rcp(L);
+                    const int64_t off =
+                        (int64_t)(u.first + tok) * p.out_stride + (int64_t)(g * p.G + row - tok * p.G) * kHd + 4 * lane;
+                    store_pair<F32>(p.out, off, make_float2(acc.x, acc.y), inv, none);
+                    store_pair<F32>(p.out, off + 2, make_float2(acc.z, acc.w), inv, none);
+                }
+                // the flags down again, for the next call or replay on this workspace
+                for (int c = c0 + (int)threadIdx.x; c <= c1; c += kConsumers)
+                    if (!rows_cta_empty(c, S.W)) atomicExch(part_flag(p, 2 * c + (c == c0)), 0ull);
+            }
+        }
+        x += tile1 - tile0;
+        w.next(p, S, u);
     }
-    rows_store<F32, 8>(p.out, off, acc, none ? 0.f : rcp(L), none);
 }
 
 // ------------------------------------------------- tensor-memory tiles (prompts)
@@ -1189,9 +1226,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     float mx = fmaxf(fmaxf(fabsf(a[i].x), fabsf(a[i].y)), fmaxf(fabsf(a[i].z), fabsf(a[i].w)));
 #pragma unroll
                     for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                    const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
-                    const float up = exp2f((float)max(-126, min(126, e)));
-                    if (lane == 0) S.f[t][r] = fmaxf(p.scale_log2 / up, kMinFactor);
+                    float up, fr;
+                    row_scale(mx, p.scale_log2, up, fr);
+                    if (lane == 0) S.f[t][r] = fr;
                     uint2 hi, lo;
                     split2(a[i].x * up, a[i].y * up, hi.x, lo.x);
                     split2(a[i].z * up, a[i].w * up, hi.y, lo.y);
@@ -1348,28 +1385,25 @@ int attn_tiles_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p,
     return GLC_OK;
 }
 
+// Flags of one call differ from those of any other and from what a workspace may
+// hold by chance (2^-64); a call leaves them down.
+unsigned long long next_nonce() {
+    static std::atomic<unsigned long long> n{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+    unsigned long long z = n.fetch_add(0x9E3779B97F4A7C15ull, std::memory_order_relaxed);
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;   // SplitMix64
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return (z ^ (z >> 31)) | 1ull;
+}
+
 template <bool F32>
-int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, cudaStream_t st) {
-    constexpr int smem = (int)sizeof(RowsSmemAll) + 1024;
+int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p, cudaStream_t st) {
+    constexpr int smem = (int)sizeof(RowsSmem) + 1024;
     static_assert(smem <= 232448, "shared memory of a CTA");
-    if ((long long)p.B * p.n_kv > 0x7fffffffLL)
-        return paged_fail(GLC_ERR_UNSUPPORTED, "%d sequences are too many for one call", p.B);
+    p.nonce = next_nonce();
     cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) {
         attn_rows_kernel<F32><<<kRowCtas, kRowThreads, smem, st>>>(tk, tv, p);
         e = cudaGetLastError();
-    }
-    if (e == cudaSuccess) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(p.B * p.n_kv));
-        cfg.blockDim = dim3(256);
-        cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, attn_rows_merge_kernel<F32>, p);
     }
     if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
     return GLC_OK;
