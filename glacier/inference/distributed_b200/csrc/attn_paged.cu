@@ -16,8 +16,8 @@
 // read once for all the heads that share it.  Eight warps take 16 of a tile's
 // 128 keys each and keep their own running maximum, sum and output in registers
 // (one pass, no exchange between warps until a unit's end, where the eight
-// partials are joined in warp order); a ninth warp streams the pages with TMA
-// into a ring of six 32 KB slots.  Products run as mma.sync m16n8k16 with
+// partials are joined in warp order); two more stream the pages with TMA
+// into a ring of six 32 KB slots, one the keys, one the values.  Products run as mma.sync m16n8k16 with
 // fp32 accumulators: 16 rows cannot fill a 128-row tensor-memory tile.
 // fp32 queries are carried as two fp16 halves after a power-of-two scale per
 // row, and so are the exponentials (two products each, ~22 bits of q and p
@@ -40,7 +40,7 @@ constexpr int kHd = 128;
 constexpr int kTile = 128;                     // keys per tile
 constexpr int kTileBytes = kTile * kHd * 2;    // K or V of a tile
 constexpr int kRowWarps = 8;
-constexpr int kRowThreads = (kRowWarps + 1) * 32;
+constexpr int kRowThreads = (kRowWarps + 2) * 32;
 constexpr int kRows = 16;                      // query rows of a tile
 constexpr float kPShift = 10.f;                // exponentials are stored as 2^10 e^(s - m): see below
 
@@ -60,7 +60,7 @@ struct AttnBatch {
     int B, T, max_new, n_heads, n_kv, G, tokens_per_tile;
     float scale_log2;               // softmax scale times log2(e)
     float* work;                    // partials of the row kernel
-    unsigned long long nonce;       // value of a set flag in this call
+    unsigned long long nonce;       // this call's mark in the workspace's counters (low 8 bits zero)
     int* err;
 };
 
@@ -132,14 +132,19 @@ __device__ __forceinline__ void seq_rows(const AttnBatch& p, int b, int& first, 
 // one CTA each: every SM streams the same number of bytes whatever the lengths.
 // A run holds whole units, which are finished in place, and at most two that it
 // shares with its neighbours.  Their partials (maximum, sum, unnormalised output)
-// go to the workspace, two places a CTA, each with a flag; the CTA that finds all
-// flags of a unit set joins them in key order.  Two may find that at once: they
-// write the same values.  No CTA waits for another.
+// go to the workspace, two places a CTA; the last CTA to bring its own, told by a
+// counter per shared unit, joins them in key order.  No CTA waits for another,
+// and the order of arrival changes no result.
+// A counter starts from whatever the workspace holds: at its start every CTA that
+// has a part of the unit sets a counter that does not carry this call's nonce to
+// the nonce (compare and swap), and counts up only after that; the last one
+// clears it, so a replayed graph starts over.
 constexpr int kRowCtas = 148;
 constexpr int kRowSlots = 6;                   // 32 KB each: K and V tiles in turn
 constexpr int kUnitCache = 256;                // sequences whose lengths are kept in shared memory
 constexpr int kPartFloats = kRows * (kHd + 2); // a partial: outputs, then (maximum, sum) of each row
-constexpr size_t kRowsWorkBytes = (size_t)2 * kRowCtas * (kPartFloats * sizeof(float) + sizeof(unsigned long long));
+constexpr size_t kRowsWorkBytes =
+    (size_t)kRowCtas * (2 * kPartFloats * sizeof(float) + sizeof(unsigned long long));
 
 struct RowsUnit {
     int first, n, kv_len, tiles;
@@ -148,7 +153,7 @@ struct RowsUnit {
 struct RowsSmem {
     uint8_t ring[kRowSlots][kTileBytes];
     uint4 q[2][8][32];                         // A fragments of the unit's rows: high and low halves, 8 steps of 16 dims
-    float o[kRowWarps][8][64];                 // joins the warps' outputs, 8 rows x 64 dims at a time
+    float o[kRowWarps][8][72];                 // joins the warps' outputs, 8 rows x 64 dims at a time (rows 8 banks apart)
     float m[kRowWarps][kRows], l[kRowWarps][kRows], qmax[kRowWarps][kRows];
     int first[kUnitCache], n[kUnitCache], kv[kUnitCache];
     uint64_t full[kRowSlots], empty[kRowSlots];
@@ -202,8 +207,18 @@ __device__ __forceinline__ bool rows_cta_empty(int c, long long W) {
 // Partials: place 2c for a unit that began before CTA c's run, 2c + 1 for one
 // that goes on behind it.
 __device__ __forceinline__ float* part_at(const AttnBatch& p, int place) { return p.work + (size_t)place * kPartFloats; }
-__device__ __forceinline__ unsigned long long* part_flag(const AttnBatch& p, int place) {
-    return reinterpret_cast<unsigned long long*>(p.work + (size_t)2 * kRowCtas * kPartFloats) + place;
+// Counter of the unit whose first tile CTA c holds and whose last one it does not.
+__device__ __forceinline__ unsigned long long* part_count(const AttnBatch& p, int c) {
+    return reinterpret_cast<unsigned long long*>(p.work + (size_t)2 * kRowCtas * kPartFloats) + c;
+}
+__device__ __forceinline__ void part_open(const AttnBatch& p, int c) {
+    unsigned long long* n = part_count(p, c);
+    unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(n);
+    while ((old & ~0xffull) != p.nonce) {
+        const unsigned long long seen = atomicCAS(n, old, p.nonce);
+        if (seen == old) break;
+        old = seen;
+    }
 }
 
 // Two outputs of a row, times inv (zeros where the row sees no key)
@@ -226,6 +241,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     constexpr int kConsumers = kRowWarps * 32;
 
     if (threadIdx.x == kConsumers) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
         for (int i = 0; i < kRowSlots; ++i) {
             mbar_init(&S.full[i], 1);
             mbar_init(&S.empty[i], kRowWarps);
@@ -284,16 +301,18 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     __syncthreads();
     RowsWalk w{S.b, S.g, S.tile, S.left};
 
-    if (warp == kRowWarps) {
-        // ------------------------------------------------------- page stream
+    if (warp >= kRowWarps) {
+        // ---------------------------------- page stream: keys, and values
+        const int m = warp - kRowWarps;
+        const CUtensorMap* tm = m ? &tv : &tk;
         const int nbox = kTile / p.box_rows, ps = 1 << p.ps_log2;
         bool ok = true;
-        int it = 0;
+        int it = m;
         while (w.left > 0 && ok) {
             const RowsUnit u = get_unit(p, S, w.b);
             const int end = w.end(u);
-            for (int j = w.tile; j < end && ok; ++j) {
-                const int r0 = j * kTile + lane * p.box_rows;
+            for (int j = w.tile; j < end; ++j, it += 2) {
+                const int r0 = j * kTile + lane * p.box_rows, st = it % kRowSlots;
                 const bool mine = lane < nbox && r0 < u.kv_len;
                 const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
                 int page = 0, row = u.first + r0;
@@ -305,26 +324,30 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                         page = p.n_pages;
                     }
                 }
-#pragma unroll
-                for (int m = 0; m < 2; ++m, ++it) {
-                    const int st = it % kRowSlots;
-                    ok = mbar_wait(&S.empty[st], ((uint32_t)(it / kRowSlots) & 1u) ^ 1u, p.err, kDevTimeoutEmpty);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&S.full[st], (uint32_t)(boxes * p.box_rows * kHd * 2));
-                    __syncwarp();
-                    if (mine)
-                        tma_load_kv(S.ring[st] + lane * p.box_rows * kHd * 2, m ? &tv : &tk, 0, row, w.g, page,
-                                    &S.full[st]);
-                    __syncwarp();
-                }
+                ok = mbar_wait(&S.empty[st], ((uint32_t)(it / kRowSlots) & 1u) ^ 1u, p.err, kDevTimeoutEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&S.full[st], (uint32_t)(boxes * p.box_rows * kHd * 2));
+                __syncwarp();
+                if (mine)
+                    tma_load_kv(S.ring[st] + lane * p.box_rows * kHd * 2, tm, 0, row, w.g, page, &S.full[st]);
+                __syncwarp();
             }
             w.next(p, S, u);
         }
-        if (lane == 0) drain_issued_stages(S.full, kRowSlots, it, kWaitLimitNs);
+        // the tiles in flight land before the CTA can exit
+        if (lane == 0)
+            for (int i = it - kRowSlots < m ? m : it - kRowSlots; i < it; i += 2)
+                mbar_wait(&S.full[i % kRowSlots], (uint32_t)(i / kRowSlots) & 1u, nullptr, 0);
         return;
     }
 
+    // the counters of the units this CTA shares (at most its first and its last)
+    if (threadIdx.x == 0 && w.left > 0) {
+        const RowsUnit u = get_unit(p, S, w.b);
+        if (w.tile > 0 || w.left < u.tiles) part_open(p, rows_cta(S.x0 - w.tile, S.W));
+        if (w.left > u.tiles - w.tile) part_open(p, blockIdx.x);   // (a last unit that is whole leaves it unused)
+    }
     // sequences without keys (zero rows) and lengths out of range: CTA b % kRowCtas sees to b
     for (int b = blockIdx.x; b < p.B; b += kRowCtas) {
         const RowsUnit u = get_unit(p, S, b);
@@ -428,19 +451,25 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[t][e] = sl[t][e] = 0.f;
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    uint32_t b[4];
-                    const int c = 2 * (ks & 3) + lc;
-                    ldsm4(kb + (ks >> 2) * box_b + lr * 128 + ((c ^ (lr & 7)) << 4), b);
-                    const uint4 q = S.q[0][ks][lane];
-                    const uint32_t qa[4] = {q.x, q.y, q.z, q.w};
-                    mma_f16(s[0], qa, b[0], b[1]);
-                    mma_f16(s[1], qa, b[2], b[3]);
-                    if constexpr (F32) {
-                        const uint4 r = S.q[1][ks][lane];
-                        const uint32_t ra[4] = {r.x, r.y, r.z, r.w};
-                        mma_f16(sl[0], ra, b[0], b[1]);
-                        mma_f16(sl[1], ra, b[2], b[3]);
+                for (int kh = 0; kh < 2; ++kh) {       // the loads of four steps ahead of their products
+                    uint32_t b[4][4];
+                    uint4 q[4], r[4];
+#pragma unroll
+                    for (int k4 = 0; k4 < 4; ++k4) {
+                        ldsm4(kb + kh * box_b + lr * 128 + (((2 * k4 + lc) ^ (lr & 7)) << 4), b[k4]);
+                        q[k4] = S.q[0][4 * kh + k4][lane];
+                        if constexpr (F32) r[k4] = S.q[1][4 * kh + k4][lane];
+                    }
+#pragma unroll
+                    for (int k4 = 0; k4 < 4; ++k4) {
+                        const uint32_t qa[4] = {q[k4].x, q[k4].y, q[k4].z, q[k4].w};
+                        mma_f16(s[0], qa, b[k4][0], b[k4][1]);
+                        mma_f16(s[1], qa, b[k4][2], b[k4][3]);
+                        if constexpr (F32) {
+                            const uint32_t ra[4] = {r[k4].x, r[k4].y, r[k4].z, r[k4].w};
+                            mma_f16(sl[0], ra, b[k4][0], b[k4][1]);
+                            mma_f16(sl[1], ra, b[k4][2], b[k4][3]);
+                        }
                     }
                 }
                 if constexpr (F32) {
@@ -590,47 +619,58 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         if (!whole) {
             const long long u0 = x - tile0;
             const int c0 = rows_cta(u0, S.W), c1 = rows_cta(u0 + u.tiles - 1, S.W);
-            __threadfence();
-            named_bar_sync(1, kConsumers);
+            // (the barrier above orders the CTA's stores before thread 0's release)
             if (warp == 0) {
+                int parts = 0;
+                for (int c = c0 + lane; c <= c1; c += 32) parts += !rows_cta_empty(c, S.W);
+                parts = __reduce_add_sync(0xffffffffu, parts);
                 if (lane == 0) {
-                    atomicExch(part_flag(p, place), p.nonce);
-                    __threadfence();   // the flag before the others are read
+                    const bool last = atom_add_acq_rel_gpu_u64(part_count(p, c0), 1ull) + 1 == p.nonce + parts;
+                    if (last) *part_count(p, c0) = 0;
+                    S.last = last && ok;
                 }
-                __syncwarp();
-                bool set = true;
-                for (int c = c0 + lane; c <= c1; c += 32)
-                    if (!rows_cta_empty(c, S.W))
-                        set = set && *reinterpret_cast<volatile unsigned long long*>(part_flag(p, 2 * c + (c == c0))) == p.nonce;
-                set = __all_sync(0xffffffffu, set);
-                if (lane == 0) S.last = set && ok;
-                __threadfence();
             }
             named_bar_sync(1, kConsumers);
             if (S.last) {
 #pragma unroll 1
                 for (int row = warp; row < rows; row += kRowWarps) {
-                    // the maximum first: then the parts' outputs come in any number at once
-                    float M = -INFINITY;
-                    for (int c = c0 + lane; c <= c1; c += 32)
-                        if (!rows_cta_empty(c, S.W))
-                            M = fmaxf(M, __ldcg(part_at(p, 2 * c + (c == c0)) + kRows * kHd + 2 * row));
-#pragma unroll
-                    for (int d = 16; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    float L = 0.f;
-#pragma unroll 4
-                    for (int c = c0; c <= c1; ++c) {
-                        if (rows_cta_empty(c, S.W)) continue;
-                        const float* d = part_at(p, 2 * c + (c == c0));
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(d + kRows * kHd + 2 * row));
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(d + row * kHd) + lane);
-                        const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-                        L = fmaf(ml.y, k, L);
-                        acc.x = fmaf(y.x, k, acc.x);
-                        acc.y = fmaf(y.y, k, acc.y);
-                        acc.z = fmaf(y.z, k, acc.z);
-                        acc.w = fmaf(y.w, k, acc.w);
+                    float M = -INFINITY, L = 0.f;
+#pragma unroll 1
+                    for (int cb = c0; cb <= c1; cb += 32) {   // lane i: part cb + i
+                        const int c = cb + lane;
+                        const bool part = c <= c1 && !rows_cta_empty(c, S.W);
+                        float2 ml = make_float2(-INFINITY, 0.f);
+                        if (part)
+                            ml = __ldcg(reinterpret_cast<const float2*>(part_at(p, 2 * c + (c == c0)) + kRows * kHd + 2 * row));
+                        float mn = fmaxf(M, ml.x);
+#pragma unroll
+                        for (int d = 16; d >= 1; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+                        const float old = M == -INFINITY ? 0.f : ex2(M - mn), k = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
+                        L = fmaf(L, old, warp_sum(ml.y * k));
+                        acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+                        M = mn;
+                        const unsigned parts = __ballot_sync(0xffffffffu, part);
+#pragma unroll 1
+                        for (int i0 = 0; i0 < 32 && cb + i0 <= c1; i0 += 8) {   // eight parts' outputs at once
+                            float4 y[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                const int q = cb + i0 + i;
+                                if (parts >> (i0 + i) & 1u)
+                                    y[i] = __ldcg(reinterpret_cast<const float4*>(part_at(p, 2 * q + (q == c0)) + row * kHd) +
+                                                  lane);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float ki = __shfl_sync(0xffffffffu, k, i0 + i);
+                                acc.x = fmaf(y[i].x, ki, acc.x);
+                                acc.y = fmaf(y[i].y, ki, acc.y);
+                                acc.z = fmaf(y[i].z, ki, acc.z);
+                                acc.w = fmaf(y[i].w, ki, acc.w);
+                            }
+                        }
                     }
                     const int tok = row / p.G;
                     const bool none = max(0, min(u.kv_len, see0 + tok)) == 0;
@@ -640,9 +680,6 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                     store_pair<F32>(p.out, off, make_float2(acc.x, acc.y), inv, none);
                     store_pair<F32>(p.out, off + 2, make_float2(acc.z, acc.w), inv, none);
                 }
-                // the flags down again, for the next call or replay on this workspace
-                for (int c = c0 + (int)threadIdx.x; c <= c1; c += kConsumers)
-                    if (!rows_cta_empty(c, S.W)) atomicExch(part_flag(p, 2 * c + (c == c0)), 0ull);
             }
         }
         x += tile1 - tile0;
@@ -1385,14 +1422,13 @@ int attn_tiles_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p,
     return GLC_OK;
 }
 
-// Flags of one call differ from those of any other and from what a workspace may
-// hold by chance (2^-64); a call leaves them down.
+// Differs from call to call, and from what a workspace may hold by chance (2^-56).
 unsigned long long next_nonce() {
     static std::atomic<unsigned long long> n{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
     unsigned long long z = n.fetch_add(0x9E3779B97F4A7C15ull, std::memory_order_relaxed);
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;   // SplitMix64
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    return (z ^ (z >> 31)) | 1ull;
+    return ((z ^ (z >> 31)) & ~0xffull) | 0x100ull;
 }
 
 template <bool F32>
