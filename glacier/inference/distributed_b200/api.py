@@ -43,7 +43,10 @@ def torch_stream_handle(stream=None) -> int:
     not order with the default stream); it is passed as cudaStreamLegacy
     instead, so work stays ordered with torch's own operations."""
     import torch
-    s = (stream if stream is not None else torch.cuda.current_stream()).cuda_stream
+    if stream is None:  # the handle alone: building the Stream object costs 3 us a call
+        s = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    else:
+        s = stream.cuda_stream
     return s if s != 0 else CUDA_STREAM_LEGACY
 
 

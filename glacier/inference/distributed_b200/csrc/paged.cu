@@ -8,6 +8,7 @@
 // batch of sequences of different lengths has no counterpart there.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -116,11 +117,15 @@ namespace {
 // give-back.
 //
 // Bound by latency, not by bytes: a few hundred KB at most, behind three
-// dependent sums.  One launch of one cluster of up to 8 CTAs: every CTA walks
-// all requests (1024 at a time, sums by warp shuffles) and writes its share of
-// the rows and entries, so the only wait between CTAs is one cluster barrier
-// between the pages given back and the pages taken.
+// dependent sums.  Up to kPlanFlat requests (kv_plan_flat_kernel) every CTA forms
+// all the sums itself, keeps them in shared memory and writes its share of the
+// rows and entries; a page that is given back and taken in the same step is
+// looked up in the row it comes from, so no CTA reads what another writes and
+// nothing waits.  More requests (kv_plan_kernel) go 1024 at a time through one
+// cluster of 8 CTAs, with a cluster barrier between the pages given back and the
+// pages taken.
 constexpr int kPlanMaxCluster = 8;
+constexpr int kPlanFlat = 4096;
 
 struct PlanParams {
     const int32_t* ctx;
@@ -307,6 +312,130 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
     }
 }
 
+// First index in [0, n) whose inclusive end is above x (ends ascending).
+__device__ __forceinline__ int upper(const int* end, int n, int x) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int m = (lo + hi) >> 1;
+        if (end[m] > x) hi = m;
+        else lo = m + 1;
+    }
+    return lo;
+}
+
+// Sums past what they are compared with (T rows, the pages there are) are held
+// one above it, so 32 bits carry them.
+__global__ void __launch_bounds__(1024, 1) kv_plan_flat_kernel(const __grid_constant__ PlanParams p) {
+    extern __shared__ int plan_smem[];
+    int* row_end = plan_smem;         // [B] inclusive ends: rows, pages given back, pages taken
+    int* back_end = row_end + p.B;
+    int* page_end = back_end + p.B;
+    int* s_ctx = page_end + p.B;
+    int* s_held = s_ctx + p.B;        // pages held, -1 - held for a request that is not served
+    __shared__ long long part[32];
+    const int tid = threadIdx.x, nt = blockDim.x, items = (p.B + nt - 1) / nt, i0 = tid * items;
+    const int ps = 1 << p.ps_log2;
+    const int n = max(0, min(items, p.B - i0));
+    const long long free0 = min(max(*p.free_in, 0), p.capacity);
+
+    long long rows = 0, back = 0;
+    for (int i = i0; i < i0 + n; ++i) {
+        const int ctx = p.ctx[i], nw = p.nw[i];
+        s_ctx[i] = ctx;
+        s_held[i] = nw;
+        rows += max(nw, 0);
+        if (nw < 0) back += min(((long long)max(ctx, 0) + ps - 1) >> p.ps_log2, (long long)p.width);
+    }
+    long long all_rows, all_back, all_need;
+    long long r = block_scan(rows, part, all_rows) - rows, g = block_scan(back, part, all_back) - back;
+    const long long avail = min(free0 + all_back, (long long)p.capacity);
+    long long need_sum = 0;
+    for (int i = i0; i < i0 + n; ++i) {
+        const int ctx = s_ctx[i], nw = s_held[i];
+        const long long held = ((long long)max(ctx, 0) + ps - 1) >> p.ps_log2;
+        const long long want = ((long long)max(ctx, 0) + max(nw, 0) + ps - 1) >> p.ps_log2;
+        r += max(nw, 0);
+        if (nw < 0) g += min(held, (long long)p.width);
+        row_end[i] = (int)min(r, (long long)p.T + (p.T < 0x7fffffff));
+        back_end[i] = (int)min(g, (long long)0x7fffffff);
+        const bool fits = nw >= 0 && ctx >= 0 && r <= p.T && want <= p.width;
+        page_end[i] = fits ? (int)(want - held) : -1;   // pages needed, for now
+        if (fits) need_sum += want - held;
+    }
+    long long e = block_scan(need_sum, part, all_need) - need_sum;
+    long long used = 0;
+    int bad = 0;
+    for (int i = i0; i < i0 + n; ++i) {
+        const int ctx = s_ctx[i], nw = s_held[i], need = page_end[i];
+        if (need > 0) e += need;
+        const bool ok = need == 0 || (need > 0 && e <= avail);
+        if (need > 0 && ok) used = e;
+        bad += nw >= 0 && !ok;
+        const int held = (int)min(((long long)max(ctx, 0) + ps - 1) >> p.ps_log2, (long long)p.width);
+        page_end[i] = (int)min(e, avail + 1);
+        s_held[i] = ok ? held : -1 - held;
+        if (blockIdx.x == 0) {
+            p.cu[i + 1] = min(row_end[i], p.T);
+            p.kv[i] = ok ? ctx + nw : 0;
+        }
+    }
+    if (blockIdx.x == 0) {
+        if (tid == 0) p.cu[0] = 0;
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) {
+            used = max(used, __shfl_xor_sync(0xffffffffu, used, off));
+            bad += __shfl_xor_sync(0xffffffffu, bad, off);
+        }
+        __syncthreads();
+        if ((tid & 31) == 0) part[tid >> 5] = used << 32 | (unsigned)bad;
+        __syncthreads();
+        if (tid == 0) {
+            used = 0;
+            bad = 0;
+            for (int w = 0; w < (nt >> 5); ++w) {
+                used = max(used, part[w] >> 32);
+                bad += (int)(part[w] & 0xffffffffll);
+            }
+            *p.free_out = (int)(avail - used);
+            *p.status = bad;
+        }
+    }
+    __syncthreads();
+
+    const int first = blockIdx.x * nt + tid, step = gridDim.x * nt;
+    auto page_of = [&](long long rank) -> int {         // the page of this rank among those taken
+        const long long at = avail - 1 - rank;
+        if (at < free0) return p.pool[at];
+        const int x = (int)(at - free0), q = upper(back_end, p.B, x);
+        return p.table[(long long)q * p.width + x - (q ? back_end[q - 1] : 0)];
+    };
+    for (long long x = first; x < min(all_back, (long long)p.capacity - free0); x += step) {
+        const int q = upper(back_end, p.B, (int)x);
+        p.pool[free0 + x] = p.table[(long long)q * p.width + x - (q ? back_end[q - 1] : 0)];
+    }
+    for (long long x = first; x < min(all_need, avail); x += step) {
+        const int q = upper(page_end, p.B, (int)x);
+        if (q < p.B && s_held[q] >= 0) {
+            const long long at = x - (q ? page_end[q - 1] : 0);
+            p.table[(long long)q * p.width + s_held[q] + at] = page_of(x);
+        }
+    }
+    for (long long t = first; t < p.T; t += step) {
+        int pos = 0;
+        long long slot = -1;
+        const int q = t < all_rows ? upper(row_end, p.B, (int)t) : p.B;
+        if (q < p.B && s_held[q] >= 0) {
+            pos = s_ctx[q] + (int)(t - (q ? row_end[q - 1] : 0));
+            const int col = pos >> p.ps_log2;
+            const int page = col < s_held[q] ? p.table[(long long)q * p.width + col]
+                                             : page_of((q ? page_end[q - 1] : 0) + (long long)(col - s_held[q]));
+            slot = ((long long)page << p.ps_log2) + (pos & (ps - 1));
+        }
+        p.pos[t] = pos;
+        p.slots[t] = slot;
+    }
+}
+
 // ------------------------------------------------- rotary embedding and store
 // Pair (i, i + 64) of a head of a token at position s turns by s theta^(-2i/128);
 // rotated queries go to q_out, rotated keys and the values as fp16 to row
@@ -363,7 +492,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
 #pragma unroll
     for (int e = 0; e < 4; ++e) rope_cs(pos, p.inv_freq[4 * sub + e], c[e], s[e]);
     const int hend = min(heads, h0 + 2 * p.run);
-#pragma unroll 2
+#pragma unroll 4
     for (int h = h0 + (lane >> 4); h < hend; h += 2) {
         const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv;
         const int kh = h - p.n_heads - (is_k ? 0 : p.n_kv);
@@ -437,20 +566,33 @@ extern "C" int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens,
     p.width = max_pages;
     p.capacity = capacity;
     p.T = T;
-    const int threads = 1024;
-    const int cluster = glc::kPlanMaxCluster;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(cluster);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, glc::kv_plan_kernel, p);
+    cudaError_t e = cudaSuccess;
+    if (B <= glc::kPlanFlat) {
+        // every CTA repeats the sums: as many as one row or page a thread takes, up to all SMs
+        const int threads = B <= 256 ? 256 : 1024;
+        const long long work = std::max<long long>(T, B);
+        const int grid = (int)std::min<long long>(148, (work + threads - 1) / threads);
+        const int smem = 5 * (int)sizeof(int) * B;
+        if (smem > 48 * 1024)
+            e = cudaFuncSetAttribute(glc::kv_plan_flat_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) {
+            glc::kv_plan_flat_kernel<<<std::max(grid, 1), threads, smem, (cudaStream_t)stream>>>(p);
+            e = cudaGetLastError();
+        }
+    } else {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(glc::kPlanMaxCluster);
+        cfg.blockDim = dim3(1024);
+        cfg.stream = (cudaStream_t)stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = glc::kPlanMaxCluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, glc::kv_plan_kernel, p);
+    }
     if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "page plan: %s", cudaGetErrorString(e));
     return GLC_OK;
 }
@@ -507,7 +649,11 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
     p.n_kv = n_kv_heads;
     for (int i = 0; i < 64; ++i) p.inv_freq[i] = std::exp(-(double)(2 * i) / 128.0 * std::log((double)rope_theta));
     const long long pairs = (n_heads + 2LL * n_kv_heads + 1) / 2;
-    p.run = 1;
+    // A warp's four angles (double reduction, sincosf: ~200 instructions) serve its
+    // run of head pairs: long runs where there are warps enough, one pair a warp
+    // where the call is short (8192 rows of 48 / 8 heads: 158 us with runs of one
+    // pair, 78 us with eight).
+    p.run = (int)std::min<long long>(8, std::max<long long>(1, (long long)T * pairs / (148 * 64)));
     const long long warps = (long long)T * ((pairs + p.run - 1) / p.run);
     const long long blocks = (warps + 7) / 8;
     if (blocks > 0x7fffffffLL) return paged_fail(GLC_ERR_UNSUPPORTED, "%d rows are too many for one call", T);

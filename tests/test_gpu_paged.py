@@ -68,7 +68,8 @@ def same_plan(got, want):
 @pytest.mark.parametrize("B,ps,max_ctx,max_new,T,short", [
     (1, 16, 100, 1, 1, 0), (1, 256, 0, 700, 800, 0), (5, 16, 40, 3, 16, 0), (64, 16, 5000, 1, 64, 0),
     (33, 32, 300, 200, 4000, 0), (1024, 16, 200, 4, 4096, 0), (1025, 16, 200, 4, 4096, 0), (3000, 64, 500, 30, 60000, 0),
-    (257, 16, 60, 60, 9000, 40), (1500, 16, 60, 60, 50000, 900), (40, 128, 300, 300, 2000, 0), (9, 16, 50, 50, 0, 0)])
+    (257, 16, 60, 60, 9000, 40), (1500, 16, 60, 60, 50000, 900), (40, 128, 300, 300, 2000, 0), (9, 16, 50, 50, 0, 0),
+    (4096, 16, 90, 3, 9000, 100), (4097, 16, 90, 3, 9000, 0), (9000, 32, 90, 3, 18000, 300)])
 def test_plan_matches_oracle(cuda, glc, B, ps, max_ctx, max_new, T, short):
     rng = np.random.default_rng(B * 7 + ps + T)
     ctx, new, table, pool, free = plan_case(rng, B, ps, max_ctx, max_new, short=short)
