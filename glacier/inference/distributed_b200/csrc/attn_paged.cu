@@ -115,9 +115,10 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 // Power of two that takes a query row's largest value to [2^12, 2^13), where the
 // low halves stay normal far below it, and the score factor that undoes it.
 __device__ __forceinline__ void row_scale(float mx, float scale_log2, float& up, float& f) {
-    const int e = (mx > 0.f && mx < INFINITY) ? 12 - ilogbf(mx) : 0;
-    up = exp2f((float)max(-126, min(126, e)));
-    f = fmaxf(scale_log2 / up, kMinFactor);
+    const int x = (int)(__float_as_uint(mx) >> 23);    // biased exponent; zeros, infinities and NaN stay as they are
+    const int e = x == 0 || x == 255 ? 0 : min(139 - x, 126);
+    up = __uint_as_float((uint32_t)(127 + e) << 23);
+    f = fmaxf(scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23), kMinFactor);
 }
 
 // Rows of sequence b, held inside [0, T] whatever cu holds.
@@ -156,20 +157,23 @@ struct RowsSmem {
     float o[kRowWarps][8][72];                 // joins the warps' outputs, 8 rows x 64 dims at a time (rows 8 banks apart)
     float m[kRowWarps][kRows], l[kRowWarps][kRows], qmax[kRowWarps][kRows];
     int first[kUnitCache], n[kUnitCache], kv[kUnitCache];
-    uint64_t full[kRowSlots], empty[kRowSlots];
-    long long sums[kRowWarps];
+    uint64_t full[kRowSlots], empty[kRowSlots], opened;
+    long long sums[kRowWarps], rest[kRowWarps];
     long long W, x0;                           // tiles in all, first tile of the CTA's run
     int b, g, tile, left;                      // where that is
     int last;
 };
 
-__device__ __forceinline__ RowsUnit load_unit(const AttnBatch& p, int b) {
+__device__ __forceinline__ RowsUnit load_unit(const AttnBatch& p, int b, bool record = false) {
     RowsUnit u;
+    int len = 0;
+    if (p.kv_lens) len = p.kv_lens[b];
     seq_rows(p, b, u.first, u.n);
     u.kv_len = u.n;
     if (p.kv_lens) {
         const long long room = (long long)p.max_pages << p.ps_log2;
-        u.kv_len = (int)min((long long)max(p.kv_lens[b], 0), room);
+        u.kv_len = (int)min((long long)max(len, 0), room);
+        if (record && (len != u.kv_len || u.n > p.max_new)) atomicExch(p.err, kDevBadArg);
     }
     u.tiles = u.n > 0 ? (u.kv_len + kTile - 1) / kTile : 0;
     return u;
@@ -200,7 +204,10 @@ struct RowsWalk {
 };
 
 // CTA that holds tile x of W: the last c with c * W / kRowCtas <= x.
-__device__ __forceinline__ int rows_cta(long long x, long long W) { return (int)(((x + 1) * kRowCtas - 1) / W); }
+__device__ __forceinline__ int rows_cta(long long x, long long W) {
+    const long long n = (x + 1) * kRowCtas - 1;
+    return W <= 0xffffffff / kRowCtas ? (int)((uint32_t)n / (uint32_t)W) : (int)(n / W);
+}
 __device__ __forceinline__ bool rows_cta_empty(int c, long long W) {
     return W * c / kRowCtas == W * (c + 1) / kRowCtas;
 }
@@ -247,29 +254,22 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             mbar_init(&S.full[i], 1);
             mbar_init(&S.empty[i], kRowWarps);
         }
+        mbar_init(&S.opened, 1);
         fence_mbar_init();
     }
     // where the CTA's run of tiles begins: sums over the sequences, 256 at a time
     if (warp < kRowWarps) {
         const int tid = threadIdx.x;
-        RowsUnit u = tid < p.B ? load_unit(p, tid) : RowsUnit{0, 0, 0, 0};
+        RowsUnit u = tid < p.B ? load_unit(p, tid, blockIdx.x == 0) : RowsUnit{0, 0, 0, 0};
         if (p.B <= kUnitCache && tid < p.B) {
             S.first[tid] = u.first;
             S.n[tid] = u.n;
             S.kv[tid] = u.kv_len;
         }
         if (tid == 0) S.left = 0;
-        long long total = u.tiles;
-        for (int b = tid + kConsumers; b < p.B; b += kConsumers) total += load_unit(p, b).tiles;
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-        if (lane == 0) S.sums[warp] = total;
-        named_bar_sync(1, kConsumers);
-        long long W = 0;
-        for (int x = 0; x < kRowWarps; ++x) W += S.sums[x];
-        W *= p.n_kv;
-        const long long x0 = W * blockIdx.x / kRowCtas, x1 = W * (blockIdx.x + 1) / kRowCtas;
-        long long before = 0;
+        long long rest = 0;   // tiles of the sequences behind the first 256
+        for (int b = tid + kConsumers; b < p.B; b += kConsumers) rest += load_unit(p, b, blockIdx.x == 0).tiles;
+        long long before = 0, W = 0, x0 = 0, x1 = 1;
         for (int b0 = 0; b0 < p.B && x1 > x0 && before * p.n_kv <= x0; b0 += kConsumers) {
             if (b0) u = b0 + tid < p.B ? load_unit(p, b0 + tid) : RowsUnit{0, 0, 0, 0};
             long long end = u.tiles;
@@ -278,7 +278,12 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 const long long o = __shfl_up_sync(0xffffffffu, end, off);
                 if (lane >= off) end += o;
             }
-            named_bar_sync(1, kConsumers);
+            if (b0) named_bar_sync(1, kConsumers);
+            if (b0 == 0 && p.B > kConsumers) {
+#pragma unroll
+                for (int off = 16; off >= 1; off >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, off);
+                if (lane == 0) S.rest[warp] = rest;
+            }
             if (lane == 31) S.sums[warp] = end;
             named_bar_sync(1, kConsumers);
             long long all = 0;
@@ -286,11 +291,19 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 if (x == warp) end += all + before;
                 all += S.sums[x];
             }
+            if (b0 == 0) {
+                W = all;
+                if (p.B > kConsumers)
+                    for (int x = 0; x < kRowWarps; ++x) W += S.rest[x];
+                W *= p.n_kv;
+                x0 = W * blockIdx.x / kRowCtas;
+                x1 = W * (blockIdx.x + 1) / kRowCtas;
+            }
             const long long in = x0 - (end - u.tiles) * p.n_kv;   // tiles into this thread's sequence
-            if (in >= 0 && in < (long long)u.tiles * p.n_kv) {
+            if (x1 > x0 && in >= 0 && in < (long long)u.tiles * p.n_kv) {
                 S.b = b0 + tid;
                 S.g = (int)(in / u.tiles);
-                S.tile = (int)(in % u.tiles);
+                S.tile = (int)(in - (long long)S.g * u.tiles);
                 S.left = (int)min(x1 - x0, (long long)0x7fffffff);
                 S.x0 = x0;
                 S.W = W;
@@ -332,6 +345,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 if (mine)
                     tma_load_kv(S.ring[st] + lane * p.box_rows * kHd * 2, tm, 0, row, w.g, page, &S.full[st]);
                 __syncwarp();
+                // the counters of the units this CTA shares (at most its first and its
+                // last), once the first keys are on their way
+                if (it == 0 && lane == 0) {
+                    if (w.tile > 0 || w.left < u.tiles) part_open(p, rows_cta(S.x0 - w.tile, S.W));
+                    if (w.left > u.tiles - w.tile) part_open(p, blockIdx.x);   // (unused where the last unit is whole)
+                    mbar_arrive(&S.opened);
+                }
+                __syncwarp();
             }
             w.next(p, S, u);
         }
@@ -342,16 +363,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         return;
     }
 
-    // the counters of the units this CTA shares (at most its first and its last)
-    if (threadIdx.x == 0 && w.left > 0) {
-        const RowsUnit u = get_unit(p, S, w.b);
-        if (w.tile > 0 || w.left < u.tiles) part_open(p, rows_cta(S.x0 - w.tile, S.W));
-        if (w.left > u.tiles - w.tile) part_open(p, blockIdx.x);   // (a last unit that is whole leaves it unused)
-    }
-    // sequences without keys (zero rows) and lengths out of range: CTA b % kRowCtas sees to b
+    // zero rows of sequences without keys: CTA b % kRowCtas sees to b
     for (int b = blockIdx.x; b < p.B; b += kRowCtas) {
         const RowsUnit u = get_unit(p, S, b);
-        if (p.kv_lens && threadIdx.x == 0 && (u.n > p.max_new || p.kv_lens[b] != u.kv_len)) atomicExch(p.err, kDevBadArg);
         if (u.n > 0 && u.tiles == 0)
             for (int i = threadIdx.x; i < min(u.n, p.tokens_per_tile) * p.n_heads * (kHd / 2); i += kConsumers) {
                 const int tok = i / (p.n_heads * (kHd / 2)), d = i - tok * p.n_heads * (kHd / 2);
@@ -426,6 +440,15 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             }
             S.q[0][warp][lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             named_bar_sync(1, kConsumers);
+        }
+
+        const bool whole = tile0 == 0 && tile1 == u.tiles;
+        int c0 = 0, c1 = 0, parts = 0;                 // CTAs that share the unit
+        if (!whole) {
+            c0 = rows_cta(x - tile0, S.W);
+            c1 = rows_cta(x - tile0 + u.tiles - 1, S.W);
+            for (int c = c0 + lane; c <= c1; c += 32) parts += !rows_cta_empty(c, S.W);
+            parts = __reduce_add_sync(0xffffffffu, parts);
         }
 
         float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -572,7 +595,6 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             }
         }
         named_bar_sync(1, kConsumers);
-        const bool whole = tile0 == 0 && tile1 == u.tiles;
         const int place = 2 * blockIdx.x + (tile0 > 0 ? 0 : 1);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
@@ -617,53 +639,50 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         }
         // --------------------------------------- a shared unit: the last one joins
         if (!whole) {
-            const long long u0 = x - tile0;
-            const int c0 = rows_cta(u0, S.W), c1 = rows_cta(u0 + u.tiles - 1, S.W);
             // (the barrier above orders the CTA's stores before thread 0's release)
-            if (warp == 0) {
-                int parts = 0;
-                for (int c = c0 + lane; c <= c1; c += 32) parts += !rows_cta_empty(c, S.W);
-                parts = __reduce_add_sync(0xffffffffu, parts);
-                if (lane == 0) {
-                    const bool last = atom_add_acq_rel_gpu_u64(part_count(p, c0), 1ull) + 1 == p.nonce + parts;
-                    if (last) *part_count(p, c0) = 0;
-                    S.last = last && ok;
-                }
+            if (threadIdx.x == 0) {
+                ok = ok && mbar_wait(&S.opened, 0, p.err, kDevTimeoutFull);
+                const bool last = ok && atom_add_acq_rel_gpu_u64(part_count(p, c0), 1ull) + 1 == p.nonce + parts;
+                if (last) *part_count(p, c0) = 0;
+                S.last = last;
             }
             named_bar_sync(1, kConsumers);
             if (S.last) {
 #pragma unroll 1
                 for (int row = warp; row < rows; row += kRowWarps) {
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    float M = -INFINITY, L = 0.f;
+                    float M = -INFINITY, L = 0.f, k = 0.f;
 #pragma unroll 1
                     for (int cb = c0; cb <= c1; cb += 32) {   // lane i: part cb + i
                         const int c = cb + lane;
                         const bool part = c <= c1 && !rows_cta_empty(c, S.W);
+                        const unsigned have = __ballot_sync(0xffffffffu, part);
                         float2 ml = make_float2(-INFINITY, 0.f);
                         if (part)
                             ml = __ldcg(reinterpret_cast<const float2*>(part_at(p, 2 * c + (c == c0)) + kRows * kHd + 2 * row));
-                        float mn = fmaxf(M, ml.x);
-#pragma unroll
-                        for (int d = 16; d >= 1; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
-                        const float old = M == -INFINITY ? 0.f : ex2(M - mn), k = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
-                        L = fmaf(L, old, warp_sum(ml.y * k));
-                        acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
-                        M = mn;
-                        const unsigned parts = __ballot_sync(0xffffffffu, part);
 #pragma unroll 1
-                        for (int i0 = 0; i0 < 32 && cb + i0 <= c1; i0 += 8) {   // eight parts' outputs at once
-                            float4 y[8];
+                        for (int i0 = 0; i0 < 32 && cb + i0 <= c1; i0 += 16) {   // sixteen parts' outputs at once
+                            float4 y[16];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
+                            for (int i = 0; i < 16; ++i) {
                                 y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                                 const int q = cb + i0 + i;
-                                if (parts >> (i0 + i) & 1u)
+                                if (have >> (i0 + i) & 1u)
                                     y[i] = __ldcg(reinterpret_cast<const float4*>(part_at(p, 2 * q + (q == c0)) + row * kHd) +
                                                   lane);
                             }
+                            if (i0 == 0) {   // the maximum so far and the parts' weights
+                                float mn = fmaxf(M, ml.x);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
+                                for (int d = 16; d >= 1; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+                                const float old = M == -INFINITY ? 0.f : ex2(M - mn);
+                                k = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
+                                L = fmaf(L, old, warp_sum(ml.y * k));
+                                acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+                                M = mn;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
                                 const float ki = __shfl_sync(0xffffffffu, k, i0 + i);
                                 acc.x = fmaf(y[i].x, ki, acc.x);
                                 acc.y = fmaf(y[i].y, ki, acc.y);
