@@ -59,7 +59,11 @@ struct AttnBatch {
     int max_pages, ps_log2, n_pages, box_rows;
     int B, T, max_new, n_heads, n_kv, G, tokens_per_tile;
     float scale_log2;               // softmax scale times log2(e)
-    float* work;                    // partials of the row kernel
+    float* work;                    // partials of the row kernel, then of the tiles
+    int rows_take;                  // most query rows of a KV head that the row kernel takes (0: not launched)
+    int split;                      // whether the tile kernel may cut a unit's keys into parts
+    int slots;                      // places of its partials
+    float* tile_work;
     unsigned long long nonce;       // this call's mark in the workspace's counters (low 8 bits zero)
     int* err;
 };
@@ -175,6 +179,7 @@ __device__ __forceinline__ RowsUnit load_unit(const AttnBatch& p, int b, bool re
         u.kv_len = (int)min((long long)max(len, 0), room);
         if (record && (len != u.kv_len || u.n > p.max_new)) atomicExch(p.err, kDevBadArg);
     }
+    if (u.n * p.G > p.rows_take) u.n = 0;   // the tile kernel's
     u.tiles = u.n > 0 ? (u.kv_len + kTile - 1) / kTile : 0;
     return u;
 }
@@ -218,11 +223,10 @@ __device__ __forceinline__ float* part_at(const AttnBatch& p, int place) { retur
 __device__ __forceinline__ unsigned long long* part_count(const AttnBatch& p, int c) {
     return reinterpret_cast<unsigned long long*>(p.work + (size_t)2 * kRowCtas * kPartFloats) + c;
 }
-__device__ __forceinline__ void part_open(const AttnBatch& p, int c) {
-    unsigned long long* n = part_count(p, c);
+__device__ __forceinline__ void part_open(unsigned long long* n, unsigned long long nonce) {
     unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(n);
-    while ((old & ~0xffull) != p.nonce) {
-        const unsigned long long seen = atomicCAS(n, old, p.nonce);
+    while ((old & ~0xffull) != nonce) {
+        const unsigned long long seen = atomicCAS(n, old, nonce);
         if (seen == old) break;
         old = seen;
     }
@@ -348,8 +352,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 // the counters of the units this CTA shares (at most its first and its
                 // last), once the first keys are on their way
                 if (it == 0 && lane == 0) {
-                    if (w.tile > 0 || w.left < u.tiles) part_open(p, rows_cta(S.x0 - w.tile, S.W));
-                    if (w.left > u.tiles - w.tile) part_open(p, blockIdx.x);   // (unused where the last unit is whole)
+                    if (w.tile > 0 || w.left < u.tiles) part_open(part_count(p, rows_cta(S.x0 - w.tile, S.W)), p.nonce);
+                    if (w.left > u.tiles - w.tile) part_open(part_count(p, blockIdx.x), p.nonce);   // (unused if whole)
                     mbar_arrive(&S.opened);
                 }
                 __syncwarp();
@@ -728,13 +732,31 @@ constexpr int kTcRows = 128;
 constexpr uint32_t kTcCols = 512;        // S_A, S_B, PV_A, PV_B
 constexpr int kMaxStages = 5;
 
+// A CTA's work: 256 rows (tile) of a KV head of a sequence, and a part of its keys.
+struct TileItem {
+    int seq, tile, g, part, parts;   // parts: the most a unit of this sequence has
+    int part_tiles;                  // key tiles of a part
+    int slot;                        // workspace place of the unit's first part
+};
+
 struct TilesSmem {
     float f[2][kTcRows];                  // score factor of each row
     uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2], p_full[2][2], o_full[2], turn[2], q_full, v_clean,
         drain[2];
     uint32_t tmem;
-    int seq, tile, found;
+    TileItem item;
+    int found;
 };
+
+// Few units with many keys: a unit's key tiles are cut into up to kMaxParts parts
+// of kMinPart tiles or more, one CTA each, whose partials (unnormalised outputs,
+// maximum, sum) are joined through the workspace as in the row kernel.  At most
+// kMaxExtra CTAs more than there are units, so twice as many places.
+constexpr int kMaxParts = 8, kMinPart = 8, kMaxExtra = 3 * 148;
+constexpr int kTilePartFloats = 2 * kTcRows * (kHd + 2);
+__device__ __forceinline__ unsigned long long* tile_count(const AttnBatch& p, int slot) {
+    return reinterpret_cast<unsigned long long*>(p.work + kRowsWorkBytes / sizeof(float)) + slot;
+}
 
 template <bool F32>
 struct TilesLayout {
@@ -812,35 +834,98 @@ constexpr uint32_t kIdescO = kIdescS | (1u << 16);                              
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Sequence and tile of the x-th tile of the batch, counted from its end (called
-// by one warp): the tiles of a sequence are its tokens in runs of
-// tokens_per_tile.  The last ones see the most keys, so they start first and
-// the short ones fill the gaps.
-__device__ __forceinline__ bool find_tile_back(const AttnBatch& p, int x, int& seq, int& tile) {
+// Units and key tiles of sequence b.
+__device__ __forceinline__ void seq_tiles(const AttnBatch& p, int b, int& units, int& tiles) {
+    units = tiles = 0;
+    if (b >= p.B || b < 0) return;
+    int first, n;
+    seq_rows(p, b, first, n);
+    if (n * p.G <= p.rows_take) return;   // none, or the row kernel's
+    units = (n + p.tokens_per_tile - 1) / p.tokens_per_tile * p.n_kv;
+    const long long room = (long long)p.max_pages << p.ps_log2;
+    const int len = p.kv_lens ? (int)min((long long)max(p.kv_lens[b], 0), room) : n;
+    tiles = (len + kTile - 1) / kTile;
+}
+
+// The x-th item of the batch (called by one warp).  Sequences are taken from the
+// batch's end and tiles from a sequence's end: the last ones see the most keys,
+// so they start first and the short ones fill the gaps.
+//
+// With a workspace, keys are cut into parts of L tiles: of the longest sequence's
+// tiles in 1 to 8 parts, the L with the least rounds of 148 CTAs times L, 3 % more
+// for each further part's own prologue and join.
+__device__ __forceinline__ bool find_item(const AttnBatch& p, int x, TileItem& item) {
     const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int b0 = p.B - 1; b0 >= 0; b0 -= 32) {
-        const int b = b0 - lane;
-        int nt = 0;
-        if (b >= 0) {
-            int first, n;
-            seq_rows(p, b, first, n);
-            nt = (n + p.tokens_per_tile - 1) / p.tokens_per_tile;
+    int L = 0x7fffffff;
+    if (p.split) {
+        int most = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 32) {
+            int units, tiles;
+            seq_tiles(p, b0 + lane, units, tiles);
+            most = max(most, tiles);
         }
-        int end = nt;
+        most = __reduce_max_sync(0xffffffffu, most);
+        int len[kMaxParts], count[kMaxParts];
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i) {
+            len[i] = max(kMinPart, (most + i) / (i + 1));
+            count[i] = 0;
+        }
+        if (most > kMinPart) {
+            for (int b0 = 0; b0 < p.B; b0 += 32) {
+                int units, tiles;
+                seq_tiles(p, b0 + lane, units, tiles);
+#pragma unroll
+                for (int i = 0; i < kMaxParts; ++i) count[i] += units * max(1, (tiles + len[i] - 1) / len[i]);
+            }
+            float best = 3.4e38f;
+            int units = 0;
+#pragma unroll
+            for (int i = 0; i < kMaxParts; ++i) {
+                count[i] = __reduce_add_sync(0xffffffffu, count[i]);
+                if (i == 0) units = count[0];
+                const float cost = (float)((count[i] + 147) / 148) * (float)len[i] * (1.f + 0.03f * i);
+                if (cost < best && count[i] - units <= kMaxExtra) {
+                    best = cost;
+                    L = len[i];
+                }
+            }
+        }
+    }
+    int before = 0, slots = 0;
+    for (int b0 = p.B - 1; b0 >= 0; b0 -= 32) {
+        int units, tiles;
+        seq_tiles(p, b0 - lane, units, tiles);
+        const int parts = max(1, (tiles - 1) / L + 1), count = units * parts, split = parts > 1 ? count : 0;
+        int end = count, send = split;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, end, off);
-            if (lane >= off) end += o;
+            const int o = __shfl_up_sync(0xffffffffu, end, off), q = __shfl_up_sync(0xffffffffu, send, off);
+            if (lane >= off) {
+                end += o;
+                send += q;
+            }
         }
-        const unsigned m = __ballot_sync(0xffffffffu, before + end > x);
-        if (m) {
-            const int l = __ffs(m) - 1;
-            seq = b0 - l;
-            tile = before + __shfl_sync(0xffffffffu, end, l) - 1 - x;
-            return true;
+        const unsigned hit = __ballot_sync(0xffffffffu, before + end > x);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            const int np = __shfl_sync(0xffffffffu, parts, l), nu = __shfl_sync(0xffffffffu, units, l);
+            const int in = x - before - __shfl_sync(0xffffffffu, end - count, l);
+            const int u = in / np;                            // unit of the sequence, from its end
+            item.seq = b0 - l;
+            item.part = in - u * np;
+            item.parts = np;
+            item.part_tiles = L;
+            item.tile = nu / p.n_kv - 1 - u / p.n_kv;
+            item.g = u % p.n_kv;
+            item.slot = slots + __shfl_sync(0xffffffffu, send - split, l) + u * np;
+            // first rows that do not ascend may name more units than the workspace has room for
+            const bool room = np == 1 || item.slot + np <= p.slots;
+            if (!room && lane == 0) atomicExch(p.err, kDevBadArg);
+            return room;
         }
         before += __shfl_sync(0xffffffffu, end, 31);
+        slots += __shfl_sync(0xffffffffu, send, 31);
     }
     return false;
 }
@@ -1073,7 +1158,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t* ring = qs + L::kQBytes;
     TilesSmem& S = *reinterpret_cast<TilesSmem*>(ring + L::kStages * kTileBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = blockIdx.x % p.n_kv;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) {
@@ -1094,16 +1178,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         fence_mbar_init();
     }
     if (warp == 0) {
-        int seq = 0, tile = 0;
-        const bool ok = find_tile_back(p, blockIdx.x / p.n_kv, seq, tile);
+        TileItem item;
+        const bool ok = find_item(p, blockIdx.x, item);
         if (lane == 0) {
-            S.seq = seq;
-            S.tile = tile;
+            S.item = item;
             S.found = ok;
         }
     }
     __syncthreads();
     if (!S.found) return;
+    const TileItem item = S.item;
+    const int seq = item.seq, g = item.g, part = item.part;
+    const int tpt = p.tokens_per_tile >> 1;   // tokens per row tile
+    int first, n;
+    seq_rows(p, seq, first, n);
+    const int tok0 = item.tile * p.tokens_per_tile;
+    int kv_len = n;
+    if (p.kv_lens) {
+        const long long room = (long long)p.max_pages << p.ps_log2;
+        kv_len = p.kv_lens[seq];
+        if ((kv_len < 0 || kv_len > room || n > p.max_new) && threadIdx.x == 0) atomicExch(p.err, kDevBadArg);
+        kv_len = kv_len < 0 ? 0 : (kv_len > room ? (int)room : kv_len);
+    }
+    // row tile t: tokens [tok0 + t tpt, +ntok[t]), keys [0, end)
+    int ntok[2], nt[2], kv_end = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        ntok[t] = max(0, min(tpt, n - tok0 - t * tpt));
+        const int end = ntok[t] ? max(0, min(kv_len, kv_len - n + tok0 + t * tpt + ntok[t])) : 0;
+        nt[t] = (end + kTile - 1) / kTile;
+        kv_end = max(kv_end, end);
+    }
+    // this CTA's part of the key tiles, [j0, j1); a tile early in its sequence has fewer parts
+    const int all_tiles = max(nt[0], nt[1]), parts = min(item.parts, max(1, (all_tiles - 1) / item.part_tiles + 1));
+    if (part >= parts) return;
+    const int j0 = (int)((long long)all_tiles * part / parts), j1 = (int)((long long)all_tiles * (part + 1) / parts);
+    const int ntiles = j1 - j0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) nt[t] = max(0, min(nt[t], j1) - j0);   // of them, row tile t's
+
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem)),
                      "r"(kTcCols)
@@ -1115,38 +1228,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_after();
     const uint32_t tmem = S.tmem;
 
-    const int seq = S.seq, tpt = p.tokens_per_tile >> 1;   // tokens per row tile
-    int first, n;
-    seq_rows(p, seq, first, n);
-    const int tok0 = S.tile * p.tokens_per_tile;
-    int kv_len = n;
-    if (p.kv_lens) {
-        const long long room = (long long)p.max_pages << p.ps_log2;
-        kv_len = p.kv_lens[seq];
-        if ((kv_len < 0 || kv_len > room || n > p.max_new) && threadIdx.x == 0) atomicExch(p.err, kDevBadArg);
-        kv_len = kv_len < 0 ? 0 : (kv_len > room ? (int)room : kv_len);
-    }
-    // row tile t: tokens [tok0 + t tpt, +ntok[t]), keys [0, end[t])
-    int ntok[2], nt[2], kv_end = 0;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        ntok[t] = max(0, min(tpt, n - tok0 - t * tpt));
-        const int end = ntok[t] ? max(0, min(kv_len, kv_len - n + tok0 + t * tpt + ntok[t])) : 0;
-        nt[t] = (end + kTile - 1) / kTile;
-        kv_end = max(kv_end, end);
-    }
-    const int ntiles = max(nt[0], nt[1]);
-
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == 8) {
+        if (warp == 11 && lane == 0 && parts > 1) {
+            part_open(tile_count(p, item.slot), p.nonce);
+        } else if (warp == 8) {
             // --------------------------------------------------- K and V tiles
             const int ps = 1 << p.ps_log2, nbox = kTile / p.box_rows, halves = nbox == 1 ? 1 : 2;
             const int box = lane / halves, half = lane - box * halves;
             bool ok = true;
             int it = 0;
             for (int j = 0; j < ntiles && ok; ++j) {
-                const int r0 = j * kTile + box * p.box_rows;
+                const int r0 = (j0 + j) * kTile + box * p.box_rows;
                 const bool mine = box < nbox && r0 < kv_end;
                 const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
                 const uint32_t bytes = (uint32_t)(boxes * p.box_rows * (nbox == 1 ? 256 : 128));
@@ -1175,9 +1268,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     __syncwarp();
                     // values past the last key may be anything, NaN included: zeros
                     // before the tensor core reads them
-                    if (m == 1 && j == ntiles - 1 && kv_end < (j + 1) * kTile) {
+                    if (m == 1 && j == ntiles - 1 && kv_end < (j0 + j + 1) * kTile) {
                         ok = mbar_wait(&S.kv_full[st], (uint32_t)(it / L::kStages) & 1u, p.err, kDevTimeoutFull);
-                        for (int r = kv_end - j * kTile + (lane >> 3); r < kTile; r += 4)
+                        for (int r = kv_end - (j0 + j) * kTile + (lane >> 3); r < kTile; r += 4)
 #pragma unroll
                             for (int h = 0; h < 2; ++h)
                                 *reinterpret_cast<uint4*>(dst + h * (kTileBytes / 2) + r * 128 + (lane & 7) * 16) =
@@ -1233,9 +1326,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int j = 0; j < ntiles && ok; ++j) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2;
                 ok = wait_kv(iv);
-                if (ok && j == ntiles - 1 && kv_end < ntiles * kTile) ok = mbar_wait(&S.v_clean, 0, p.err, kDevTimeoutFull);
-                // the next keys too, while the weights are on their way
-                if (ok && j + 1 < ntiles) ok = wait_kv(ik);
+                if (ok && j == ntiles - 1 && kv_end < j1 * kTile) ok = mbar_wait(&S.v_clean, 0, p.err, kDevTimeoutFull);
+                // the next keys too, while the weights are on their way (fp16 queries; the
+                // three slots of fp32 ones do not hold them yet)
+                if (!F32 && ok && j + 1 < ntiles) ok = wait_kv(ik);
                 if (j < mine) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -1247,8 +1341,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (ok && (F32 || j + 1 == mine)) tc_arrive(&S.o_full[t]);
                 }
                 if (!ok) break;
+                if (F32) {
+                    tc_arrive(&S.kv_empty[iv % L::kStages]);
+                    if (j + 1 < ntiles && !wait_kv(ik)) break;
+                }
                 if (j + 1 < mine) qk(ik);
-                tc_arrive(&S.kv_empty[iv % L::kStages]);
+                if (!F32) tc_arrive(&S.kv_empty[iv % L::kStages]);
                 if (j + 1 < ntiles) tc_arrive(&S.kv_empty[ik % L::kStages]);
             }
             // every product is done before the CTA frees its tensor memory
@@ -1325,6 +1423,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float f = F32 ? S.f[t][row] : p.scale_log2;
         const uint32_t trow = tmem + 128u * t + ((uint32_t)wrow << 16);
         const int64_t out_off = (tok_first + tok) * p.out_stride + (int64_t)(g * p.G + row - tok * p.G) * kHd;
+        float* part_out = p.tile_work + (size_t)(item.slot + part) * kTilePartFloats;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         const int both = min(nt[0], nt[1]);
@@ -1343,8 +1442,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (!ok) break;
                 tc_after();
                 const Turn turn = turn_of(j);
-                const float corr = (j + 1) * kTile > lim0
-                                       ? softmax_row<true>(trow, lim - j * kTile, f, m, l, S.p_full[t], turn, ok)
+                const float corr = (j0 + j + 1) * kTile > lim0
+                                       ? softmax_row<true>(trow, lim - (j0 + j) * kTile, f, m, l, S.p_full[t], turn, ok)
                                        : softmax_row<false>(trow, 0, f, m, l, S.p_full[t], turn, ok);
                 ok = ok && mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1364,7 +1463,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 tc_before();
             }
-            if (live && ok) {
+            if (parts > 1) {
+                if (live && ok) {   // unnormalised, to the workspace
+                    *reinterpret_cast<float2*>(part_out + 2 * kTcRows * kHd + 2 * (kTcRows * t + row)) = make_float2(m, l);
+                    uint4* d = reinterpret_cast<uint4*>(part_out + (size_t)(kTcRows * t + row) * kHd);
+#pragma unroll
+                    for (int e = 0; e < kHd / 2; e += 2) store_f32(d + e / 2, o[e], o[e + 1], pair(1.f, 1.f));
+                }
+            } else if (live && ok) {
                 uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + out_off);
                 if (lim > 0) {
                     const float rl = rcp(l);
@@ -1383,12 +1489,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (!ok) break;
                 tc_after();
                 const Turn turn = turn_of(j);
-                if ((j + 1) * kTile > lim0)
-                    softmax_row_f16<true>(trow, lim - j * kTile, f, j == 0, m, l, S.p_full[t], turn, ok);
+                if ((j0 + j + 1) * kTile > lim0)
+                    softmax_row_f16<true>(trow, lim - (j0 + j) * kTile, f, j == 0, m, l, S.p_full[t], turn, ok);
                 else softmax_row_f16<false>(trow, 0, f, j == 0, m, l, S.p_full[t], turn, ok);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
             }
+            if (parts > 1 && live)
+                *reinterpret_cast<float2*>(part_out + 2 * kTcRows * kHd + 2 * (kTcRows * t + row)) = make_float2(m, l);
             if (ok && nt[t] > 0) {
                 ok = mbar_wait(&S.o_full[t], 0, p.err, kDevTimeoutFull);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1402,6 +1510,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     uint32_t r[32];
                     if (nt[t] > 0) TMEM_LD32(trow + 256u + 32 * c, r);
                     tmem_wait_ld();
+                    if (parts > 1) {   // unnormalised, to the workspace
+                        uint4* x = reinterpret_cast<uint4*>(part_out + (size_t)(kTcRows * t + row) * kHd + 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            if (live)
+                                x[e >> 2] = nt[t] > 0 ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3])
+                                                      : make_uint4(0u, 0u, 0u, 0u);
+                        __syncwarp();
+                        continue;
+                    }
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         uint4 u = make_uint4(0u, 0u, 0u, 0u);
@@ -1424,21 +1542,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcCols) : "memory");
     }
-}
+    if (parts == 1) return;
 
-template <bool F32>
-int attn_tiles_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p, cudaStream_t st) {
-    p.tokens_per_tile = 2 * (kTcRows / p.G);
-    constexpr int smem = TilesLayout<F32>::kBytes;
-    static_assert(smem <= 232448, "shared memory of a CTA");
-    cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
-    const long long tiles = (long long)p.T / p.tokens_per_tile + std::min(p.B, p.T);
-    if (tiles * p.n_kv > 0x7fffffffLL) return paged_fail(GLC_ERR_UNSUPPORTED, "%d rows are too many for one call", p.T);
-    attn_tiles_kernel<F32><<<(unsigned)(tiles * p.n_kv), kTcThreads, smem, st>>>(tk, tv, p);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
-    return GLC_OK;
+    // ------------------------- parts of a unit: the last CTA to end joins them
+    if (threadIdx.x == 0) {
+        const unsigned long long n = atom_add_acq_rel_gpu_u64(tile_count(p, item.slot), 1ull) + 1;
+        S.found = n == p.nonce + parts;
+        if (S.found) *tile_count(p, item.slot) = 0;
+    }
+    __syncthreads();
+    if (!S.found || warp >= 8) return;
+    const float* part0 = p.tile_work + (size_t)item.slot * kTilePartFloats;
+    const int t = warp >> 2, rows = ntok[t] * p.G;
+#pragma unroll 1
+    for (int row = 32 * (warp & 3); row < min(rows, 32 * (warp & 3) + 32); ++row) {
+        const int r = kTcRows * t + row, tok = row / p.G;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < parts)
+            ml = __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)lane * kTilePartFloats + 2 * kTcRows * kHd + 2 * r));
+        float4 y[kMaxParts];
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i)
+            if (i < parts)
+                y[i] = __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)i * kTilePartFloats + (size_t)r * kHd) + lane);
+        float M = ml.x;
+#pragma unroll
+        for (int d = 4; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        M = __shfl_sync(0xffffffffu, M, 0);
+        const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M), kl = warp_sum(k * ml.y);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i) {
+            const float ki = __shfl_sync(0xffffffffu, k, i);
+            if (i < parts)
+                acc = make_float4(fmaf(y[i].x, ki, acc.x), fmaf(y[i].y, ki, acc.y), fmaf(y[i].z, ki, acc.z),
+                                  fmaf(y[i].w, ki, acc.w));
+        }
+        const bool none = kv_len - n + tok0 + t * tpt + tok + 1 <= 0 || kv_len == 0;
+        const float inv = none ? 0.f : rcp(kl);
+        const int64_t off = (int64_t)(first + tok0 + t * tpt + tok) * p.out_stride +
+                            (int64_t)(g * p.G + row - tok * p.G) * kHd + 4 * lane;
+        store_pair<F32>(p.out, off, make_float2(acc.x, acc.y), inv, none);
+        store_pair<F32>(p.out, off + 2, make_float2(acc.z, acc.w), inv, none);
+    }
 }
 
 // Differs from call to call, and from what a workspace may hold by chance (2^-56).
@@ -1451,10 +1597,9 @@ unsigned long long next_nonce() {
 }
 
 template <bool F32>
-int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p, cudaStream_t st) {
+int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, cudaStream_t st) {
     constexpr int smem = (int)sizeof(RowsSmem) + 1024;
     static_assert(smem <= 232448, "shared memory of a CTA");
-    p.nonce = next_nonce();
     cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) {
         attn_rows_kernel<F32><<<kRowCtas, kRowThreads, smem, st>>>(tk, tv, p);
@@ -1464,14 +1609,60 @@ int attn_rows_launch(const CUtensorMap& tk, const CUtensorMap& tv, AttnBatch p, 
     return GLC_OK;
 }
 
-// Tiles where a sequence may have more rows of a KV head than one 16-row tile
-// holds, the row kernel where none has.
-bool takes_tiles(int G, int max_new) { return (long long)max_new * G > kRows; }
+template <bool F32>
+int attn_tiles_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, long long items, cudaStream_t st) {
+    constexpr int smem = TilesLayout<F32>::kBytes;
+    static_assert(smem <= 232448, "shared memory of a CTA");
+    cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
+    if (items > 0x7fffffffLL) return paged_fail(GLC_ERR_UNSUPPORTED, "%d rows are too many for one call", p.T);
+    attn_tiles_kernel<F32><<<(unsigned)items, kTcThreads, smem, st>>>(tk, tv, p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
+    return GLC_OK;
+}
 
-int attn_launch(const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, bool f32, int max_new,
-                cudaStream_t st) {
-    if (!takes_tiles(p.G, max_new)) return f32 ? attn_rows_launch<true>(tk, tv, p, st) : attn_rows_launch<false>(tk, tv, p, st);
-    return f32 ? attn_tiles_launch<true>(tk, tv, p, st) : attn_tiles_launch<false>(tk, tv, p, st);
+// How a call runs, from what the host knows of it.
+struct AttnPlan {
+    bool rows, tiles;     // kernels that are launched
+    bool split;           // units of the tile kernel may be cut
+    long long items;      // most CTAs of it that have work
+    int slots;            // and of their partials
+    size_t work;          // workspace bytes
+    size_t tile_work;     // where the partials of the tile kernel begin
+};
+AttnPlan plan_attention(int n_heads, int n_kv, int B, int T, int max_new, bool workspace) {
+    const int G = n_heads / n_kv;
+    AttnPlan a{};
+    // A sequence of up to 16 rows a KV head is the row kernel's.  With longer ones
+    // in the batch the row kernel comes first where there may be several short
+    // ones; a batch of up to four is left to the tiles, the empty launch costs 3 us.
+    a.tiles = (long long)max_new * G > kRows;
+    a.rows = !a.tiles || (workspace && B > 4);
+    const long long units = ((long long)T / (2 * (kTcRows / G)) + std::min(B, T)) * n_kv;
+    // Many units fill the SMs by themselves, and each CTA looks through all sequences
+    a.split = a.tiles && workspace && units <= 16 * 148;
+    a.items = units + (a.split ? kMaxExtra : 0);
+    a.slots = a.split ? (int)std::min<long long>(units * kMaxParts, 2 * kMaxExtra) : 0;
+    a.tile_work = kRowsWorkBytes + ((size_t)a.slots * sizeof(unsigned long long) + 255) / 256 * 256;
+    a.work = a.tile_work + (size_t)a.slots * kTilePartFloats * sizeof(float);
+    return a;
+}
+
+int attn_launch(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& ttk, const CUtensorMap& ttv, AttnBatch p,
+                const AttnPlan& a, bool f32, cudaStream_t st) {
+    p.nonce = next_nonce();
+    p.rows_take = a.rows ? kRows : 0;
+    p.split = a.split;
+    p.slots = a.slots;
+    p.tile_work = p.work ? p.work + a.tile_work / sizeof(float) : nullptr;
+    if (a.rows) {
+        p.tokens_per_tile = kRows / p.G;
+        if (int rc = f32 ? attn_rows_launch<true>(tk, tv, p, st) : attn_rows_launch<false>(tk, tv, p, st)) return rc;
+    }
+    if (!a.tiles) return GLC_OK;
+    p.tokens_per_tile = 2 * (kTcRows / p.G);
+    return f32 ? attn_tiles_launch<true>(ttk, ttv, p, a.items, st) : attn_tiles_launch<false>(ttk, ttv, p, a.items, st);
 }
 
 // What both attentions ask of their queries, outputs and heads.
@@ -1507,7 +1698,6 @@ AttnBatch make_batch(const void* q, int64_t q_stride, void* out, int64_t out_str
     p.n_heads = n_heads;
     p.n_kv = n_kv;
     p.G = n_heads / n_kv;
-    p.tokens_per_tile = kRows / p.G;
     p.scale_log2 = (float)((scale > 0.f ? (double)scale : 1.0 / std::sqrt((double)kHd)) * 1.4426950408889634);
     return p;
 }
@@ -1536,7 +1726,8 @@ extern "C" int glc_attn_prompt_dev(const void* q, int32_t q_type, int64_t q_stri
     CUtensorMap tk, tv;
     if (int rc = glc::paged_tensor_map(&tk, k, T, kv_stride, n_kv_heads, 128, 1, kv_stride, p.box_rows, 2)) return rc;
     if (int rc = glc::paged_tensor_map(&tv, v, T, kv_stride, n_kv_heads, 128, 1, kv_stride, p.box_rows, 2)) return rc;
-    return glc::attn_launch(tk, tv, p, q_type == GLC_GGUF_F32, T, (cudaStream_t)stream);
+    return glc::attn_launch(tk, tv, tk, tv, p, glc::plan_attention(n_heads, n_kv_heads, B, T, T, false),
+                            q_type == GLC_GGUF_F32, (cudaStream_t)stream);
 }
 
 extern "C" int glc_attn_paged_workspace_bytes(int32_t n_heads, int32_t n_kv_heads, int32_t B, int32_t T,
@@ -1546,7 +1737,7 @@ extern "C" int glc_attn_paged_workspace_bytes(int32_t n_heads, int32_t n_kv_head
         max_new < 0)
         return paged_fail(GLC_ERR_INVALID_ARG, "bad attention shape (%d heads, %d KV heads, %d sequences, %d rows)",
                           n_heads, n_kv_heads, B, T);
-    *bytes = glc::kRowsWorkBytes;
+    *bytes = glc::plan_attention(n_heads, n_kv_heads, B, T, max_new, true).work;
     return GLC_OK;
 }
 
@@ -1580,15 +1771,18 @@ extern "C" int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_strid
     p.n_pages = cache->n_pages;
     while ((1 << p.ps_log2) < cache->page_size) ++p.ps_log2;
     p.box_rows = std::min(cache->page_size, glc::kTile);
-    // a tile's K and V lie as two blocks of 64 dims: a box that covers part of the
-    // tile's keys is one block's, one that covers them all takes both
-    const int halves = glc::takes_tiles(p.G, max_new) && p.box_rows < glc::kTile ? 1 : 2;
-    CUtensorMap tk, tv;
-    if (int rc = glc::paged_tensor_map(&tk, cache->k, cache->page_size, cache->row_stride, cache->n_kv_heads,
-                                       cache->head_stride, cache->n_pages, cache->page_stride, p.box_rows, halves))
-        return rc;
-    if (int rc = glc::paged_tensor_map(&tv, cache->v, cache->page_size, cache->row_stride, cache->n_kv_heads,
-                                       cache->head_stride, cache->n_pages, cache->page_stride, p.box_rows, halves))
-        return rc;
-    return glc::attn_launch(tk, tv, p, q_type == GLC_GGUF_F32, max_new, (cudaStream_t)stream);
+    const glc::AttnPlan a = glc::plan_attention(n_heads, cache->n_kv_heads, B, T, max_new, true);
+    CUtensorMap tk, tv, ttk, ttv;
+    const auto map = [&](CUtensorMap* m, const void* base, int halves) {
+        return glc::paged_tensor_map(m, base, cache->page_size, cache->row_stride, cache->n_kv_heads, cache->head_stride,
+                                     cache->n_pages, cache->page_stride, p.box_rows, halves);
+    };
+    if (int rc = map(&tk, cache->k, 2)) return rc;
+    if (int rc = map(&tv, cache->v, 2)) return rc;
+    // the tile kernel's K and V lie as two blocks of 64 dims: a box that covers part
+    // of a tile's keys is one block's, one that covers them all takes both
+    const int halves = p.box_rows < glc::kTile ? 1 : 2;
+    if (int rc = map(&ttk, cache->k, halves)) return rc;
+    if (int rc = map(&ttv, cache->v, halves)) return rc;
+    return glc::attn_launch(tk, tv, ttk, ttv, p, a, q_type == GLC_GGUF_F32, (cudaStream_t)stream);
 }
