@@ -21,9 +21,10 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-contract=off",
           "-I", CSRC, "-I", INCLUDE, "--expt-relaxed-constexpr"]
 SOURCES = ["api.cu", "gemv_q4k.cu", "gemv_chain.cu", "decode_fused.cu", "decode_wide.cu", "router.cu", "wire.cu", "prefill.cu", "grouped_mma.cu",
-           "noalloc.cu", "ep.cu", "comm.cu", "attention.cu", "paged.cu", "attn_paged.cu", "stage.cu",
+           "noalloc.cu", "ep.cu", "comm.cu", "attention.cu", "paged.cu", "attn_paged.cu", "attn_rows.cu", "attn_tiles.cu",
+           "stage.cu",
            "synth.cpp"]
-HEADERS = ["common.cuh", "gemv_lane.cuh", "kernels.h", "paged.cuh", "synth.h"]
+HEADERS = ["attn.cuh", "common.cuh", "gemv_lane.cuh", "kernels.h", "paged.cuh", "synth.h"]
 
 
 def _compile(src: str, force: bool) -> str:

@@ -1,0 +1,1113 @@
+// attn_tiles.cu -- attention of many query rows (prompts, chunks of prompts) over
+// packed keys or pages: see attn_paged.cu for the operator.
+//
+// An item is 256 query rows of one KV head, as two row tiles A and B of 128
+// (floor(128 / G) tokens times their G heads) that share every K and V tile of
+// 128 keys.  One CTA per SM works through items.  Per key tile and row tile:
+//   S = Q K^T   tcgen05.mma, S in tensor memory;
+//   P = 2^(S f - m)  one warpgroup per row tile, one row per thread: no
+//               exchange between threads; P overwrites S in tensor memory;
+//   PV          tcgen05.mma, P from tensor memory, V from shared memory.
+// While one row tile's warpgroup works on its softmax the tensor core runs the
+// other's products.
+// fp16 queries: PV adds up in tensor memory; a row is rescaled there when its
+// maximum has grown by more than 2^5, which after the first tiles hardly happens.
+// fp32 queries: S and PV take two products each (halves of q and of p, low
+// halves first), and PV is a tile of its own that the row's thread adds to its
+// fp32 output in registers: the tensor core cuts its running sum at every 16
+// keys, which over 32,000 keys costs a decimal digit.  The low halves of q are
+// read from tensor memory and the two row tiles share one PV tile, so both types
+// leave room for five K or V tiles in flight.
+// Warps 0-7: softmax; 8: TMA; 9 and 10: MMA issue; 11: the next items.
+#include <algorithm>
+
+#include "attn.cuh"
+
+namespace glc {
+
+namespace {
+
+constexpr int kTcThreads = 12 * 32;
+constexpr int kTcRows = 128;
+constexpr uint32_t kTcCols = 512;
+// tensor memory: S_A, S_B, then O_A, O_B (fp16 queries) or PV, low halves of Q_A, Q_B (fp32)
+constexpr uint32_t kColO = 256, kColQlo = 384;
+constexpr int kSlots = 5;                 // K and V tiles in flight
+constexpr int kItemBufs = 2;
+#ifndef KPOLY
+#define KPOLY 0
+#endif
+constexpr bool kPoly = KPOLY;
+
+// Few units with many keys: a unit's key tiles are cut into up to kMaxParts parts
+// of kMinPart tiles or more, one item each, whose partials (unnormalised outputs,
+// maximum, sum) are joined through the workspace.  At most kMaxExtra items more
+// than there are units, so twice as many places.
+constexpr int kMaxParts = kTileParts, kMinPart = 8, kMaxExtra = kTileExtra;
+
+// One item, as the roles need it.
+struct TileItem {
+    int seq;          // -1: no more
+    int g;
+    int row0;         // first token of row tile A in q and out
+    int see0;         // keys its first token sees
+    int kv_len, kv_end, kv_row0;
+    int ntok[2];      // tokens of the row tiles
+    int nt[2];        // key tiles of this part that row tile t sees
+    int j0, ntiles;   // this part's key tiles
+    int part, parts, slot;
+};
+
+struct TilesSmem {
+    float f[2][kTcRows];                  // score factor of each row
+    uint64_t kv_full[kSlots], kv_empty[kSlots], s_full[2], p_full[2][2], o_full[2], turn[2], q_full[2], q_free[2], landed,
+        stored, told, item_full[kItemBufs], item_empty[kItemBufs], drain[2];
+    uint32_t tmem;
+    int reads[2];                         // fp32: PV tiles read by each row tile's four warps, counted per warp
+    int last;
+    TileItem item[kItemBufs];
+};
+template <bool F32>
+constexpr int tiles_smem_bytes() {
+    return 2 * kTileBytes + kSlots * kTileBytes + (int)sizeof(TilesSmem) + 1024;
+}
+
+__device__ __forceinline__ unsigned long long* tile_count(const AttnBatch& p, int slot) {
+    return reinterpret_cast<unsigned long long*>(p.work + kRowsWorkBytes / sizeof(float)) + slot;
+}
+
+__device__ __forceinline__ void tma_load_q(void* dst, const CUtensorMap* tm, int head, int token, int half, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+        "l"(tm), "r"(0), "r"(head), "r"(token), "r"(half), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_arrive(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// SWIZZLE_128B matrix descriptors, the low word only: start address and the
+// leading offset; kDescHi holds 1024 bytes between groups of 8 rows (or keys),
+// the version and the swizzle.  K-major (Q, K: 64 dims a row of 128 bytes) has
+// no leading offset; MN-major (V: the dims run along a row, the keys down the
+// rows) has 16 KB between its blocks of 64 dims.  The 64-bit descriptors are put
+// together inside the instruction's block: kept as values, the issuing thread's
+// 64 loop-invariant descriptors spilled to local memory (10x the kernel's time
+// with 227 KB of shared memory, which leaves no first-level cache).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) {
+    return ((addr >> 4) & 0x3FFFu) | (((uint32_t)(kTileBytes / 2) >> 4) << 16);
+}
+// D[tmem] (+)= A[smem] B[smem]^T and D[tmem] (+)= A[tmem] B[smem], fp16 operands, fp32 accumulators
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc),
+        "r"(kDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc),
+        "r"(kDescHi)
+        : "memory");
+}
+constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);   // f32 += f16 x f16, M = N = 128
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);                                     // B MN-major
+
+#define TMEM_LD32(taddr, r)                                                                                        \
+    asm volatile(                                                                                                  \
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"         \
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                                     \
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),           \
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),     \
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),   \
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])    \
+        : "r"(taddr)                                                                                               \
+        : "memory")
+#define TMEM_LD16(taddr, r)                                                                                        \
+    asm volatile(                                                                                                  \
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"     \
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),           \
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])      \
+        : "r"(taddr)                                                                                               \
+        : "memory")
+#define TMEM_ST16(taddr, r)                                                                                        \
+    asm volatile(                                                                                                  \
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"    \
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),       \
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])              \
+        : "memory")
+#define TMEM_ST8(taddr, r)                                                                                         \
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),  \
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])                        \
+                 : "memory")
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Units and key tiles of sequence b.
+__device__ __forceinline__ void seq_tiles(const AttnBatch& p, int b, int& units, int& tiles) {
+    units = tiles = 0;
+    if (b >= p.B || b < 0) return;
+    int first, n;
+    seq_rows(p, b, first, n);
+    if (n * p.G <= p.rows_take) return;   // none, or the row kernel's
+    units = (n + p.tokens_per_tile - 1) / p.tokens_per_tile * p.n_kv;
+    const long long room = (long long)p.max_pages << p.ps_log2;
+    const int len = p.kv_lens ? (int)min((long long)max(p.kv_lens[b], 0), room) : n;
+    tiles = (len + kTile - 1) / kTile;
+}
+
+// Walks a CTA's items (one warp).  Sequences are taken from the batch's end and
+// tiles from a sequence's end: the last ones see the most keys, so they come first
+// and the short ones fill the gaps; CTA c takes items c, 2 * CTAs - 1 - c, and so
+// on back and forth, which evens the sums out.
+//
+// With a workspace, keys are cut into parts of L tiles: of the longest sequence's
+// tiles in 1 to 8 parts, the L with the least rounds of all CTAs times L, 3 % more
+// for each further part's own prologue and join.
+struct ItemWalk {
+    int L, total;                 // tiles of a part, items in all
+    int b0, before, slots;        // chunk of 32 sequences: the one of lane 0, items and places before it
+    int parts, count, split, end, send, chunk, schunk;   // of the lane's sequence; sums of the chunk
+
+    __device__ __forceinline__ void load(const AttnBatch& p) {
+        const int lane = threadIdx.x & 31;
+        int units, tiles;
+        seq_tiles(p, b0 - lane, units, tiles);
+        parts = max(1, (tiles - 1) / L + 1);
+        count = units * parts;
+        split = parts > 1 ? count : 0;
+        end = count;
+        send = split;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, end, off), q = __shfl_up_sync(0xffffffffu, send, off);
+            if (lane >= off) {
+                end += o;
+                send += q;
+            }
+        }
+        chunk = __shfl_sync(0xffffffffu, end, 31);
+        schunk = __shfl_sync(0xffffffffu, send, 31);
+    }
+
+    __device__ __forceinline__ void init(const AttnBatch& p) {
+        const int lane = threadIdx.x & 31;
+        L = 0x7fffffff;
+        int most = 0, units_all = 0;
+        for (int c = 0; c < p.B; c += 32) {
+            int units, tiles;
+            seq_tiles(p, c + lane, units, tiles);
+            most = max(most, tiles);
+            units_all += units;
+        }
+        units_all = __reduce_add_sync(0xffffffffu, units_all);
+        most = __reduce_max_sync(0xffffffffu, most);
+        total = units_all;
+        if (p.split && most > kMinPart) {
+            int len[kMaxParts], n[kMaxParts];
+#pragma unroll
+            for (int i = 0; i < kMaxParts; ++i) {
+                len[i] = max(kMinPart, (most + i) / (i + 1));
+                n[i] = 0;
+            }
+            for (int c = 0; c < p.B; c += 32) {
+                int units, tiles;
+                seq_tiles(p, c + lane, units, tiles);
+#pragma unroll
+                for (int i = 0; i < kMaxParts; ++i) n[i] += units * max(1, (tiles + len[i] - 1) / len[i]);
+            }
+            float best = 3.4e38f;
+            const int ctas = gridDim.x;
+#pragma unroll
+            for (int i = 0; i < kMaxParts; ++i) {
+                n[i] = __reduce_add_sync(0xffffffffu, n[i]);
+                const float cost = (float)((n[i] + ctas - 1) / ctas) * (float)len[i] * (1.f + 0.03f * i);
+                if (cost < best && n[i] - units_all <= kMaxExtra) {
+                    best = cost;
+                    L = len[i];
+                    total = n[i];
+                }
+            }
+        }
+        b0 = p.B - 1;
+        before = slots = 0;
+        load(p);
+    }
+
+    // item x (ascending from call to call); false when this one has no work
+    __device__ __forceinline__ bool get(const AttnBatch& p, int x, TileItem& it) {
+        while (before + chunk <= x) {   // x < total, so a chunk holds it
+            before += chunk;
+            slots += schunk;
+            b0 -= 32;
+            load(p);
+        }
+        const int l = __ffs(__ballot_sync(0xffffffffu, before + end > x)) - 1;
+        const int np = __shfl_sync(0xffffffffu, parts, l), nu = __shfl_sync(0xffffffffu, count, l) / np;
+        const int in = x - before - __shfl_sync(0xffffffffu, end - count, l);
+        const int u = in / np, part = in - u * np;            // unit of the sequence, from its end
+        const int slot = slots + __shfl_sync(0xffffffffu, send - split, l) + u * np;
+        const int tpt = p.tokens_per_tile >> 1;
+        it.seq = b0 - l;
+        it.g = u % p.n_kv;
+        const int tok0 = (nu / p.n_kv - 1 - u / p.n_kv) * p.tokens_per_tile;
+        int first, n;
+        seq_rows(p, it.seq, first, n);
+        it.kv_len = n;
+        it.kv_row0 = p.kv_lens ? 0 : first;
+        if (p.kv_lens) {
+            const long long room = (long long)p.max_pages << p.ps_log2;
+            const int len = p.kv_lens[it.seq];
+            it.kv_len = (int)min((long long)max(len, 0), room);
+            if ((len != it.kv_len || n > p.max_new) && (threadIdx.x & 31) == 0) atomicExch(p.err, kDevBadArg);
+        }
+        it.row0 = first + tok0;
+        it.see0 = it.kv_len - n + tok0 + 1;
+        it.kv_end = 0;
+        int nt[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            it.ntok[t] = max(0, min(tpt, n - tok0 - t * tpt));
+            const int see = it.ntok[t] ? max(0, min(it.kv_len, it.see0 - 1 + t * tpt + it.ntok[t])) : 0;
+            nt[t] = (see + kTile - 1) / kTile;
+            it.kv_end = max(it.kv_end, see);
+        }
+        // a tile early in its sequence has fewer parts
+        const int all = max(nt[0], nt[1]);
+        it.part = part;
+        it.parts = min(np, max(1, (all - 1) / L + 1));
+        it.slot = slot;
+        if (part >= it.parts) return false;
+        it.j0 = (int)((long long)all * part / it.parts);
+        it.ntiles = (int)((long long)all * (part + 1) / it.parts) - it.j0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) it.nt[t] = max(0, min(nt[t], it.j0 + it.ntiles) - it.j0);
+        // first rows that do not ascend may name more units than the workspace has room for
+        if (it.parts > 1 && slot + np > p.slots) {
+            if ((threadIdx.x & 31) == 0) atomicExch(p.err, kDevBadArg);
+            return false;
+        }
+        return true;
+    }
+};
+
+// Pairs of fp32 values in one 64-bit register: half the issue slots of scalar
+// arithmetic.  Volatile on purpose: the compiler otherwise sinks a chunk's
+// arithmetic below the next chunk's tensor-memory load, keeps several chunks
+// alive next to the row's 128 outputs, and spills.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+    return d;
+}
+// o = o * c + (a, b)
+__device__ __forceinline__ void fma_pair(uint64_t& o, uint64_t c, uint32_t a, uint32_t b) {
+    asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, %0, %3, t;\n\t}"
+                 : "+l"(o)
+                 : "r"(a), "r"(b), "l"(c));
+}
+__device__ __forceinline__ void mul_pair(uint32_t& a, uint32_t& b, uint64_t c) {
+    asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tmul.rn.f32x2 t, t, %2;\n\tmov.b64 {%0, %1}, t;\n\t}"
+                 : "+r"(a), "+r"(b)
+                 : "l"(c));
+}
+// 16 bytes of output: the pairs times c
+__device__ __forceinline__ void store_f32(uint4* d, uint64_t a, uint64_t b, uint64_t c) {
+    asm volatile(
+        "{\n\t.reg .b64 t, u;\n\tmul.rn.f32x2 t, %1, %3;\n\tmul.rn.f32x2 u, %2, %3;\n\tst.global.v2.b64 [%0], {t, u};\n\t}" ::
+            "l"(d),
+        "l"(a), "l"(b), "l"(c)
+        : "memory");
+}
+// 2^((a, b) * f - mu)
+__device__ __forceinline__ void exp_pair(uint32_t a, uint32_t b, uint64_t f, uint64_t mu, float& x, float& y) {
+    asm volatile(
+        "{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tfma.rn.f32x2 t, t, %4, %5;\n\tmov.b64 {%0, %1}, t;\n\t"
+        "ex2.approx.ftz.f32 %0, %0;\n\tex2.approx.ftz.f32 %1, %1;\n\t}"
+        : "=f"(x), "=f"(y)
+        : "r"(a), "r"(b), "l"(f), "l"(mu));
+}
+__device__ __forceinline__ void add_pair(uint64_t& s, float a, float b) {
+    asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(s) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void max3(float& m, uint32_t a, uint32_t b) {
+    asm volatile("max.f32 %0, %0, %1, %2;" : "+f"(m) : "r"(a), "r"(b));
+}
+// The same without the exponential unit, on the fp32 pipe: x = n + r with n the
+// nearest integer (adding 1.5 * 2^23 leaves it in the low bits) and |r| <= 1/2, a
+// polynomial for 2^r and n added to its exponent.  The coefficients are a minimax
+// fit of the relative error on [-1/2, 1/2] (Remez exchange): 2^-22.1 in fp32.  x is
+// held above -127, where the result is nothing to an fp16 weight.
+__device__ __forceinline__ void poly_pair(uint32_t a, uint32_t b, uint64_t f, uint64_t mu, float& x, float& y) {
+    constexpr uint64_t kC5 = 0x3aae04733aae0473ull, kC4 = 0x3c1e86293c1e8629ull, kC3 = 0x3d635b723d635b72ull,
+                       kC2 = 0x3e75fc8c3e75fc8cull, kC1 = 0x3f3172143f317214ull, kC0 = 0x3f8000013f800001ull,
+                       kRound = 0x4b4000004b400000ull;
+    asm volatile(
+        "{\n\t.reg .b64 t, n, q;\n\t.reg .b32 ta, tb, na, nb;\n\t"
+        "mov.b64 t, {%2, %3};\n\tfma.rn.f32x2 t, t, %4, %5;\n\t"
+        "mov.b64 {ta, tb}, t;\n\tmax.f32 ta, ta, 0fC2FE0000;\n\tmax.f32 tb, tb, 0fC2FE0000;\n\tmov.b64 t, {ta, tb};\n\t"
+        "add.rn.f32x2 n, t, %6;\n\tsub.rn.f32x2 q, n, %6;\n\tsub.rn.f32x2 t, t, q;\n\t"
+        "fma.rn.f32x2 q, t, %7, %8;\n\tfma.rn.f32x2 q, q, t, %9;\n\tfma.rn.f32x2 q, q, t, %10;\n\t"
+        "fma.rn.f32x2 q, q, t, %11;\n\tfma.rn.f32x2 q, q, t, %12;\n\t"
+        "mov.b64 {ta, tb}, q;\n\tmov.b64 {na, nb}, n;\n\t"
+        "shl.b32 na, na, 23;\n\tshl.b32 nb, nb, 23;\n\tadd.s32 na, ta, na;\n\tadd.s32 nb, tb, nb;\n\tmov.b32 %0, na;\n\tmov.b32 %1, nb;\n\t}"
+        : "=f"(x), "=f"(y)
+        : "r"(a), "r"(b), "l"(f), "l"(mu), "l"(kRound), "l"(kC5), "l"(kC4), "l"(kC3),
+          "l"(kC2), "l"(kC1), "l"(kC0));
+}
+
+// 16 scores of a row: MASK takes keys at or past lim out
+template <bool MASK>
+__device__ __forceinline__ void mask16(uint32_t (&r)[16], int lim) {
+    if (MASK) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e >= lim) r[e] = 0xff800000u;
+    }
+}
+__device__ __forceinline__ void max16(const uint32_t (&r)[16], float& m0, float& m1) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+        max3(m0, r[e], r[e + 1]);
+        max3(m1, r[e + 2], r[e + 3]);
+    }
+}
+// The weights of 16 scores over the scores' columns: 8 columns of high halves,
+// then 8 of low halves
+__device__ __forceinline__ void exp16(const uint32_t (&r)[16], uint32_t col, uint64_t f, uint64_t mu, uint64_t& s0,
+                                      uint64_t& s1) {
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        float a, b;
+        exp_pair(r[e], r[e + 1], f, mu, a, b);
+        add_pair((e & 2) ? s1 : s0, a, b);
+        split2(a, b, hi[e >> 1], lo[e >> 1]);
+    }
+    TMEM_ST8(col, hi);
+    TMEM_ST8(col + 8, lo);
+}
+
+// The two warpgroups take turns at the exponentials: one row tile's run while the
+// other's products do.  Left alone the two fall into step, and the tensor core
+// and the exponential unit wait for each other (4.2k cycles a key tile against
+// 2.9k in turns, fp16 queries).  Warpgroup 0 starts; a turn is passed on before
+// the last quarter of the exponentials.
+struct Turn {
+    uint64_t *mine, *other;   // other null: this tile has no partner
+    uint32_t phase;
+    bool wait;
+    int* err;
+    __device__ __forceinline__ bool take() const {
+        return !wait || mbar_wait(mine, phase, err, kDevTimeoutFull);
+    }
+    __device__ __forceinline__ void pass() const {
+        if (other && (threadIdx.x & 31) == 0) mbar_arrive(other);
+    }
+};
+
+// One arrival per warp: its rows' weights of 64 keys are in tensor memory.
+__device__ __forceinline__ void weights_ready(uint64_t* bar) {
+    tmem_wait_st();
+    tc_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// fp32 queries: softmax of one row against one key tile.  Two passes over the
+// scores in tensor memory (a row's 128 scores next to its 128 outputs would not
+// fit the registers): the maximum, then the exponentials.  Both loop over 32
+// scores as two loads of 16, the next in flight while one is worked on, and stay
+// rolled: unrolled, all the loads move to the top and their values spill.  MASK:
+// keys at or past lim count as -inf.  Returns the rescale of what came before.
+template <bool MASK>
+__device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, float& m, float& l, uint64_t* p_full,
+                                             const Turn& turn, bool& ok) {
+    uint32_t a[16], b[16];
+    float mx0 = -INFINITY, mx1 = -INFINITY;
+    TMEM_LD16(trow, a);
+    tmem_wait_ld();
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        TMEM_LD16(trow + 32 * c + 16, b);
+        mask16<MASK>(a, lim - 32 * c);
+        max16(a, mx0, mx1);
+        tmem_wait_ld();
+        TMEM_LD16(trow + ((32 * c + 32) & 127), a);   // after the last chunk: the first again, for the second pass
+        mask16<MASK>(b, lim - 32 * c - 16);
+        max16(b, mx0, mx1);
+        tmem_wait_ld();
+    }
+    const float mn = fmaxf(m, fmaxf(mx0, mx1) * f);
+    const float mu = mn == -INFINITY ? 0.f : mn - kPShift;
+    const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+    m = mn;
+    const uint64_t f2 = pair(f, f), mu2 = pair(-mu, -mu);
+    uint64_t s0 = 0, s1 = 0;
+    ok = turn.take();
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        if (c == 3) turn.pass();
+        TMEM_LD16(trow + 32 * c + 16, b);
+        mask16<MASK>(a, lim - 32 * c);
+        exp16(a, trow + 32 * c, f2, mu2, s0, s1);
+        tmem_wait_ld();
+        if (c < 3) TMEM_LD16(trow + 32 * c + 32, a);
+        mask16<MASK>(b, lim - 32 * c - 16);
+        exp16(b, trow + 32 * c + 16, f2, mu2, s0, s1);
+        tmem_wait_ld();
+        if (c & 1) weights_ready(p_full + (c >> 1));
+    }
+    const float2 u = unpair(s0), v = unpair(s1);
+    l = fmaf(l, corr, (u.x + u.y) + (v.x + v.y));
+    return corr;
+}
+
+// fp16 queries: the row's 128 scores in registers, its outputs in tensor memory.
+// The maximum in use may lag the row's by kLazy before the outputs are rescaled
+// (the weights then reach 2^(kPShift + kLazy), inside fp16): after the first
+// tiles that hardly happens.
+constexpr float kLazy = 5.f;
+template <bool MASK>
+__device__ __forceinline__ void softmax_row_f16(uint32_t trow, uint32_t orow, int lim, float f, bool first, float& m, float& l,
+                                                uint64_t* p_full, const Turn& turn, bool& ok) {
+    uint32_t s[kTile];
+    TMEM_LD32(trow, s);
+    TMEM_LD32(trow + 32, (s + 32));
+    TMEM_LD32(trow + 64, (s + 64));
+    TMEM_LD32(trow + 96, (s + 96));
+    tmem_wait_ld();
+    if (MASK) {
+#pragma unroll
+        for (int e = 0; e < kTile; ++e)
+            if (e >= lim) s[e] = 0xff800000u;
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < kTile; e += 2) max3(mx[(e >> 1) & 3], s[e], s[e + 1]);
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+    const bool grow = top > m + kLazy;
+    if (__any_sync(0xffffffffu, grow)) {   // each row by itself: its result does not depend on its neighbours
+        const float corr = grow ? ex2(m - top) : 1.f;
+        m = grow ? top : m;
+        l *= corr;
+        if (!first) {   // S of this tile is there, so the product before it is done
+            const uint64_t corr2 = pair(corr, corr);
+#pragma unroll 1
+            for (int c = 0; c < kHd; c += 16) {
+                uint32_t r[16];
+                TMEM_LD16(orow + c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) mul_pair(r[e], r[e + 1], corr2);
+                TMEM_ST16(orow + c, r);
+            }
+        }
+    }
+    const float mu = m == -INFINITY ? 0.f : m - kPShift;
+    const uint64_t f2 = pair(f, f), mu2 = pair(-mu, -mu);
+    uint64_t s0 = 0, s1 = 0;
+    ok = turn.take();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (c == 3) turn.pass();
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+            float a, b;
+            if (kPoly && (e & 6) == 6) poly_pair(s[32 * c + e], s[32 * c + e + 1], f2, mu2, a, b);
+            else exp_pair(s[32 * c + e], s[32 * c + e + 1], f2, mu2, a, b);
+            add_pair((e & 2) ? s1 : s0, a, b);
+            w[e >> 1] = pack2(a, b);
+        }
+        TMEM_ST16(trow + 16 * c, w);
+        if (c & 1) weights_ready(p_full + (c >> 1));
+    }
+    const float2 u = unpair(s0), v = unpair(s1);
+    l += (u.x + u.y) + (v.x + v.y);
+}
+
+// Bounded wait for a counter that only grows (a row tile may run ahead of the other
+// by any number of key tiles, which a barrier's one phase bit cannot tell).
+__device__ __forceinline__ bool wait_reads(const int* count, int target, int* err) {
+    const uint32_t a = smem_u32(count);
+    uint64_t t0 = 0;
+    for (int i = 0;; ++i) {
+        int v;
+        asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+        if (v >= target) return true;
+        if (i == 0) t0 = global_timer_ns();
+        else if ((i & 31) == 0 && global_timer_ns() - t0 > kWaitLimitNs) break;
+    }
+    if (err) atomicExch(err, kDevTimeoutFull);
+    return false;
+}
+
+// fp32 queries of a row tile (a warp's 32 rows): scaled, their high halves to shared
+// memory (64 dims a 128-byte swizzled row) and their low halves, by way of the same
+// place, to tensor memory.
+__device__ __forceinline__ void load_queries(const AttnBatch& p, TilesSmem& S, uint8_t* qt, uint32_t qlo, int t, int wrow,
+                                             int rows, int64_t tok_first, int g) {
+    const int lane = threadIdx.x & 31, c = lane >> 1;
+    float4 a[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const int r = wrow + i, tok = r / p.G, h = r - tok * p.G;
+        a[i] = r < rows ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + (tok_first + tok) * p.q_stride +
+                                                                (int64_t)(g * p.G + h) * kHd) +
+                                lane)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    uint8_t* d0 = qt + (c >> 3) * (kTileBytes / 2) + wrow * 128 + (lane & 1) * 8;
+    uint2 hi[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        float mx = fmaxf(fmaxf(fabsf(a[i].x), fabsf(a[i].y)), fmaxf(fabsf(a[i].z), fabsf(a[i].w)));
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        float up, fr;
+        row_scale(mx, p.scale_log2, up, fr);
+        if (lane == 0) S.f[t][wrow + i] = fr;
+        uint2 lo;
+        split2(a[i].x * up, a[i].y * up, hi[i].x, lo.x);
+        split2(a[i].z * up, a[i].w * up, hi[i].y, lo.y);
+        *reinterpret_cast<uint2*>(d0 + i * 128 + (((c & 7) ^ (i & 7)) << 4)) = lo;
+    }
+    __syncwarp();
+    // the thread's own row of low halves: 64 columns of fp16 pairs
+    const uint8_t* mine = qt + (wrow + lane) * 128;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint4 v = lds128(mine + h * (kTileBytes / 2) + (((4 * q + k) ^ (lane & 7)) << 4));
+                w[4 * k] = v.x;
+                w[4 * k + 1] = v.y;
+                w[4 * k + 2] = v.z;
+                w[4 * k + 3] = v.w;
+            }
+            TMEM_ST16(qlo + 32 * h + 16 * q, w);
+        }
+    tmem_wait_st();
+    tc_before();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) *reinterpret_cast<uint2*>(d0 + i * 128 + (((c & 7) ^ (i & 7)) << 4)) = hi[i];
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.q_full[t]);
+}
+
+// Parts of a unit: the last CTA to bring its own joins them (the 256 softmax
+// threads; phase counts the CTA's joins).  False when a wait gave up.
+template <bool F32>
+__device__ __forceinline__ bool join_parts(const AttnBatch& p, TilesSmem& S, const TileItem& it, int t, int tpt,
+                                           uint32_t phase) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.stored);
+    bool ok = true;
+    if (threadIdx.x == 0) {
+        ok = mbar_wait(&S.stored, phase & 1u, p.err, kDevTimeoutFull);
+        const bool last = ok && atom_add_acq_rel_gpu_u64(tile_count(p, it.slot), 1ull) + 1 == p.nonce + it.parts;
+        if (last) *tile_count(p, it.slot) = 0;
+        S.last = last;
+        mbar_arrive(&S.told);
+    }
+    __syncwarp();
+    ok = mbar_wait(&S.told, phase & 1u, p.err, kDevTimeoutFull) && ok;
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok || !S.last) return ok;
+    const float* part0 = p.tile_work + (size_t)it.slot * kTilePartFloats;
+    const int rows = it.ntok[t] * p.G, r0 = 32 * (warp & 3);
+#pragma unroll 1
+    for (int row = r0; row < min(rows, r0 + 32); ++row) {
+        const int r = kTcRows * t + row, tok = row / p.G;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < it.parts)
+            ml = __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)lane * kTilePartFloats + 2 * kTcRows * kHd + 2 * r));
+        float4 y[kMaxParts];
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i)
+            y[i] = i < it.parts
+                       ? __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)i * kTilePartFloats + (size_t)r * kHd) + lane)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+        float M = ml.x;
+#pragma unroll
+        for (int d = 4; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        M = __shfl_sync(0xffffffffu, M, 0);
+        const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M), kl = warp_sum(k * ml.y);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i) {
+            const float ki = __shfl_sync(0xffffffffu, k, i);
+            acc = make_float4(fmaf(y[i].x, ki, acc.x), fmaf(y[i].y, ki, acc.y), fmaf(y[i].z, ki, acc.z),
+                                  fmaf(y[i].w, ki, acc.w));
+        }
+        const bool none = min(it.kv_len, it.see0 + t * tpt + tok) <= 0;
+        const float inv = none ? 0.f : rcp(kl);
+        const int64_t off = (int64_t)(it.row0 + t * tpt + tok) * p.out_stride +
+                            (int64_t)(it.g * p.G + row - tok * p.G) * kHd + 4 * lane;
+        store_pair<F32>(p.out, off, make_float2(acc.x, acc.y), inv, none);
+        store_pair<F32>(p.out, off + 2, make_float2(acc.z, acc.w), inv, none);
+    }
+    return true;
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attn_tiles_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tv, const __grid_constant__ AttnBatch p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* qs = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);   // fp16 queries or high halves, [row tile][2 x 64 dims][128 rows]
+    uint8_t* ring = qs + 2 * kTileBytes;
+    TilesSmem& S = *reinterpret_cast<TilesSmem*>(ring + kSlots * kTileBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&S.kv_full[i], 1);
+            mbar_init(&S.kv_empty[i], 2);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&S.s_full[t], 1);
+            mbar_init(&S.p_full[t][0], 4);
+            mbar_init(&S.p_full[t][1], 4);
+            mbar_init(&S.o_full[t], 1);
+            S.reads[t] = 0;
+            mbar_init(&S.turn[t], 4);
+            mbar_init(&S.q_full[t], F32 ? 4 : 1);
+            mbar_init(&S.q_free[t], 1);
+            mbar_init(&S.drain[t], 1);
+        }
+        mbar_init(&S.landed, 1);
+        mbar_init(&S.stored, 8);
+        mbar_init(&S.told, 1);
+        for (int i = 0; i < kItemBufs; ++i) {
+            mbar_init(&S.item_full[i], 1);
+            mbar_init(&S.item_empty[i], 11);   // TMA, two issuers, eight softmax warps
+        }
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem)),
+                     "r"(kTcCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = S.tmem;
+    const int tpt = p.tokens_per_tile >> 1;   // tokens per row tile
+
+    // the i-th item of the CTA, for a role (a whole warp): false at the end
+    auto take = [&](int i, bool& ok) {
+        const int buf = i % kItemBufs;
+        ok = mbar_wait(&S.item_full[buf], (uint32_t)(i / kItemBufs) & 1u, p.err, kDevTimeoutFull);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok && S.item[buf].seq >= 0;
+    };
+    auto give = [&](int i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.item_empty[i % kItemBufs]);
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 11) {
+            // ------------------------------------------------------- next items
+            ItemWalk w;
+            w.init(p);
+            const int ctas = gridDim.x, c = blockIdx.x;
+            bool ok = true;
+            int i = 0;
+            for (int r = 0; ok; ++r) {
+                const int x = r * ctas + ((r & 1) ? ctas - 1 - c : c);
+                TileItem it;
+                if (r * ctas >= w.total) it.seq = -1;
+                else if (x >= w.total || !w.get(p, x, it)) continue;
+                const int buf = i % kItemBufs;
+                ok = mbar_wait_backoff(&S.item_empty[buf], ((uint32_t)(i / kItemBufs) & 1u) ^ 1u, p.err, kDevTimeoutEmpty,
+                                       64);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    if (it.seq >= 0 && it.parts > 1) part_open(tile_count(p, it.slot), p.nonce);
+                    S.item[buf] = it;
+                    mbar_arrive(&S.item_full[buf]);
+                }
+                __syncwarp();
+                ++i;
+                if (it.seq < 0) break;
+            }
+        } else if (warp == 8) {
+            // --------------------------------------------- Q (fp16), K and V tiles
+            const int ps = 1 << p.ps_log2, nbox = kTile / p.box_rows, halves = nbox == 1 ? 1 : 2;
+            const int box = lane / halves, half = lane - box * halves;
+            bool ok = true;
+            int slot = 0, landings = 0;         // K and V tiles so far, last ones of items among them
+            int nq[2] = {0, 0};
+            for (int i = 0; ok && take(i, ok); ++i) {
+                const TileItem& it = S.item[i % kItemBufs];
+                for (int j = 0; j < it.ntiles && ok; ++j) {
+                    const int r0 = (it.j0 + j) * kTile + box * p.box_rows;
+                    const bool mine = box < nbox && r0 < it.kv_end;
+                    const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+                    const uint32_t bytes = (uint32_t)(boxes * p.box_rows * (nbox == 1 ? 256 : 128));
+                    int page = 0, row = it.kv_row0 + r0;
+                    if (mine && p.table) {
+                        page = p.table[(long long)it.seq * p.max_pages + (r0 >> p.ps_log2)];
+                        row = r0 & (ps - 1);
+                        if ((unsigned)page >= (unsigned)p.n_pages) {  // reads as zeros
+                            atomicExch(p.err, kDevBadArg);
+                            page = p.n_pages;
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m, ++slot) {
+                        const int st = slot % kSlots;
+                        ok = mbar_wait_backoff(&S.kv_empty[st], ((uint32_t)(slot / kSlots) & 1u) ^ 1u, p.err,
+                                               kDevTimeoutEmpty, 32);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        // values past the last key may be anything, NaN included: zeros
+                        // before the tensor core reads them, so that tile lands on a
+                        // barrier of its own
+                        const bool tail = m == 1 && j == it.ntiles - 1 && it.kv_end < (it.j0 + j + 1) * kTile;
+                        uint64_t* bar = tail ? &S.landed : &S.kv_full[st];
+                        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+                        __syncwarp();
+                        uint8_t* dst = ring + st * kTileBytes;
+                        if (mine)
+                            tma_load_kv(dst + half * (kTileBytes / 2) + box * p.box_rows * 128, m ? &tv : &tk, half, row, it.g,
+                                        page, bar);
+                        __syncwarp();
+                        if (!F32 && m == 0 && j == 0) {   // the queries, once the products on the last ones are done
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                if (it.nt[t] > 0) {
+                                    if (nq[t]) ok = ok && mbar_wait(&S.q_free[t], (uint32_t)(nq[t] - 1) & 1u, p.err, kDevTimeoutEmpty);
+                                    ++nq[t];
+                                    if (ok && lane == 0) {
+                                        mbar_arrive_expect_tx(&S.q_full[t], (uint32_t)(2 * tpt * p.G * 128));
+                                        for (int h = 0; h < 2; ++h)
+                                            tma_load_q(qs + t * kTileBytes + h * (kTileBytes / 2), &tq, it.g * p.G,
+                                                       it.row0 + t * tpt, h, &S.q_full[t]);
+                                    }
+                                }
+                            ok = __all_sync(0xffffffffu, ok);
+                        }
+                        if (tail) {
+                            ok = ok && mbar_wait(&S.landed, (uint32_t)landings & 1u, p.err, kDevTimeoutFull);
+                            ++landings;
+                            for (int r = it.kv_end - (it.j0 + j) * kTile + (lane >> 3); r < kTile; r += 4)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    *reinterpret_cast<uint4*>(dst + h * (kTileBytes / 2) + r * 128 + (lane & 7) * 16) =
+                                        make_uint4(0u, 0u, 0u, 0u);
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&S.kv_full[st]);
+                            ok = __all_sync(0xffffffffu, ok);
+                        }
+                    }
+                }
+                give(i);
+            }
+            // the copies in flight land before the CTA can exit
+            if (lane == 0) {
+                drain_issued_stages(S.kv_full, kSlots, slot, kWaitLimitNs);
+                if (!F32)
+                    for (int t = 0; t < 2; ++t)
+                        if (nq[t]) mbar_wait(&S.q_full[t], (uint32_t)(nq[t] - 1) & 1u, nullptr, 0);
+            }
+        } else {
+            // ------------------------------------------------------------- MMA
+            // One issuer per row tile: an issuing thread's waits queue behind its
+            // own products (~200 cycles each, measured), and the other issuer's
+            // products run meanwhile.
+            const int t = warp - 9;
+            const uint32_t qb = desc_k(smem_u32(qs + t * kTileBytes));
+            const uint32_t s_col = tmem + 128u * t, o_col = tmem + kColO + (F32 ? 0u : 128u * t), q_col = tmem + kColQlo + 64u * t;
+            auto wait_kv = [&](int i) {
+                return mbar_wait(&S.kv_full[i % kSlots], (uint32_t)(i / kSlots) & 1u, p.err, kDevTimeoutFull);
+            };
+            auto qk = [&](int i) {   // S = Q K^T
+                const uint32_t kb = desc_k(smem_u32(ring + (i % kSlots) * kTileBytes));
+#pragma unroll
+                for (int part = F32 ? 1 : 0; part >= 0; --part)
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t off = ((uint32_t)(ks >> 2) * (kTileBytes / 2) + (uint32_t)(ks & 3) * 32u) >> 4;
+                        const uint32_t acc = (ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u;
+                        if (part) mma_ts(s_col, q_col + 8u * ks, kb + off, kIdescS, acc);
+                        else mma_ss(s_col, qb + off, kb + off, kIdescS, acc);
+                    }
+                tc_arrive(&S.s_full[t]);
+            };
+            auto pv = [&](int i, int half, bool fresh) {   // PV (+)= P V over 64 of the tile's keys
+                const uint32_t vb = desc_mn(smem_u32(ring + (i % kSlots) * kTileBytes)) + (uint32_t)half * (8192u >> 4);
+#pragma unroll
+                for (int part = F32 ? 1 : 0; part >= 0; --part)
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint32_t col = (uint32_t)(4 * half + ks) * (F32 ? 16u : 8u) + 8u * part;
+                        mma_ts(o_col, s_col + col, vb + (uint32_t)ks * (2048u >> 4), kIdescO,
+                               (fresh && ks == 0 && part == (F32 ? 1 : 0)) ? 0u : 1u);
+                    }
+            };
+            bool ok = true;
+            int slot = 0, tiles = 0, nq = 0, others = 0;   // ring places, this row tile's key tiles, queries, the other's tiles
+            for (int i = 0; ok && take(i, ok); ++i) {
+                const TileItem& it = S.item[i % kItemBufs];
+                const int mine = it.nt[t], theirs = it.nt[t ^ 1];
+                if (lane == 0 && it.ntiles > 0) {
+                    if (mine > 0) ok = mbar_wait(&S.q_full[t], (uint32_t)nq & 1u, p.err, kDevTimeoutFull);
+                    ok = ok && wait_kv(slot);
+                    tc_after();
+                    if (ok) {
+                        if (mine > 0) qk(slot);
+                        if (mine == 1) tc_arrive(&S.q_free[t]);
+                        tc_arrive(&S.kv_empty[slot % kSlots]);
+                    }
+                    for (int j = 0; j < it.ntiles && ok; ++j) {
+                        const int iv = slot + 2 * j + 1, ik = iv + 1;
+                        const bool more = j + 1 < it.ntiles;
+                        ok = wait_kv(iv);
+                        // the next keys too, while the weights are on their way
+                        if (ok && more) ok = wait_kv(ik);
+                        if (j < mine) {
+                            if (F32) {   // the other row tile's last PV has been read
+                                const int reads = others + min(j + t, theirs);
+                                if (reads) ok = ok && wait_reads(&S.reads[t ^ 1], 4 * reads, p.err);
+                            }
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                ok = ok && mbar_wait(&S.p_full[t][half], (uint32_t)(tiles + j) & 1u, p.err, kDevTimeoutFull);
+                                if (!ok) break;
+                                tc_after();
+                                pv(iv, half, half == 0 && (F32 || j == 0));
+                            }
+                            if (ok && (F32 || j + 1 == mine)) tc_arrive(&S.o_full[t]);
+                        }
+                        if (!ok) break;
+                        if (j + 1 < mine) {
+                            qk(ik);
+                            if (j + 2 == mine) tc_arrive(&S.q_free[t]);
+                        }
+                        tc_arrive(&S.kv_empty[iv % kSlots]);
+                        if (more) tc_arrive(&S.kv_empty[ik % kSlots]);
+                    }
+                    nq += mine > 0;
+                    tiles += mine;
+                    others += theirs;
+                    slot += 2 * it.ntiles;
+                }
+                give(i);
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            // every product is done before the CTA frees its tensor memory
+            if (lane == 0) {
+                tc_arrive(&S.drain[t]);
+                mbar_wait(&S.drain[t], 0, nullptr, 0, kWaitLimitNs);
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = warp >> 2, wrow = 32 * (warp & 3), row = wrow + lane, tok = row / p.G;
+        const uint32_t trow = tmem + 128u * t + ((uint32_t)wrow << 16);
+        const uint32_t orow = tmem + kColO + (F32 ? 0u : 128u * t) + ((uint32_t)wrow << 16);
+        int tiles = 0, outs = 0, turns = 0, joins = 0;
+        bool ok = true;
+        for (int i = 0; ok && take(i, ok); ++i) {
+            const TileItem& it = S.item[i % kItemBufs];
+            const int rows = it.ntok[t] * p.G, nt = it.nt[t];
+            if (F32 && nt > 0)
+                load_queries(p, S, qs + t * kTileBytes, tmem + kColQlo + 64u * t + ((uint32_t)wrow << 16), t, wrow, rows,
+                             it.row0 + t * tpt, it.g);
+
+            // --------------------------------------------------------- softmax
+            const bool live = row < rows;
+            const int see = it.see0 + t * tpt;                       // keys the row tile's first token sees
+            const int lim = live ? max(0, min(it.kv_len, see + tok)) : 0, lim0 = max(0, see);
+            const float f = F32 ? S.f[t][row] : p.scale_log2;
+            // (addresses are formed after the loops, which need the registers)
+            auto out_off = [&] {
+                return ((int64_t)it.row0 + t * tpt + tok) * p.out_stride + (int64_t)(it.g * p.G + row - tok * p.G) * kHd;
+            };
+            auto part_out = [&] { return p.tile_work + (size_t)(it.slot + it.part) * kTilePartFloats; };
+            float m = -INFINITY, l = 0.f;
+            const int both = min(it.nt[0], it.nt[1]);
+            auto turn_of = [&](int j) {   // warpgroup 0 waits for 1's last turn, 1 for 0's of the same tile
+                const int n = turns + j;
+                return Turn{&S.turn[t], j < both ? &S.turn[t ^ 1] : nullptr, (uint32_t)(n - 1 + t) & 1u,
+                            j < both && n + t > 0, p.err};
+            };
+            if constexpr (F32) {
+                uint64_t o[kHd / 2];   // the row's outputs in pairs
+#pragma unroll
+                for (int d = 0; d < kHd / 2; ++d) o[d] = 0;
+                for (int j = 0; j < nt; ++j) {
+                    const uint32_t ph = (uint32_t)(tiles + j) & 1u;
+                    ok = mbar_wait(&S.s_full[t], ph, p.err, kDevTimeoutFull);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_after();
+                    const Turn turn = turn_of(j);
+                    const int k0 = (it.j0 + j) * kTile;
+                    const float corr = k0 + kTile > lim0 ? softmax_row<true>(trow, lim - k0, f, m, l, S.p_full[t], turn, ok)
+                                                         : softmax_row<false>(trow, 0, f, m, l, S.p_full[t], turn, ok);
+                    ok = ok && mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_after();
+                    const uint64_t corr2 = pair(corr, corr);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        // the barrier once more: a branch that keeps the later loads from
+                        // moving to the top, where their values would spill
+                        if (c == 2 && !mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull)) ok = false;
+                        uint32_t r[32];
+                        TMEM_LD32(orow + 32 * c, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) fma_pair(o[16 * c + e], corr2, r[2 * e], r[2 * e + 1]);
+                    }
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        asm volatile("red.release.cta.shared::cta.add.s32 [%0], 1;" ::"r"(smem_u32(&S.reads[t])) : "memory");
+                }
+                if (ok && live) {
+                    if (it.parts > 1) {   // unnormalised, to the workspace
+                        float* x = part_out();
+                        *reinterpret_cast<float2*>(x + 2 * kTcRows * kHd + 2 * (kTcRows * t + row)) = make_float2(m, l);
+                        uint4* d = reinterpret_cast<uint4*>(x + (size_t)(kTcRows * t + row) * kHd);
+                        const uint64_t one = pair(1.f, 1.f);
+#pragma unroll
+                        for (int e = 0; e < kHd / 2; e += 2) store_f32(d + e / 2, o[e], o[e + 1], one);
+                    } else {
+                        uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + out_off());
+                        if (lim > 0) {
+                            const float rl = rcp(l);
+                            const uint64_t inv = pair(rl, rl);
+#pragma unroll
+                            for (int e = 0; e < kHd / 2; e += 2) store_f32(d + e / 2, o[e], o[e + 1], inv);
+                        } else {   // no key seen
+#pragma unroll
+                            for (int e = 0; e < kHd / 4; ++e) d[e] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                }
+            } else {
+                for (int j = 0; j < nt; ++j) {
+                    ok = mbar_wait(&S.s_full[t], (uint32_t)(tiles + j) & 1u, p.err, kDevTimeoutFull);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_after();
+                    const Turn turn = turn_of(j);
+                    const int k0 = (it.j0 + j) * kTile;
+                    if (k0 + kTile > lim0)
+                        softmax_row_f16<true>(trow, orow, lim - k0, f, j == 0, m, l, S.p_full[t], turn, ok);
+                    else softmax_row_f16<false>(trow, orow, 0, f, j == 0, m, l, S.p_full[t], turn, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                if (ok && nt > 0) {
+                    ok = mbar_wait(&S.o_full[t], (uint32_t)outs & 1u, p.err, kDevTimeoutFull);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_after();
+                    ++outs;
+                }
+                if (ok) {
+                    if (it.parts > 1 && live)
+                        *reinterpret_cast<float2*>(part_out() + 2 * kTcRows * kHd + 2 * (kTcRows * t + row)) = make_float2(m, l);
+                    const float rl = rcp(l);
+                    uint4* d = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + out_off());
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t r[32];
+                        if (nt > 0) TMEM_LD32(orow + 32 * c, r);
+                        tmem_wait_ld();
+                        if (it.parts > 1) {   // unnormalised, to the workspace
+                            uint4* x = reinterpret_cast<uint4*>(part_out() + (size_t)(kTcRows * t + row) * kHd + 32 * c);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                if (live)
+                                    x[e >> 2] = nt > 0 ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3])
+                                                       : make_uint4(0u, 0u, 0u, 0u);
+                            __syncwarp();
+                            continue;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                            if (lim > 0) {
+                                u.x = pack2(__uint_as_float(r[e]) * rl, __uint_as_float(r[e + 1]) * rl);
+                                u.y = pack2(__uint_as_float(r[e + 2]) * rl, __uint_as_float(r[e + 3]) * rl);
+                                u.z = pack2(__uint_as_float(r[e + 4]) * rl, __uint_as_float(r[e + 5]) * rl);
+                                u.w = pack2(__uint_as_float(r[e + 6]) * rl, __uint_as_float(r[e + 7]) * rl);
+                            }
+                            if (live) d[4 * c + (e >> 3)] = u;
+                        }
+                        __syncwarp();
+                    }
+                    tc_before();   // the next item's products may overwrite the outputs
+                }
+            }
+            tiles += nt;
+            turns += both;
+            if (ok && it.parts > 1) ok = join_parts<F32>(p, S, it, t, tpt, (uint32_t)joins++);
+            give(i);
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcCols) : "memory");
+    }
+}
+
+template <bool F32>
+int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, long long items,
+           cudaStream_t st) {
+    constexpr int smem = tiles_smem_bytes<F32>();
+    static_assert(smem <= 232448, "shared memory of a CTA");
+    cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) {
+        attn_tiles_kernel<F32><<<(unsigned)std::min<long long>(items, 148), kTcThreads, smem, st>>>(tq, tk, tv, p);
+        e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
+    return GLC_OK;
+}
+
+}  // namespace
+
+int attn_tiles_launch(bool f32, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p,
+                      long long items, cudaStream_t st) {
+    return f32 ? launch<true>(tq, tk, tv, p, items, st) : launch<false>(tq, tk, tv, p, items, st);
+}
+
+}  // namespace glc

@@ -83,8 +83,8 @@ typedef CUresult (*PFN_encodeTiledKv)(CUtensorMap*, CUtensorMapDataType, cuuint3
                                       const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                       CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-int paged_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_stride, int64_t heads,
-                     int64_t head_stride, int64_t pages, int64_t page_stride, int box_rows, int box_halves) {
+int paged_encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                 const cuuint32_t* box) {
     static PFN_encodeTiledKv fn = [] {
         void* ptr = nullptr;
         cudaDriverEntryPointQueryResult qr;
@@ -94,16 +94,21 @@ int paged_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t r
         return (PFN_encodeTiledKv)ptr;
     }();
     if (!fn) return paged_fail(GLC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box,
+                          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return paged_fail(GLC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return GLC_OK;
+}
+
+int paged_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_stride, int64_t heads,
+                     int64_t head_stride, int64_t pages, int64_t page_stride, int box_rows, int box_halves) {
     const cuuint64_t dims[5] = {64, (cuuint64_t)rows, 2, (cuuint64_t)heads, (cuuint64_t)pages};
     const cuuint64_t strides[4] = {(cuuint64_t)row_stride * 2, 128, (cuuint64_t)head_stride * 2,
                                    (cuuint64_t)page_stride * 2};
     const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_halves, 1, 1};
-    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return paged_fail(GLC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return GLC_OK;
+    return paged_encode(map, base, 5, dims, strides, box);
 }
 
 namespace {

@@ -26,6 +26,10 @@ int paged_check_device(const void* device_ptr, const char* what);
 // The shape, strides and alignment rules of a page set.
 int paged_check_pages(const glc_kv_pages* c);
 
+// A 128-byte swizzled fp16 descriptor (strides in bytes, one less than the rank).
+int paged_encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                 const cuuint32_t* box);
+
 // A descriptor of 128-wide fp16 rows as [pages][heads][2 halves][rows][64]:
 // a box is `box_rows` rows of `box_halves` 64-element halves of one head of
 // one page, 128-byte swizzled.  Rows and pages past the end read as zeros.

@@ -256,6 +256,32 @@ def test_prompt_matches_oracle(cuda, glc, lens, Hq, Hkv, pad, qt):
 
 
 @pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("lens,Hq,Hkv", [
+    ([517, 1, 700, 130, 0, 63, 199, 300, 257, 64, 301, 333], 48, 8), ([3, 140, 1, 90, 250] * 9, 32, 8),
+    ([1] * 170 + [40] * 30, 8, 8), ([30, 3] * 100, 16, 4), ([129, 1, 260] * 12, 8, 8)])
+def test_prompt_many_items(cuda, glc, lens, Hq, Hkv, qt):
+    """More items than SMs, with and without a second row tile: one CTA works
+    through several.  Sequences are checked one in five (the oracle is slow), and
+    all of them against themselves alone, bit for bit."""
+    torch = cuda
+    rng = np.random.default_rng(len(lens))
+    T, cu = sum(lens), np.concatenate([[0], np.cumsum(lens)])
+    q = rng.standard_normal((T, Hq, 128)).astype(NP[qt])
+    k, v = (rng.standard_normal((T, Hkv, 128)).astype(np.float16) for _ in range(2))
+    got = run_prompt(torch, glc, q, k, v, cu, qt).reshape(T, Hq, 128)
+    for b in range(len(lens)):
+        s = slice(cu[b], cu[b + 1])
+        if not lens[b]:
+            continue
+        if b % 5 == 0 and lens[b] < 600:
+            h = slice(0, 2 * Hq // Hkv)          # two KV heads
+            check_attention(got[s][:, h], q[s][:, h], k[s][:, :2], v[s][:, :2], 0, qt == F32)
+        if lens[b] * Hq // Hkv > 16:             # the tile kernel by itself
+            alone = run_prompt(torch, glc, q[s], k[s], v[s], [0, lens[b]], qt).reshape(lens[b], Hq, 128)
+            assert np.array_equal(alone, got[s]), b
+
+
+@pytest.mark.parametrize("qt", [F32, F16])
 def test_prompt_neighbours_do_not_leak(cuda, glc, qt):
     """A sequence of NaN and infinities between two others changes neither."""
     rng = np.random.default_rng(4)
