@@ -34,10 +34,6 @@ constexpr uint32_t kTcCols = 512;
 constexpr uint32_t kColO = 256, kColQlo = 384;
 constexpr int kSlots = 5;                 // K and V tiles in flight
 constexpr int kItemBufs = 2;
-#ifndef KPOLY
-#define KPOLY 0
-#endif
-constexpr bool kPoly = KPOLY;
 
 // Few units with many keys: a unit's key tiles are cut into up to kMaxParts parts
 // of kMinPart tiles or more, one item each, whose partials (unnormalised outputs,
@@ -348,28 +344,6 @@ __device__ __forceinline__ void add_pair(uint64_t& s, float a, float b) {
 __device__ __forceinline__ void max3(float& m, uint32_t a, uint32_t b) {
     asm volatile("max.f32 %0, %0, %1, %2;" : "+f"(m) : "r"(a), "r"(b));
 }
-// The same without the exponential unit, on the fp32 pipe: x = n + r with n the
-// nearest integer (adding 1.5 * 2^23 leaves it in the low bits) and |r| <= 1/2, a
-// polynomial for 2^r and n added to its exponent.  The coefficients are a minimax
-// fit of the relative error on [-1/2, 1/2] (Remez exchange): 2^-22.1 in fp32.  x is
-// held above -127, where the result is nothing to an fp16 weight.
-__device__ __forceinline__ void poly_pair(uint32_t a, uint32_t b, uint64_t f, uint64_t mu, float& x, float& y) {
-    constexpr uint64_t kC5 = 0x3aae04733aae0473ull, kC4 = 0x3c1e86293c1e8629ull, kC3 = 0x3d635b723d635b72ull,
-                       kC2 = 0x3e75fc8c3e75fc8cull, kC1 = 0x3f3172143f317214ull, kC0 = 0x3f8000013f800001ull,
-                       kRound = 0x4b4000004b400000ull;
-    asm volatile(
-        "{\n\t.reg .b64 t, n, q;\n\t.reg .b32 ta, tb, na, nb;\n\t"
-        "mov.b64 t, {%2, %3};\n\tfma.rn.f32x2 t, t, %4, %5;\n\t"
-        "mov.b64 {ta, tb}, t;\n\tmax.f32 ta, ta, 0fC2FE0000;\n\tmax.f32 tb, tb, 0fC2FE0000;\n\tmov.b64 t, {ta, tb};\n\t"
-        "add.rn.f32x2 n, t, %6;\n\tsub.rn.f32x2 q, n, %6;\n\tsub.rn.f32x2 t, t, q;\n\t"
-        "fma.rn.f32x2 q, t, %7, %8;\n\tfma.rn.f32x2 q, q, t, %9;\n\tfma.rn.f32x2 q, q, t, %10;\n\t"
-        "fma.rn.f32x2 q, q, t, %11;\n\tfma.rn.f32x2 q, q, t, %12;\n\t"
-        "mov.b64 {ta, tb}, q;\n\tmov.b64 {na, nb}, n;\n\t"
-        "shl.b32 na, na, 23;\n\tshl.b32 nb, nb, 23;\n\tadd.s32 na, ta, na;\n\tadd.s32 nb, tb, nb;\n\tmov.b32 %0, na;\n\tmov.b32 %1, nb;\n\t}"
-        : "=f"(x), "=f"(y)
-        : "r"(a), "r"(b), "l"(f), "l"(mu), "l"(kRound), "l"(kC5), "l"(kC4), "l"(kC3),
-          "l"(kC2), "l"(kC1), "l"(kC0));
-}
 
 // 16 scores of a row: MASK takes keys at or past lim out
 template <bool MASK>
@@ -392,29 +366,29 @@ __device__ __forceinline__ void max16(const uint32_t (&r)[16], float& m0, float&
 __device__ __forceinline__ void exp16(const uint32_t (&r)[16], uint32_t col, uint64_t f, uint64_t mu, uint64_t& s0,
                                       uint64_t& s1) {
     uint32_t hi[8], lo[8];
+    float a[16];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) exp_pair(r[e], r[e + 1], f, mu, a[e], a[e + 1]);
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-        float a, b;
-        exp_pair(r[e], r[e + 1], f, mu, a, b);
-        add_pair((e & 2) ? s1 : s0, a, b);
-        split2(a, b, hi[e >> 1], lo[e >> 1]);
+        add_pair((e & 2) ? s1 : s0, a[e], a[e + 1]);
+        split2(a[e], a[e + 1], hi[e >> 1], lo[e >> 1]);
     }
     TMEM_ST8(col, hi);
     TMEM_ST8(col + 8, lo);
 }
 
-// The two warpgroups take turns at the exponentials: one row tile's run while the
-// other's products do.  Left alone the two fall into step, and the tensor core
-// and the exponential unit wait for each other (4.2k cycles a key tile against
-// 2.9k in turns, fp16 queries).  Warpgroup 0 starts; a turn is passed on before
-// the last quarter of the exponentials.
+// fp32 queries: the two warpgroups take turns at the exponentials, one row tile's
+// run while the other's products do.  Left alone the two fall into step, and the
+// tensor core and the exponential unit wait for each other.  Warpgroup 0 starts;
+// a turn is passed on before the last quarter of the exponentials.
 struct Turn {
     uint64_t *mine, *other;   // other null: this tile has no partner
     uint32_t phase;
     bool wait;
     int* err;
     __device__ __forceinline__ bool take() const {
-        return !wait || mbar_wait(mine, phase, err, kDevTimeoutFull);
+        return !wait || mbar_wait_spin(mine, phase, err, kDevTimeoutFull);
     }
     __device__ __forceinline__ void pass() const {
         if (other && (threadIdx.x & 31) == 0) mbar_arrive(other);
@@ -480,9 +454,10 @@ __device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, fl
 
 // fp16 queries: the row's 128 scores in registers, its outputs in tensor memory.
 // The maximum in use may lag the row's by kLazy before the outputs are rescaled
-// (the weights then reach 2^(kPShift + kLazy), inside fp16): after the first
-// tiles that hardly happens.
-constexpr float kLazy = 5.f;
+// (the weights, kept as 2^kShift16 p, then reach 2^15, inside fp16): after the
+// first tiles that hardly happens (a lag of 2^5 was overtaken by one of a warp's
+// 32 rows in most tiles).
+constexpr float kShift16 = 4.f, kLazy = 11.f;
 template <bool MASK>
 __device__ __forceinline__ void softmax_row_f16(uint32_t trow, uint32_t orow, int lim, float f, bool first, float& m, float& l,
                                                 uint64_t* p_full, const Turn& turn, bool& ok) {
@@ -519,7 +494,7 @@ __device__ __forceinline__ void softmax_row_f16(uint32_t trow, uint32_t orow, in
             }
         }
     }
-    const float mu = m == -INFINITY ? 0.f : m - kPShift;
+    const float mu = m == -INFINITY ? 0.f : m - kShift16;
     const uint64_t f2 = pair(f, f), mu2 = pair(-mu, -mu);
     uint64_t s0 = 0, s1 = 0;
     ok = turn.take();
@@ -530,8 +505,7 @@ __device__ __forceinline__ void softmax_row_f16(uint32_t trow, uint32_t orow, in
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
             float a, b;
-            if (kPoly && (e & 6) == 6) poly_pair(s[32 * c + e], s[32 * c + e + 1], f2, mu2, a, b);
-            else exp_pair(s[32 * c + e], s[32 * c + e + 1], f2, mu2, a, b);
+            exp_pair(s[32 * c + e], s[32 * c + e + 1], f2, mu2, a, b);
             add_pair((e & 2) ? s1 : s0, a, b);
             w[e >> 1] = pack2(a, b);
         }
@@ -565,27 +539,48 @@ __device__ __forceinline__ void load_queries(const AttnBatch& p, TilesSmem& S, u
                                              int rows, int64_t tok_first, int g) {
     const int lane = threadIdx.x & 31, c = lane >> 1;
     float4 a[32];
+    {
+        const int tok = wrow / p.G;
+        int h = wrow - tok * p.G;
+        const float* src = static_cast<const float*>(p.q) + (tok_first + tok) * p.q_stride + (int64_t)(g * p.G + h) * kHd;
+        const int64_t next_token = p.q_stride - (int64_t)(p.G - 1) * kHd;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const int r = wrow + i, tok = r / p.G, h = r - tok * p.G;
-        a[i] = r < rows ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + (tok_first + tok) * p.q_stride +
-                                                                (int64_t)(g * p.G + h) * kHd) +
-                                lane)
-                        : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < 32; ++i) {
+            a[i] = wrow + i < rows ? __ldg(reinterpret_cast<const float4*>(src) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const bool wrap = ++h == p.G;
+            src += wrap ? next_token : kHd;
+            h = wrap ? 0 : h;
+        }
     }
+    // largest value of each row: 32 values a lane to one, lane i row i, by halving
+    // (31 shuffles; a butterfly a row takes 160)
+    float v[16];
+    {
+        auto top = [&](int i) {
+            return fmaxf(fmaxf(fabsf(a[i].x), fabsf(a[i].y)), fmaxf(fabsf(a[i].z), fabsf(a[i].w)));
+        };
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float x = top(i), y = top(16 + i);
+            v[i] = fmaxf(lane & 16 ? y : x, __shfl_xor_sync(0xffffffffu, lane & 16 ? x : y, 16));
+        }
+#pragma unroll
+        for (int w = 8; w >= 1; w >>= 1)
+#pragma unroll
+            for (int i = 0; i < w; ++i)
+                v[i] = fmaxf(lane & w ? v[w + i] : v[i], __shfl_xor_sync(0xffffffffu, lane & w ? v[i] : v[w + i], w));
+    }
+    float up, fr;
+    row_scale(v[0], p.scale_log2, up, fr);
+    S.f[t][wrow + lane] = fr;
     uint8_t* d0 = qt + (c >> 3) * (kTileBytes / 2) + wrow * 128 + (lane & 1) * 8;
     uint2 hi[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-        float mx = fmaxf(fmaxf(fabsf(a[i].x), fabsf(a[i].y)), fmaxf(fabsf(a[i].z), fabsf(a[i].w)));
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-        float up, fr;
-        row_scale(mx, p.scale_log2, up, fr);
-        if (lane == 0) S.f[t][wrow + i] = fr;
+        const float u = __shfl_sync(0xffffffffu, up, i);
         uint2 lo;
-        split2(a[i].x * up, a[i].y * up, hi[i].x, lo.x);
-        split2(a[i].z * up, a[i].w * up, hi[i].y, lo.y);
+        split2(a[i].x * u, a[i].y * u, hi[i].x, lo.x);
+        split2(a[i].z * u, a[i].w * u, hi[i].y, lo.y);
         *reinterpret_cast<uint2*>(d0 + i * 128 + (((c & 7) ^ (i & 7)) << 4)) = lo;
     }
     __syncwarp();
@@ -638,36 +633,64 @@ __device__ __forceinline__ bool join_parts(const AttnBatch& p, TilesSmem& S, con
     if (!ok || !S.last) return ok;
     const float* part0 = p.tile_work + (size_t)it.slot * kTilePartFloats;
     const int rows = it.ntok[t] * p.G, r0 = 32 * (warp & 3);
-#pragma unroll 1
-    for (int row = r0; row < min(rows, r0 + 32); ++row) {
-        const int r = kTcRows * t + row, tok = row / p.G;
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < it.parts)
-            ml = __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)lane * kTilePartFloats + 2 * kTcRows * kHd + 2 * r));
-        float4 y[kMaxParts];
+    // lane i: the parts' weights in row r0 + i
+    float k[kMaxParts], M = -INFINITY, L = 0.f;
+    {
+        float2 ml[kMaxParts];
 #pragma unroll
         for (int i = 0; i < kMaxParts; ++i)
-            y[i] = i < it.parts
-                       ? __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)i * kTilePartFloats + (size_t)r * kHd) + lane)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-        float M = ml.x;
+            ml[i] = i < it.parts && r0 + lane < rows
+                        ? __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)i * kTilePartFloats + 2 * kTcRows * kHd) +
+                                 kTcRows * t + r0 + lane)
+                        : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int d = 4; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        M = __shfl_sync(0xffffffffu, M, 0);
-        const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M), kl = warp_sum(k * ml.y);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < kMaxParts; ++i) M = fmaxf(M, ml[i].x);
 #pragma unroll
         for (int i = 0; i < kMaxParts; ++i) {
-            const float ki = __shfl_sync(0xffffffffu, k, i);
-            acc = make_float4(fmaf(y[i].x, ki, acc.x), fmaf(y[i].y, ki, acc.y), fmaf(y[i].z, ki, acc.z),
-                                  fmaf(y[i].w, ki, acc.w));
+            k[i] = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - M);
+            L = fmaf(k[i], ml[i].y, L);
         }
-        const bool none = min(it.kv_len, it.see0 + t * tpt + tok) <= 0;
-        const float inv = none ? 0.f : rcp(kl);
-        const int64_t off = (int64_t)(it.row0 + t * tpt + tok) * p.out_stride +
-                            (int64_t)(it.g * p.G + row - tok * p.G) * kHd + 4 * lane;
-        store_pair<F32>(p.out, off, make_float2(acc.x, acc.y), inv, none);
-        store_pair<F32>(p.out, off + 2, make_float2(acc.z, acc.w), inv, none);
+        // a row that sees no key: zeros
+        const float inv = min(it.kv_len, it.see0 + t * tpt + (r0 + lane) / p.G) > 0 ? rcp(L) : 0.f;
+#pragma unroll
+        for (int i = 0; i < kMaxParts; ++i) k[i] = inv == 0.f ? 0.f : k[i] * inv;
+    }
+#pragma unroll 1
+    for (int i0 = 0; i0 < 32 && r0 + i0 < rows; i0 += 4) {   // four rows at once, lane d dims 4 d ..
+        float4 acc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < kMaxParts; q += 4) {
+            if (q >= it.parts) break;
+            float4 y[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    y[c][i] = q + c < it.parts && r0 + i0 + i < rows
+                                  ? __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)(q + c) * kTilePartFloats +
+                                                                           (size_t)(kTcRows * t + r0 + i0 + i) * kHd) +
+                                           lane)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float w = __shfl_sync(0xffffffffu, k[q + c], i0 + i);
+                    acc[i] = make_float4(fmaf(y[c][i].x, w, acc[i].x), fmaf(y[c][i].y, w, acc[i].y),
+                                         fmaf(y[c][i].z, w, acc[i].z), fmaf(y[c][i].w, w, acc[i].w));
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = r0 + i0 + i, tok = row / p.G;
+            if (row >= rows) break;
+            const int64_t off = (int64_t)(it.row0 + t * tpt + tok) * p.out_stride +
+                                (int64_t)(it.g * p.G + row - tok * p.G) * kHd + 4 * lane;
+            store_pair<F32>(p.out, off, make_float2(acc[i].x, acc[i].y), 1.f, false);
+            store_pair<F32>(p.out, off + 2, make_float2(acc[i].z, acc[i].w), 1.f, false);
+        }
     }
     return true;
 }
@@ -849,7 +872,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t qb = desc_k(smem_u32(qs + t * kTileBytes));
             const uint32_t s_col = tmem + 128u * t, o_col = tmem + kColO + (F32 ? 0u : 128u * t), q_col = tmem + kColQlo + 64u * t;
             auto wait_kv = [&](int i) {
-                return mbar_wait(&S.kv_full[i % kSlots], (uint32_t)(i / kSlots) & 1u, p.err, kDevTimeoutFull);
+                return mbar_wait_spin(&S.kv_full[i % kSlots], (uint32_t)(i / kSlots) & 1u, p.err, kDevTimeoutFull);
             };
             auto qk = [&](int i) {   // S = Q K^T
                 const uint32_t kb = desc_k(smem_u32(ring + (i % kSlots) * kTileBytes));
@@ -881,7 +904,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const TileItem& it = S.item[i % kItemBufs];
                 const int mine = it.nt[t], theirs = it.nt[t ^ 1];
                 if (lane == 0 && it.ntiles > 0) {
-                    if (mine > 0) ok = mbar_wait(&S.q_full[t], (uint32_t)nq & 1u, p.err, kDevTimeoutFull);
+                    if (mine > 0) ok = mbar_wait_spin(&S.q_full[t], (uint32_t)nq & 1u, p.err, kDevTimeoutFull);
                     ok = ok && wait_kv(slot);
                     tc_after();
                     if (ok) {
@@ -902,18 +925,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             }
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
-                                ok = ok && mbar_wait(&S.p_full[t][half], (uint32_t)(tiles + j) & 1u, p.err, kDevTimeoutFull);
+                                ok = ok && mbar_wait_spin(&S.p_full[t][half], (uint32_t)(tiles + j) & 1u, p.err, kDevTimeoutFull);
                                 if (!ok) break;
                                 tc_after();
                                 pv(iv, half, half == 0 && (F32 || j == 0));
                             }
-                            if (ok && (F32 || j + 1 == mine)) tc_arrive(&S.o_full[t]);
-                        }
-                        if (!ok) break;
-                        if (j + 1 < mine) {
-                            qk(ik);
+                            if (!ok) break;
+                            if (F32 || j + 1 == mine) tc_arrive(&S.o_full[t]);
+                            if (j + 1 < mine) qk(ik);
                             if (j + 2 == mine) tc_arrive(&S.q_free[t]);
                         }
+                        if (!ok) break;
                         tc_arrive(&S.kv_empty[iv % kSlots]);
                         if (more) tc_arrive(&S.kv_empty[ik % kSlots]);
                     }
@@ -969,7 +991,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int d = 0; d < kHd / 2; ++d) o[d] = 0;
                 for (int j = 0; j < nt; ++j) {
                     const uint32_t ph = (uint32_t)(tiles + j) & 1u;
-                    ok = mbar_wait(&S.s_full[t], ph, p.err, kDevTimeoutFull);
+                    ok = mbar_wait_spin(&S.s_full[t], ph, p.err, kDevTimeoutFull);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_after();
@@ -977,7 +999,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int k0 = (it.j0 + j) * kTile;
                     const float corr = k0 + kTile > lim0 ? softmax_row<true>(trow, lim - k0, f, m, l, S.p_full[t], turn, ok)
                                                          : softmax_row<false>(trow, 0, f, m, l, S.p_full[t], turn, ok);
-                    ok = ok && mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull);
+                    ok = ok && mbar_wait_spin(&S.o_full[t], ph, p.err, kDevTimeoutFull);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_after();
@@ -986,7 +1008,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int c = 0; c < 4; ++c) {
                         // the barrier once more: a branch that keeps the later loads from
                         // moving to the top, where their values would spill
-                        if (c == 2 && !mbar_wait(&S.o_full[t], ph, p.err, kDevTimeoutFull)) ok = false;
+                        if (c == 2 && !mbar_wait_spin(&S.o_full[t], ph, p.err, kDevTimeoutFull)) ok = false;
                         uint32_t r[32];
                         TMEM_LD32(orow + 32 * c, r);
                         tmem_wait_ld();
@@ -1021,7 +1043,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             } else {
                 for (int j = 0; j < nt; ++j) {
-                    ok = mbar_wait(&S.s_full[t], (uint32_t)(tiles + j) & 1u, p.err, kDevTimeoutFull);
+                    ok = mbar_wait_spin(&S.s_full[t], (uint32_t)(tiles + j) & 1u, p.err, kDevTimeoutFull);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_after();
@@ -1029,12 +1051,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int k0 = (it.j0 + j) * kTile;
                     if (k0 + kTile > lim0)
                         softmax_row_f16<true>(trow, orow, lim - k0, f, j == 0, m, l, S.p_full[t], turn, ok);
-                    else softmax_row_f16<false>(trow, orow, 0, f, j == 0, m, l, S.p_full[t], turn, ok);
+                    else
+                        softmax_row_f16<false>(trow, orow, 0, f, j == 0, m, l, S.p_full[t], turn, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
                 if (ok && nt > 0) {
-                    ok = mbar_wait(&S.o_full[t], (uint32_t)outs & 1u, p.err, kDevTimeoutFull);
+                    ok = mbar_wait_spin(&S.o_full[t], (uint32_t)outs & 1u, p.err, kDevTimeoutFull);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_after();
                     ++outs;

@@ -91,11 +91,14 @@ def attend_tolerance(out, wv, peak, mag, L, f32):
     maximum (3 more), and for fp32 queries the two halves' 2^-22; numerator and
     denominator both feel it.  The exponential is good to 2^-21.  A weight is
     rounded to fp16 (2^-11) or kept as two halves (2^-21), with an absolute
-    floor of 2^-34 of the row's largest.  The sum over keys takes L / 16 steps
+    floor: fp16's half step below its normal range is 2^-25, and weights are
+    kept as 2^4 p (fp16 queries on tiles) or 2^10 p, p relative to a value not
+    above the row's largest: 2^-29 (fp16) or 2^-35 of the largest, doubled
+    for the sum's share.  The sum over keys takes L / 16 steps
     of at most 32 roundings, and rescaling and merging at most 32 more.  The
     output is rounded once to its type."""
     score = mag * (27 * 2.0 ** -23 + (2.0 ** -21 if f32 else 0.0))
     weight = 2 * score + 2.0 ** -20 + (2.0 ** -21 if f32 else 2.0 ** -11)
     total = weight + (L / 16 + 64) * 2.0 ** -23
     final = 2.0 ** -24 if f32 else 2.0 ** -11
-    return wv * total + np.abs(out) * final + peak * 2.0 ** -33 + (1e-30 if f32 else 2.0 ** -25)
+    return wv * total + np.abs(out) * final + peak * (2.0 ** -34 if f32 else 2.0 ** -28) + (1e-30 if f32 else 2.0 ** -25)
