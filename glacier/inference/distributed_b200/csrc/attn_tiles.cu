@@ -149,38 +149,55 @@ constexpr uint32_t kIdescO = kIdescS | (1u << 16);                              
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Units and key tiles of sequence b.
-__device__ __forceinline__ void seq_tiles(const AttnBatch& p, int b, int& units, int& tiles) {
-    units = tiles = 0;
-    if (b >= p.B || b < 0) return;
-    int first, n;
-    seq_rows(p, b, first, n);
-    if (n * p.G <= p.rows_take) return;   // none, or the row kernel's
-    units = (n + p.tokens_per_tile - 1) / p.tokens_per_tile * p.n_kv;
+// Units of sequence b whose key tiles number up to x: the tiles a unit sees grow along
+// the sequence.
+struct SeqUnits {
+    int n, kv_len, per;           // new tokens, keys, tokens of a unit
+    __device__ __forceinline__ int upto(int x) const {
+        const int all = (n + per - 1) / per;
+        if (x < 0) return 0;
+        if (kv_len <= x * (long long)kTile) return all;
+        const long long t = (long long)x * kTile - (kv_len - n);   // tokens whose keys fit x tiles
+        return t <= 0 ? 0 : (int)min((long long)all - 1, t / per);
+    }
+};
+__device__ __forceinline__ SeqUnits seq_units(const AttnBatch& p, int b) {
+    SeqUnits u{0, 0, p.tokens_per_tile};
+    if (b < 0 || b >= p.B) return u;
+    int first;
+    seq_rows(p, b, first, u.n);
+    if (u.n * p.G <= p.rows_take) u.n = 0;   // none, or the row kernel's
     const long long room = (long long)p.max_pages << p.ps_log2;
-    const int len = p.kv_lens ? (int)min((long long)max(p.kv_lens[b], 0), room) : n;
-    tiles = (len + kTile - 1) / kTile;
+    u.kv_len = p.kv_lens ? (int)min((long long)max(p.kv_lens[b], 0), room) : u.n;
+    return u;
 }
 
-// Walks a CTA's items (one warp).  Sequences are taken from the batch's end and
-// tiles from a sequence's end: the last ones see the most keys, so they come first
-// and the short ones fill the gaps; CTA c takes items c, 2 * CTAs - 1 - c, and so
-// on back and forth, which evens the sums out.
+// Walks a CTA's items (one warp), long ones first: the units in kBuckets classes of
+// their key tiles, from the class with the most down, the sequences of a class
+// from the batch's end.  CTA c takes items c, 2 * CTAs - 1 - c, and so on back and
+// forth, which evens the sums out.
 //
-// With a workspace, keys are cut into parts of L tiles: of the longest sequence's
-// tiles in 1 to 8 parts, the L with the least rounds of all CTAs times L, 3 % more
-// for each further part's own prologue and join.
+// With a workspace, keys are cut into parts of up to L tiles: of the longest
+// sequence's tiles in 1 to 8 parts, the L with the least rounds of all CTAs times
+// an item's cost, in key tiles: its own, two for its prologue and epilogue, and
+// three and half a tile a part for the join.
+constexpr int kBuckets = 16;
 struct ItemWalk {
-    int L, total;                 // tiles of a part, items in all
-    int b0, before, slots;        // chunk of 32 sequences: the one of lane 0, items and places before it
-    int parts, count, split, end, send, chunk, schunk;   // of the lane's sequence; sums of the chunk
+    int L, most, total;           // tiles of a part, of the longest unit; items in all
+    int bucket, b0, before, slots;   // class; chunk of 32 sequences (the one of lane 0); items and places before it
+    int low, units, parts, count, split, end, send, chunk, schunk;   // of the lane's sequence; sums of the chunk
+
+    __device__ __forceinline__ int parts_of(int tiles) const { return max(1, (tiles - 1) / L + 1); }
 
     __device__ __forceinline__ void load(const AttnBatch& p) {
         const int lane = threadIdx.x & 31;
-        int units, tiles;
-        seq_tiles(p, b0 - lane, units, tiles);
-        parts = max(1, (tiles - 1) / L + 1);
-        count = units * parts;
+        const SeqUnits u = seq_units(p, b0 - lane);
+        // classes (lo, hi] of key tiles; the last one takes units without keys too
+        const int hi = (int)((long long)most * (bucket + 1) / kBuckets), lo = bucket ? (int)((long long)most * bucket / kBuckets) : -1;
+        low = u.upto(lo);
+        units = u.n > 0 ? u.upto(hi) - low : 0;
+        parts = parts_of((u.kv_len + kTile - 1) / kTile);
+        count = units * p.n_kv * parts;
         split = parts > 1 ? count : 0;
         end = count;
         send = split;
@@ -199,16 +216,16 @@ struct ItemWalk {
     __device__ __forceinline__ void init(const AttnBatch& p) {
         const int lane = threadIdx.x & 31;
         L = 0x7fffffff;
-        int most = 0, units_all = 0;
+        most = total = 0;
         for (int c = 0; c < p.B; c += 32) {
-            int units, tiles;
-            seq_tiles(p, c + lane, units, tiles);
-            most = max(most, tiles);
-            units_all += units;
+            const SeqUnits u = seq_units(p, c + lane);
+            if (u.n > 0) {
+                most = max(most, (u.kv_len + kTile - 1) / kTile);
+                total += (u.n + u.per - 1) / u.per * p.n_kv;
+            }
         }
-        units_all = __reduce_add_sync(0xffffffffu, units_all);
+        total = __reduce_add_sync(0xffffffffu, total);
         most = __reduce_max_sync(0xffffffffu, most);
-        total = units_all;
         if (p.split && most > kMinPart) {
             int len[kMaxParts], n[kMaxParts];
 #pragma unroll
@@ -217,24 +234,25 @@ struct ItemWalk {
                 n[i] = 0;
             }
             for (int c = 0; c < p.B; c += 32) {
-                int units, tiles;
-                seq_tiles(p, c + lane, units, tiles);
+                const SeqUnits u = seq_units(p, c + lane);
+                const int units = (u.n + u.per - 1) / u.per * p.n_kv, tiles = (u.kv_len + kTile - 1) / kTile;
 #pragma unroll
                 for (int i = 0; i < kMaxParts; ++i) n[i] += units * max(1, (tiles + len[i] - 1) / len[i]);
             }
             float best = 3.4e38f;
-            const int ctas = gridDim.x;
+            const int ctas = gridDim.x, whole = total;
 #pragma unroll
             for (int i = 0; i < kMaxParts; ++i) {
                 n[i] = __reduce_add_sync(0xffffffffu, n[i]);
-                const float cost = (float)((n[i] + ctas - 1) / ctas) * (float)len[i] * (1.f + 0.03f * i);
-                if (cost < best && n[i] - units_all <= kMaxExtra) {
+                const float cost = (float)((n[i] + ctas - 1) / ctas) * ((float)len[i] + 2.f + (i ? 3.5f + 0.5f * i : 0.f));
+                if (cost < best && n[i] - whole <= kMaxExtra) {
                     best = cost;
                     L = len[i];
                     total = n[i];
                 }
             }
         }
+        bucket = kBuckets - 1;
         b0 = p.B - 1;
         before = slots = 0;
         load(p);
@@ -242,21 +260,25 @@ struct ItemWalk {
 
     // item x (ascending from call to call); false when this one has no work
     __device__ __forceinline__ bool get(const AttnBatch& p, int x, TileItem& it) {
-        while (before + chunk <= x) {   // x < total, so a chunk holds it
+        while (before + chunk <= x) {
             before += chunk;
             slots += schunk;
             b0 -= 32;
+            if (b0 < 0) {
+                if (--bucket < 0) return false;   // (x < total: a chunk holds it)
+                b0 = p.B - 1;
+            }
             load(p);
         }
         const int l = __ffs(__ballot_sync(0xffffffffu, before + end > x)) - 1;
-        const int np = __shfl_sync(0xffffffffu, parts, l), nu = __shfl_sync(0xffffffffu, count, l) / np;
+        const int np = __shfl_sync(0xffffffffu, parts, l), nu = __shfl_sync(0xffffffffu, units, l);
         const int in = x - before - __shfl_sync(0xffffffffu, end - count, l);
-        const int u = in / np, part = in - u * np;            // unit of the sequence, from its end
+        const int u = in / np, part = in - u * np;            // unit of the class's, from its end
         const int slot = slots + __shfl_sync(0xffffffffu, send - split, l) + u * np;
         const int tpt = p.tokens_per_tile >> 1;
         it.seq = b0 - l;
         it.g = u % p.n_kv;
-        const int tok0 = (nu / p.n_kv - 1 - u / p.n_kv) * p.tokens_per_tile;
+        const int tok0 = (__shfl_sync(0xffffffffu, low, l) + nu - 1 - u / p.n_kv) * p.tokens_per_tile;
         int first, n;
         seq_rows(p, it.seq, first, n);
         it.kv_len = n;
@@ -281,7 +303,7 @@ struct ItemWalk {
         // a tile early in its sequence has fewer parts
         const int all = max(nt[0], nt[1]);
         it.part = part;
-        it.parts = min(np, max(1, (all - 1) / L + 1));
+        it.parts = min(np, parts_of(all));
         it.slot = slot;
         if (part >= it.parts) return false;
         it.j0 = (int)((long long)all * part / it.parts);
@@ -660,28 +682,24 @@ __device__ __forceinline__ bool join_parts(const AttnBatch& p, TilesSmem& S, con
         float4 acc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 y[kMaxParts][4];
 #pragma unroll
-        for (int q = 0; q < kMaxParts; q += 4) {
-            if (q >= it.parts) break;
-            float4 y[4][4];
+        for (int c = 0; c < kMaxParts; ++c)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int i = 0; i < 4; ++i)
+                y[c][i] = c < it.parts && r0 + i0 + i < rows
+                              ? __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)c * kTilePartFloats +
+                                                                       (size_t)(kTcRows * t + r0 + i0 + i) * kHd) +
+                                       lane)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    y[c][i] = q + c < it.parts && r0 + i0 + i < rows
-                                  ? __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)(q + c) * kTilePartFloats +
-                                                                           (size_t)(kTcRows * t + r0 + i0 + i) * kHd) +
-                                           lane)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < kMaxParts; ++c)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w = __shfl_sync(0xffffffffu, k[q + c], i0 + i);
-                    acc[i] = make_float4(fmaf(y[c][i].x, w, acc[i].x), fmaf(y[c][i].y, w, acc[i].y),
-                                         fmaf(y[c][i].z, w, acc[i].z), fmaf(y[c][i].w, w, acc[i].w));
-                }
-        }
+            for (int i = 0; i < 4; ++i) {
+                const float w = __shfl_sync(0xffffffffu, k[c], i0 + i);
+                acc[i] = make_float4(fmaf(y[c][i].x, w, acc[i].x), fmaf(y[c][i].y, w, acc[i].y),
+                                     fmaf(y[c][i].z, w, acc[i].z), fmaf(y[c][i].w, w, acc[i].w));
+            }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = r0 + i0 + i, tok = row / p.G;
