@@ -122,6 +122,7 @@ constexpr int kTileRows = 256;                  // query rows of an item of the 
 constexpr int kTileParts = 8;                   // most parts of a unit's keys
 constexpr int kTileExtra = 3 * 148;             // most items that cutting units into parts adds
 constexpr int kTilePartFloats = kTileRows * (kHd + 2);
+constexpr int kTileUnitBytes = 32;              // a place's entry for the join
 int attn_rows_launch(bool f32, const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p, cudaStream_t st);
 // tq: the fp16 queries (unused with fp32 ones)
 int attn_tiles_launch(bool f32, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnBatch& p,

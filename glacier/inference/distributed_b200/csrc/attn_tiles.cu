@@ -20,6 +20,7 @@
 // leave room for five K or V tiles in flight.
 // Warps 0-7: softmax; 8: TMA; 9 and 10: MMA issue; 11: the next items.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn.cuh"
 
@@ -37,8 +38,11 @@ constexpr int kItemBufs = 2;
 
 // Few units with many keys: a unit's key tiles are cut into up to kMaxParts parts
 // of kMinPart tiles or more, one item each, whose partials (unnormalised outputs,
-// maximum, sum) are joined through the workspace.  At most kMaxExtra items more
-// than there are units, so twice as many places.
+// maximum, sum) go to the workspace and are joined by a second launch.  (The last
+// CTA of a unit joining them itself took 30 to 45 thousand cycles for 256 rows of
+// five parts: with nearly all of the first-level cache given to shared memory an SM
+// loads 25 bytes a cycle.)  At most kMaxExtra items more than there are units, so
+// twice as many places.
 constexpr int kMaxParts = kTileParts, kMinPart = 8, kMaxExtra = kTileExtra;
 
 // One item, as the roles need it.
@@ -57,10 +61,9 @@ struct TileItem {
 struct TilesSmem {
     float f[2][kTcRows];                  // score factor of each row
     uint64_t kv_full[kSlots], kv_empty[kSlots], s_full[2], p_full[2][2], o_full[2], turn[2], q_full[2], q_free[2], landed,
-        stored, told, item_full[kItemBufs], item_empty[kItemBufs], drain[2];
+        item_full[kItemBufs], item_empty[kItemBufs], drain[2];
     uint32_t tmem;
     int reads[2];                         // fp32: PV tiles read by each row tile's four warps, counted per warp
-    int last;
     TileItem item[kItemBufs];
 };
 template <bool F32>
@@ -68,8 +71,16 @@ constexpr int tiles_smem_bytes() {
     return 2 * kTileBytes + kSlots * kTileBytes + (int)sizeof(TilesSmem) + 1024;
 }
 
-__device__ __forceinline__ unsigned long long* tile_count(const AttnBatch& p, int slot) {
-    return reinterpret_cast<unsigned long long*>(p.work + kRowsWorkBytes / sizeof(float)) + slot;
+// Places of the workspace in use, and what each holds, for the launch that joins the
+// parts: a unit whose keys are cut at the place of its first part, nothing at the
+// others.  Every place in use is written by every call.
+struct TileUnit {
+    int parts, g, row0, see0, kv_len, ntok[2];   // parts 0: nothing
+};
+static_assert(sizeof(TileUnit) <= kTileUnitBytes, "places of the units");
+__device__ __forceinline__ int* tile_places(const AttnBatch& p) { return reinterpret_cast<int*>(p.work + kRowsWorkBytes / sizeof(float)); }
+__device__ __forceinline__ TileUnit* tile_unit(const AttnBatch& p, int slot) {
+    return reinterpret_cast<TileUnit*>(tile_places(p) + (slot + 1) * (kTileUnitBytes / (int)sizeof(int)));
 }
 
 __device__ __forceinline__ void tma_load_q(void* dst, const CUtensorMap* tm, int head, int token, int half, uint64_t* bar) {
@@ -179,11 +190,11 @@ __device__ __forceinline__ SeqUnits seq_units(const AttnBatch& p, int b) {
 //
 // With a workspace, keys are cut into parts of up to L tiles: of the longest
 // sequence's tiles in 1 to 8 parts, the L with the least rounds of all CTAs times
-// an item's cost, in key tiles: its own, two for its prologue and epilogue, and
-// three and half a tile a part for the join.
+// an item's cost, in key tiles: its own, two for its prologue and epilogue, and a
+// third of one for each part that the join reads.
 constexpr int kBuckets = 16;
 struct ItemWalk {
-    int L, most, total;           // tiles of a part, of the longest unit; items in all
+    int L, most, total, cut;      // tiles of a part, of the longest unit; items in all, and those of cut units
     int bucket, b0, before, slots;   // class; chunk of 32 sequences (the one of lane 0); items and places before it
     int low, units, parts, count, split, end, send, chunk, schunk;   // of the lane's sequence; sums of the chunk
 
@@ -216,7 +227,7 @@ struct ItemWalk {
     __device__ __forceinline__ void init(const AttnBatch& p) {
         const int lane = threadIdx.x & 31;
         L = 0x7fffffff;
-        most = total = 0;
+        most = total = cut = 0;
         for (int c = 0; c < p.B; c += 32) {
             const SeqUnits u = seq_units(p, c + lane);
             if (u.n > 0) {
@@ -239,16 +250,26 @@ struct ItemWalk {
 #pragma unroll
                 for (int i = 0; i < kMaxParts; ++i) n[i] += units * max(1, (tiles + len[i] - 1) / len[i]);
             }
+            int c[kMaxParts] = {};        // items of the units that are cut
+            for (int b = 0; b < p.B; b += 32) {
+                const SeqUnits u = seq_units(p, b + lane);
+                const int units = (u.n + u.per - 1) / u.per * p.n_kv, tiles = (u.kv_len + kTile - 1) / kTile;
+#pragma unroll
+                for (int i = 0; i < kMaxParts; ++i)
+                    if (tiles > len[i]) c[i] += units * ((tiles + len[i] - 1) / len[i]);
+            }
             float best = 3.4e38f;
             const int ctas = gridDim.x, whole = total;
 #pragma unroll
             for (int i = 0; i < kMaxParts; ++i) {
                 n[i] = __reduce_add_sync(0xffffffffu, n[i]);
-                const float cost = (float)((n[i] + ctas - 1) / ctas) * ((float)len[i] + 2.f + (i ? 3.5f + 0.5f * i : 0.f));
+                c[i] = __reduce_add_sync(0xffffffffu, c[i]);
+                const float cost = (float)((n[i] + ctas - 1) / ctas) * ((float)len[i] + 2.f) + 0.33f * i;
                 if (cost < best && n[i] - whole <= kMaxExtra) {
                     best = cost;
                     L = len[i];
                     total = n[i];
+                    cut = c[i];
                 }
             }
         }
@@ -305,16 +326,21 @@ struct ItemWalk {
         it.part = part;
         it.parts = min(np, parts_of(all));
         it.slot = slot;
+        if (np > 1) {
+            // first rows that do not ascend may name more units than the workspace has room for
+            if (slot + np > p.slots) {
+                if ((threadIdx.x & 31) == 0) atomicExch(p.err, kDevBadArg);
+                return false;
+            }
+            if ((threadIdx.x & 31) == 0)
+                *tile_unit(p, slot + part) = TileUnit{part == 0 && it.parts > 1 ? it.parts : 0, it.g, it.row0, it.see0, it.kv_len,
+                                                      {it.ntok[0], it.ntok[1]}};
+        }
         if (part >= it.parts) return false;
         it.j0 = (int)((long long)all * part / it.parts);
         it.ntiles = (int)((long long)all * (part + 1) / it.parts) - it.j0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) it.nt[t] = max(0, min(nt[t], it.j0 + it.ntiles) - it.j0);
-        // first rows that do not ascend may name more units than the workspace has room for
-        if (it.parts > 1 && slot + np > p.slots) {
-            if ((threadIdx.x & 31) == 0) atomicExch(p.err, kDevBadArg);
-            return false;
-        }
         return true;
     }
 };
@@ -633,38 +659,35 @@ __device__ __forceinline__ void load_queries(const AttnBatch& p, TilesSmem& S, u
     if (lane == 0) mbar_arrive(&S.q_full[t]);
 }
 
-// Parts of a unit: the last CTA to bring its own joins them (the 256 softmax
-// threads; phase counts the CTA's joins).  False when a wait gave up.
+// A partial: [row tile][32 groups of 4 dims][128 rows][4], then (maximum, sum) of each
+// row: a warp's rows are neighbours, for the thread that holds one and for the join.
+template <typename T>
+__device__ __forceinline__ auto part_at(T* part, int t, int d4, int row) {
+    using V = std::conditional_t<std::is_const_v<T>, const float4, float4>;
+    return reinterpret_cast<V*>(part) + (t * (kHd / 4) + d4) * kTcRows + row;
+}
+
+// Joins the parts of the units that were cut: 32 rows of a unit at a time, a row a
+// lane, a warp four groups of four dims.
+constexpr int kJoinCtas = 4 * 148;
 template <bool F32>
-__device__ __forceinline__ bool join_parts(const AttnBatch& p, TilesSmem& S, const TileItem& it, int t, int tpt,
-                                           uint32_t phase) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&S.stored);
-    bool ok = true;
-    if (threadIdx.x == 0) {
-        ok = mbar_wait(&S.stored, phase & 1u, p.err, kDevTimeoutFull);
-        const bool last = ok && atom_add_acq_rel_gpu_u64(tile_count(p, it.slot), 1ull) + 1 == p.nonce + it.parts;
-        if (last) *tile_count(p, it.slot) = 0;
-        S.last = last;
-        mbar_arrive(&S.told);
-    }
-    __syncwarp();
-    ok = mbar_wait(&S.told, phase & 1u, p.err, kDevTimeoutFull) && ok;
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok || !S.last) return ok;
-    const float* part0 = p.tile_work + (size_t)it.slot * kTilePartFloats;
-    const int rows = it.ntok[t] * p.G, r0 = 32 * (warp & 3);
-    // lane i: the parts' weights in row r0 + i
-    float k[kMaxParts], M = -INFINITY, L = 0.f;
-    {
+__global__ void __launch_bounds__(256, 4) attn_tiles_join_kernel(const __grid_constant__ AttnBatch p) {
+    grid_dep_wait();
+    const int places = *tile_places(p), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tpt = p.tokens_per_tile >> 1;
+    for (int w = blockIdx.x; w < 8 * places; w += kJoinCtas) {
+        const TileUnit u = *tile_unit(p, w >> 3);
+        const int t = (w >> 2) & 1, row = 32 * (w & 3) + lane;
+        if (u.parts == 0 || row >= u.ntok[t] * p.G) continue;
+        const float* part0 = p.tile_work + (size_t)(w >> 3) * kTilePartFloats;
+        const int tok = row / p.G;
+        const int64_t off = (int64_t)(u.row0 + t * tpt + tok) * p.out_stride + (int64_t)(u.g * p.G + row - tok * p.G) * kHd;
+        float k[kMaxParts], M = -INFINITY, L = 0.f;
         float2 ml[kMaxParts];
 #pragma unroll
         for (int i = 0; i < kMaxParts; ++i)
-            ml[i] = i < it.parts && r0 + lane < rows
-                        ? __ldcg(reinterpret_cast<const float2*>(part0 + (size_t)i * kTilePartFloats + 2 * kTcRows * kHd) +
-                                 kTcRows * t + r0 + lane)
-                        : make_float2(-INFINITY, 0.f);
+            ml[i] = i < u.parts ? *(reinterpret_cast<const float2*>(part0 + (size_t)i * kTilePartFloats + 2 * kTcRows * kHd) +
+                                    kTcRows * t + row)
+                                : make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int i = 0; i < kMaxParts; ++i) M = fmaxf(M, ml[i].x);
 #pragma unroll
@@ -672,45 +695,22 @@ __device__ __forceinline__ bool join_parts(const AttnBatch& p, TilesSmem& S, con
             k[i] = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - M);
             L = fmaf(k[i], ml[i].y, L);
         }
-        // a row that sees no key: zeros
-        const float inv = min(it.kv_len, it.see0 + t * tpt + (r0 + lane) / p.G) > 0 ? rcp(L) : 0.f;
+        const bool none = min(u.kv_len, u.see0 + t * tpt + tok) <= 0;   // a row that sees no key: zeros
+        const float inv = none ? 0.f : rcp(L);
+#pragma unroll 2
+        for (int d = 4 * warp; d < 4 * warp + 4; ++d) {
+            float4 y[kMaxParts], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < kMaxParts; ++i) k[i] = inv == 0.f ? 0.f : k[i] * inv;
-    }
-#pragma unroll 1
-    for (int i0 = 0; i0 < 32 && r0 + i0 < rows; i0 += 4) {   // four rows at once, lane d dims 4 d ..
-        float4 acc[4];
+            for (int c = 0; c < kMaxParts; ++c)
+                y[c] = c < u.parts ? *part_at(part0 + (size_t)c * kTilePartFloats, t, d, row) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        float4 y[kMaxParts][4];
-#pragma unroll
-        for (int c = 0; c < kMaxParts; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                y[c][i] = c < it.parts && r0 + i0 + i < rows
-                              ? __ldcg(reinterpret_cast<const float4*>(part0 + (size_t)c * kTilePartFloats +
-                                                                       (size_t)(kTcRows * t + r0 + i0 + i) * kHd) +
-                                       lane)
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int c = 0; c < kMaxParts; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float w = __shfl_sync(0xffffffffu, k[c], i0 + i);
-                acc[i] = make_float4(fmaf(y[c][i].x, w, acc[i].x), fmaf(y[c][i].y, w, acc[i].y),
-                                     fmaf(y[c][i].z, w, acc[i].z), fmaf(y[c][i].w, w, acc[i].w));
-            }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = r0 + i0 + i, tok = row / p.G;
-            if (row >= rows) break;
-            const int64_t off = (int64_t)(it.row0 + t * tpt + tok) * p.out_stride +
-                                (int64_t)(it.g * p.G + row - tok * p.G) * kHd + 4 * lane;
-            store_pair<F32>(p.out, off, make_float2(acc[i].x, acc[i].y), 1.f, false);
-            store_pair<F32>(p.out, off + 2, make_float2(acc[i].z, acc[i].w), 1.f, false);
+            for (int c = 0; c < kMaxParts; ++c)
+                acc = make_float4(fmaf(y[c].x, k[c], acc.x), fmaf(y[c].y, k[c], acc.y), fmaf(y[c].z, k[c], acc.z),
+                                  fmaf(y[c].w, k[c], acc.w));
+            store_pair<F32>(p.out, off + 4 * d, make_float2(acc.x, acc.y), inv, none);
+            store_pair<F32>(p.out, off + 4 * d + 2, make_float2(acc.z, acc.w), inv, none);
         }
     }
-    return true;
 }
 
 template <bool F32>
@@ -740,8 +740,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&S.drain[t], 1);
         }
         mbar_init(&S.landed, 1);
-        mbar_init(&S.stored, 8);
-        mbar_init(&S.told, 1);
         for (int i = 0; i < kItemBufs; ++i) {
             mbar_init(&S.item_full[i], 1);
             mbar_init(&S.item_empty[i], 11);   // TMA, two issuers, eight softmax warps
@@ -758,6 +756,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
     tc_after();
     const uint32_t tmem = S.tmem;
+    grid_dep_launch_dependents();
     const int tpt = p.tokens_per_tile >> 1;   // tokens per row tile
 
     // the i-th item of the CTA, for a role (a whole warp): false at the end
@@ -778,6 +777,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ------------------------------------------------------- next items
             ItemWalk w;
             w.init(p);
+            if (p.split && blockIdx.x == 0 && lane == 0) *tile_places(p) = min(w.cut, p.slots);
             const int ctas = gridDim.x, c = blockIdx.x;
             bool ok = true;
             int i = 0;
@@ -792,7 +792,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (lane == 0) {
-                    if (it.seq >= 0 && it.parts > 1) part_open(tile_count(p, it.slot), p.nonce);
                     S.item[buf] = it;
                     mbar_arrive(&S.item_full[buf]);
                 }
@@ -977,7 +976,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int t = warp >> 2, wrow = 32 * (warp & 3), row = wrow + lane, tok = row / p.G;
         const uint32_t trow = tmem + 128u * t + ((uint32_t)wrow << 16);
         const uint32_t orow = tmem + kColO + (F32 ? 0u : 128u * t) + ((uint32_t)wrow << 16);
-        int tiles = 0, outs = 0, turns = 0, joins = 0;
+        int tiles = 0, outs = 0, turns = 0;
         bool ok = true;
         for (int i = 0; ok && take(i, ok); ++i) {
             const TileItem& it = S.item[i % kItemBufs];
@@ -1042,10 +1041,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (it.parts > 1) {   // unnormalised, to the workspace
                         float* x = part_out();
                         *reinterpret_cast<float2*>(x + 2 * kTcRows * kHd + 2 * (kTcRows * t + row)) = make_float2(m, l);
-                        uint4* d = reinterpret_cast<uint4*>(x + (size_t)(kTcRows * t + row) * kHd);
                         const uint64_t one = pair(1.f, 1.f);
 #pragma unroll
-                        for (int e = 0; e < kHd / 2; e += 2) store_f32(d + e / 2, o[e], o[e + 1], one);
+                        for (int e = 0; e < kHd / 2; e += 2)
+                            store_f32(reinterpret_cast<uint4*>(part_at(x, t, e / 2, row)), o[e], o[e + 1], one);
                     } else {
                         uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + out_off());
                         if (lim > 0) {
@@ -1091,12 +1090,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         if (nt > 0) TMEM_LD32(orow + 32 * c, r);
                         tmem_wait_ld();
                         if (it.parts > 1) {   // unnormalised, to the workspace
-                            uint4* x = reinterpret_cast<uint4*>(part_out() + (size_t)(kTcRows * t + row) * kHd + 32 * c);
+                            uint4* x = reinterpret_cast<uint4*>(part_at(part_out(), t, 8 * c, row));
 #pragma unroll
                             for (int e = 0; e < 32; e += 4)
                                 if (live)
-                                    x[e >> 2] = nt > 0 ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3])
-                                                       : make_uint4(0u, 0u, 0u, 0u);
+                                    x[(e >> 2) * kTcRows] = nt > 0 ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3])
+                                                                   : make_uint4(0u, 0u, 0u, 0u);
                             __syncwarp();
                             continue;
                         }
@@ -1118,7 +1117,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             tiles += nt;
             turns += both;
-            if (ok && it.parts > 1) ok = join_parts<F32>(p, S, it, t, tpt, (uint32_t)joins++);
             give(i);
         }
     }
@@ -1139,6 +1137,18 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
     if (e == cudaSuccess) {
         attn_tiles_kernel<F32><<<(unsigned)std::min<long long>(items, 148), kTcThreads, smem, st>>>(tq, tk, tv, p);
         e = cudaGetLastError();
+    }
+    if (e == cudaSuccess && p.split) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(kJoinCtas);
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, attn_tiles_join_kernel<F32>, p);
     }
     if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "attention: %s", cudaGetErrorString(e));
     return GLC_OK;
