@@ -8,6 +8,8 @@
 // partials are joined in warp order); two more stream the pages with TMA
 // into a ring of six 32 KB slots, one the keys, one the values.  Products run as mma.sync m16n8k16 with
 // fp32 accumulators: 16 rows cannot fill a 128-row tensor-memory tile.
+#include <type_traits>
+
 #include "attn.cuh"
 
 namespace glc {
@@ -37,13 +39,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 // A unit is one KV head of one sequence; its keys come in tiles of 128.  The
 // tiles of all units, one unit after another, are cut into kRowCtas equal runs,
 // one CTA each: every SM streams the same number of bytes whatever the lengths.
-// A run holds whole units, which are finished in place, and at most two that it
-// shares with its neighbours; their partials go to the workspace, two places a
-// CTA, and the last CTA to bring its own joins them in key order.
+// A unit counts kUnitOver tiles more than it has, one before and one behind, for its
+// queries and its merge (3.5k cycles against 2k a tile).  A run holds whole units,
+// which are finished in place, and at most two that it shares with its neighbours;
+// their partials go to the workspace, two places a CTA, and the last CTA to bring
+// its own joins them in key order.
+constexpr int kUnitOver = 2;
 constexpr int kRowSlots = 6;                   // 32 KB each: K and V tiles in turn
 constexpr int kUnitCache = 256;                // sequences whose lengths are kept in shared memory
 struct RowsUnit {
     int first, n, kv_len, tiles;
+    __device__ __forceinline__ int weight() const { return tiles ? tiles + kUnitOver : 0; }
 };
 
 struct RowsSmem {
@@ -52,10 +58,11 @@ struct RowsSmem {
     float o[kRowWarps][8][72];                 // joins the warps' outputs, 8 rows x 64 dims at a time (rows 8 banks apart)
     float m[kRowWarps][kRows], l[kRowWarps][kRows], qmax[kRowWarps][kRows];
     int first[kUnitCache], n[kUnitCache], kv[kUnitCache];
-    uint64_t full[kRowSlots], empty[kRowSlots], opened;
+    uint64_t full[kRowSlots], empty[kRowSlots];
+    uint64_t opened[2];                        // the CTA's shared units: at most its first and its last
     long long sums[kRowWarps], rest[kRowWarps];
-    long long W, x0;                           // tiles in all, first tile of the CTA's run
-    int b, g, tile, left;                      // where that is
+    long long W, x0, x1, u0;                   // weight in all, the CTA's run of it, start of the run's first unit
+    int b, g;                                  // which that is
     int last;
 };
 
@@ -84,14 +91,16 @@ __device__ __forceinline__ RowsUnit get_unit(const AttnBatch& p, const RowsSmem&
     return u;
 }
 
-// A position in the flattened tiles, and how many are left of the CTA's run.
+// A unit of the CTA's run [x0, x1): it begins at u0, and its tile j lies at u0 + 1 + j.
 struct RowsWalk {
-    int b, g, tile, left;
-    __device__ __forceinline__ int end(const RowsUnit& u) const { return min(u.tiles, tile + left); }
+    int b, g;
+    long long u0, x0, x1;
+    __device__ __forceinline__ bool more() const { return u0 < x1; }
+    __device__ __forceinline__ int first(const RowsUnit& u) const { return (int)max(0ll, min((long long)u.tiles, x0 - u0 - 1)); }
+    __device__ __forceinline__ int end(const RowsUnit& u) const { return (int)max(0ll, min((long long)u.tiles, x1 - u0 - 1)); }
     __device__ __forceinline__ void next(const AttnBatch& p, const RowsSmem& S, const RowsUnit& u) {
-        left -= end(u) - tile;
-        tile = 0;
-        if (left > 0 && ++g == p.n_kv) {
+        u0 += u.weight();
+        if (u0 < x1 && ++g == p.n_kv) {
             g = 0;
             do ++b;
             while (b + 1 < p.B && get_unit(p, S, b).tiles == 0);
@@ -99,7 +108,7 @@ struct RowsWalk {
     }
 };
 
-// CTA that holds tile x of W: the last c with c * W / kRowCtas <= x.
+// CTA that holds position x of W: the last c with c * W / kRowCtas <= x.
 __device__ __forceinline__ int rows_cta(long long x, long long W) {
     const long long n = (x + 1) * kRowCtas - 1;
     return W <= 0xffffffff / kRowCtas ? (int)((uint32_t)n / (uint32_t)W) : (int)(n / W);
@@ -130,7 +139,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             mbar_init(&S.full[i], 1);
             mbar_init(&S.empty[i], kRowWarps);
         }
-        mbar_init(&S.opened, 1);
+        mbar_init(&S.opened[0], 1);
+        mbar_init(&S.opened[1], 1);
         fence_mbar_init();
     }
     // where the CTA's run of tiles begins: sums over the sequences, 256 at a time
@@ -142,13 +152,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             S.n[tid] = u.n;
             S.kv[tid] = u.kv_len;
         }
-        if (tid == 0) S.left = 0;
-        long long rest = 0;   // tiles of the sequences behind the first 256
-        for (int b = tid + kConsumers; b < p.B; b += kConsumers) rest += load_unit(p, b, blockIdx.x == 0).tiles;
+        if (tid == 0) S.u0 = S.x1 = 0;
+        long long rest = 0;   // weight of the sequences behind the first 256
+        for (int b = tid + kConsumers; b < p.B; b += kConsumers) rest += load_unit(p, b, blockIdx.x == 0).weight();
         long long before = 0, W = 0, x0 = 0, x1 = 1;
         for (int b0 = 0; b0 < p.B && x1 > x0 && before * p.n_kv <= x0; b0 += kConsumers) {
             if (b0) u = b0 + tid < p.B ? load_unit(p, b0 + tid) : RowsUnit{0, 0, 0, 0};
-            long long end = u.tiles;
+            long long end = u.weight();
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const long long o = __shfl_up_sync(0xffffffffu, end, off);
@@ -175,20 +185,20 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 x0 = W * blockIdx.x / kRowCtas;
                 x1 = W * (blockIdx.x + 1) / kRowCtas;
             }
-            const long long in = x0 - (end - u.tiles) * p.n_kv;   // tiles into this thread's sequence
-            if (x1 > x0 && in >= 0 && in < (long long)u.tiles * p.n_kv) {
+            const long long in = x0 - (end - u.weight()) * p.n_kv;   // into this thread's sequence
+            if (x1 > x0 && in >= 0 && in < (long long)u.weight() * p.n_kv) {
                 S.b = b0 + tid;
-                S.g = (int)(in / u.tiles);
-                S.tile = (int)(in - (long long)S.g * u.tiles);
-                S.left = (int)min(x1 - x0, (long long)0x7fffffff);
+                S.g = (int)(in / u.weight());
+                S.u0 = x0 - (in - (long long)S.g * u.weight());
                 S.x0 = x0;
+                S.x1 = x1;
                 S.W = W;
             }
             before += all;
         }
     }
     __syncthreads();
-    RowsWalk w{S.b, S.g, S.tile, S.left};
+    RowsWalk w{S.b, S.g, S.u0, S.x0, S.x1};
 
     if (warp >= kRowWarps) {
         // ---------------------------------- page stream: keys, and values
@@ -196,11 +206,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const CUtensorMap* tm = m ? &tv : &tk;
         const int nbox = kTile / p.box_rows, ps = 1 << p.ps_log2;
         bool ok = true;
-        int it = m;
-        while (w.left > 0 && ok) {
+        int it = m, shared = 0;
+        while (w.more() && ok) {
             const RowsUnit u = get_unit(p, S, w.b);
-            const int end = w.end(u);
-            for (int j = w.tile; j < end; ++j, it += 2) {
+            const int tile0 = w.first(u), end = w.end(u);
+            for (int j = tile0; j < end; ++j, it += 2) {
                 const int r0 = j * kTile + lane * p.box_rows, st = it % kRowSlots;
                 const bool mine = lane < nbox && r0 < u.kv_len;
                 const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
@@ -221,12 +231,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 if (mine)
                     tma_load_kv(S.ring[st] + lane * p.box_rows * kHd * 2, tm, 0, row, w.g, page, &S.full[st]);
                 __syncwarp();
-                // the counters of the units this CTA shares (at most its first and its
-                // last), once the first keys are on their way
-                if (it == 0 && lane == 0) {
-                    if (w.tile > 0 || w.left < u.tiles) part_open(part_count(p, rows_cta(S.x0 - w.tile, S.W)), p.nonce);
-                    if (w.left > u.tiles - w.tile) part_open(part_count(p, blockIdx.x), p.nonce);   // (unused if whole)
-                    mbar_arrive(&S.opened);
+                // the counter of a unit this CTA shares, once its first keys are on their way
+                if (m == 0 && j == tile0 && lane == 0 && (tile0 > 0 || end < u.tiles)) {
+                    part_open(part_count(p, rows_cta(w.u0 + 1, S.W)), p.nonce);
+                    mbar_arrive(&S.opened[shared++]);
                 }
                 __syncwarp();
             }
@@ -256,18 +264,44 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     // ldmatrix lane addresses (rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7))
     const int lr = (lane & 7) + ((lane >> 4) << 3), lc = (lane >> 3) & 1;          // K: matrices (keys 0-7, c), (keys 0-7, c + 1), (keys 8-15, ..)
     const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;          // V (transposed): (keys 0-7, c), (keys 8-15, c), (.., c + 1)
-    long long x = S.x0;                            // flattened position
+    // a unit's queries on their way: warp ks brings step ks of the A fragments, thread
+    // (gr, gc) rows gr, gr + 8, columns 16 ks + 2 gc + {0, 1} and + 8.  The next unit's
+    // are loaded while this one's keys are worked on.
+    using QRaw = std::conditional_t<F32, float2, uint32_t>;
+    QRaw qraw[2][2];
+    auto load_q = [&](const RowsUnit& u, int g) {
+        const int rows = min(u.n, p.tokens_per_tile) * p.G;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            const int r = gr + 8 * hh, tok = r / p.G, h = r - tok * p.G;
+            const int64_t off = (int64_t)(u.first + tok) * p.q_stride + (int64_t)(g * p.G + h) * kHd + 16 * warp + 2 * gc;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                qraw[hh][c] = QRaw{};
+                if (r < rows)
+                    qraw[hh][c] = __ldg(reinterpret_cast<const QRaw*>(
+                        reinterpret_cast<const char*>(p.q) + (off + 8 * c) * (F32 ? sizeof(float) : sizeof(__half))));
+            }
+        }
+    };
+    auto skip = [&](RowsWalk& v) {   // to the next unit that has tiles in the run
+        while (v.more()) {
+            const RowsUnit u = get_unit(p, S, v.b);
+            if (v.first(u) < v.end(u)) return;
+            v.next(p, S, u);
+        }
+    };
+    skip(w);
+    if (w.more()) load_q(get_unit(p, S, w.b), w.g);
     bool ok = true;
-    int it = 0;
-    while (w.left > 0) {
+    int it = 0, shared = 0;
+    while (w.more()) {
         const RowsUnit u = get_unit(p, S, w.b);
-        const int g = w.g, tile0 = w.tile, tile1 = w.end(u);
+        const int g = w.g, tile0 = w.first(u), tile1 = w.end(u);
         const int ntok = min(u.n, p.tokens_per_tile), rows = ntok * p.G;
         const int see0 = u.kv_len - u.n + 1;           // keys the first token sees (may be <= 0)
 
         // ------------------------------------------------------------ queries
-        // warp ks brings step ks of the A fragments: thread (gr, gc) holds rows
-        // gr, gr + 8, columns 16 ks + 2 gc + {0, 1} and + 8
         float f[2];                                    // score factor: scale * log2(e) * the row's power of two
         int lim[2];                                    // keys seen by the thread's two rows
         {
@@ -275,21 +309,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             float2 a[2][2];
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-                const int r = gr + 8 * hh, tok = r / p.G, h = r - tok * p.G;
-                const bool live = r < rows;
-                lim[hh] = live ? max(0, min(u.kv_len, see0 + tok)) : 0;
+                const int r = gr + 8 * hh, tok = r / p.G;
+                lim[hh] = r < rows ? max(0, min(u.kv_len, see0 + tok)) : 0;
                 f[hh] = p.scale_log2;
-                const int64_t off =
-                    (int64_t)(u.first + tok) * p.q_stride + (int64_t)(g * p.G + h) * kHd + 16 * warp + 2 * gc;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    if constexpr (F32)
-                        a[hh][c] = live ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + off + 8 * c))
-                                        : make_float2(0.f, 0.f);
-                    else
-                        hi[2 * c + hh] = live ? __ldg(reinterpret_cast<const uint32_t*>(static_cast<const __half*>(p.q) +
-                                                                                        off + 8 * c))
-                                              : 0u;
+                    if constexpr (F32) a[hh][c] = qraw[hh][c];
+                    else hi[2 * c + hh] = qraw[hh][c];
                 }
             }
             if constexpr (F32) {
@@ -317,12 +343,16 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             S.q[0][warp][lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             named_bar_sync(1, kConsumers);
         }
+        RowsWalk nw = w;
+        nw.next(p, S, u);
+        skip(nw);
+        if (nw.more()) load_q(get_unit(p, S, nw.b), nw.g);
 
         const bool whole = tile0 == 0 && tile1 == u.tiles;
         int c0 = 0, c1 = 0, parts = 0;                 // CTAs that share the unit
         if (!whole) {
-            c0 = rows_cta(x - tile0, S.W);
-            c1 = rows_cta(x - tile0 + u.tiles - 1, S.W);
+            c0 = rows_cta(w.u0 + 1, S.W);
+            c1 = rows_cta(w.u0 + u.tiles, S.W);
             for (int c = c0 + lane; c <= c1; c += 32) parts += !rows_cta_empty(c, S.W);
             parts = __reduce_add_sync(0xffffffffu, parts);
         }
@@ -517,7 +547,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         if (!whole) {
             // (the barrier above orders the CTA's stores before thread 0's release)
             if (threadIdx.x == 0) {
-                ok = ok && mbar_wait(&S.opened, 0, p.err, kDevTimeoutFull);
+                ok = ok && mbar_wait(&S.opened[shared], 0, p.err, kDevTimeoutFull);
                 const bool last = ok && atom_add_acq_rel_gpu_u64(part_count(p, c0), 1ull) + 1 == p.nonce + parts;
                 if (last) *part_count(p, c0) = 0;
                 S.last = last;
@@ -577,8 +607,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                 }
             }
         }
-        x += tile1 - tile0;
-        w.next(p, S, u);
+        shared += !whole;
+        w = nw;
     }
 }
 
