@@ -228,15 +228,25 @@ struct ItemWalk {
         const int lane = threadIdx.x & 31;
         L = 0x7fffffff;
         most = total = cut = 0;
+        long long rows = 0;
         for (int c = 0; c < p.B; c += 32) {
             const SeqUnits u = seq_units(p, c + lane);
             if (u.n > 0) {
+                rows += u.n;
                 most = max(most, (u.kv_len + kTile - 1) / kTile);
                 total += (u.n + u.per - 1) / u.per * p.n_kv;
             }
         }
         total = __reduce_add_sync(0xffffffffu, total);
         most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) rows += __shfl_xor_sync(0xffffffffu, rows, off);
+        // first rows that do not ascend may name more units than there is room for: no items
+        if (rows > p.T) {
+            if (lane == 0) atomicExch(p.err, kDevBadArg);
+            total = 0;
+            return;
+        }
         if (p.split && most > kMinPart) {
             int len[kMaxParts], n[kMaxParts];
 #pragma unroll
@@ -326,16 +336,9 @@ struct ItemWalk {
         it.part = part;
         it.parts = min(np, parts_of(all));
         it.slot = slot;
-        if (np > 1) {
-            // first rows that do not ascend may name more units than the workspace has room for
-            if (slot + np > p.slots) {
-                if ((threadIdx.x & 31) == 0) atomicExch(p.err, kDevBadArg);
-                return false;
-            }
-            if ((threadIdx.x & 31) == 0)
-                *tile_unit(p, slot + part) = TileUnit{part == 0 && it.parts > 1 ? it.parts : 0, it.g, it.row0, it.see0, it.kv_len,
-                                                      {it.ntok[0], it.ntok[1]}};
-        }
+        if (np > 1 && (threadIdx.x & 31) == 0)
+            *tile_unit(p, slot + part) = TileUnit{part == 0 && it.parts > 1 ? it.parts : 0, it.g, it.row0, it.see0, it.kv_len,
+                                                  {it.ntok[0], it.ntok[1]}};
         if (part >= it.parts) return false;
         it.j0 = (int)((long long)all * part / it.parts);
         it.ntiles = (int)((long long)all * (part + 1) / it.parts) - it.j0;

@@ -440,6 +440,26 @@ def test_paged_rows_outside_are_not_read(cuda, glc):
     assert torch.isfinite(p.out).all()
 
 
+def test_paged_first_rows_that_do_not_ascend(cuda, glc):
+    """Sequences that name the same rows over and over: recorded, and nothing
+    outside the outputs' rows is written; the workspace serves the next call."""
+    torch = cuda
+    p = Paged(torch, glc, np.random.default_rng(15), [150] * 4, [3000, 2000, 1500, 1200], 16, 2, 16, F16, pad=5)
+    guard = torch.full((64 + p.out.numel() + 64,), 7.0, dtype=p.out.dtype, device="cuda")
+    p.out = guard[64:-64].view(p.out.shape)
+    p.dc.copy_(dev(torch, np.array([0, 600, 0, 600, 0], np.int32)))
+    p.max_new = 600
+    p.ws = torch.full((glc.attn_paged_workspace_bytes(16, 2, 4, p.T, 600),), 255, dtype=torch.uint8, device="cuda")
+    p.call()
+    with pytest.raises(glc.GlcError, match="out of range"):
+        glc.paged_poll_error()
+    assert torch.all(guard[:64] == 7) and torch.all(guard[-64:] == 7) and torch.all(p.out[600:] == 7)
+    p.dc.copy_(dev(torch, p.cu))
+    p.call()
+    glc.paged_poll_error()
+    p.check()
+
+
 @pytest.mark.parametrize("new,kv", [([1, 1, 1], [100, 600, 33]), ([100, 5], [400, 700])])
 def test_paged_captured_and_replayed(cuda, glc, new, kv):
     """A captured call follows the device's lengths: replays with other ones."""
