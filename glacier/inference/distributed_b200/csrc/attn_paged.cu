@@ -68,7 +68,8 @@ AttnPlan plan_attention(int n_heads, int n_kv, int B, int T, int max_new, bool w
     // Many units fill the SMs by themselves, and each CTA looks through all sequences
     a.split = a.tiles && workspace && units <= 16 * 148;
     a.items = units + (a.split ? kTileExtra : 0);
-    a.slots = a.split ? (int)std::min<long long>(units * kTileParts, 2 * kTileExtra) : 0;
+    // (room for parts also where none are cut: a workspace serves every smaller call)
+    a.slots = a.tiles && workspace ? (int)std::min<long long>(units * kTileParts, 2 * kTileExtra) : 0;
     a.tile_work = kRowsWorkBytes + ((size_t)(a.slots + 1) * kTileUnitBytes + 255) / 256 * 256;
     a.work = a.tile_work + (size_t)a.slots * kTilePartFloats * sizeof(float);
     return a;

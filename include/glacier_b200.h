@@ -348,7 +348,8 @@ int glc_attn_prompt_dev(const void* q, int32_t q_type, int64_t q_stride, const v
  * longer than max_new is recorded (glc_paged_poll_error) and that sequence's
  * rows are unspecified; first rows that do not ascend may be recorded, and all
  * rows are unspecified then.  workspace: glc_attn_paged_workspace_bytes device
- * bytes, 16-byte aligned, any contents; calls that may overlap need their own. */
+ * bytes, 16-byte aligned, any contents; those of the largest B, T and max_new
+ * serve all smaller calls; calls that may overlap need their own. */
 int glc_attn_paged_workspace_bytes(int32_t n_heads, int32_t n_kv_heads, int32_t B, int32_t T, int32_t max_new,
                                    uint64_t* bytes);
 int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_stride, const glc_kv_pages* cache,

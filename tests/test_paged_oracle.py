@@ -166,3 +166,15 @@ def test_workspace_bytes_refuses(glc):
         with pytest.raises(glc.GlcError):
             glc.attn_paged_workspace_bytes(*bad)
     assert glc.attn_paged_workspace_bytes(40, 8, 64, 64, 1) > 0
+
+
+@pytest.mark.parametrize("heads,kv", [(40, 8), (28, 4), (16, 1), (8, 8)])
+def test_workspace_of_the_largest_call_serves_smaller_ones(glc, heads, kv):
+    sizes = [glc.attn_paged_workspace_bytes(heads, kv, B, T, T) for B, T in
+             ((1, 1), (2, 17), (2, 64), (9, 300), (9, 4096), (64, 16384), (64, 70000), (500, 1000000))]
+    assert sizes == sorted(sizes)
+    for T in (1, 40, 5000, 400000):
+        by_new = [glc.attn_paged_workspace_bytes(heads, kv, 300, T, n) for n in (0, 1, 2, 16, 17, 500)]
+        assert by_new == sorted(by_new)
+        by_batch = [glc.attn_paged_workspace_bytes(heads, kv, B, T, 500) for B in (0, 1, 4, 5, 40, 300, 5000)]
+        assert by_batch == sorted(by_batch)
