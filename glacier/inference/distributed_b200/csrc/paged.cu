@@ -545,7 +545,8 @@ extern "C" int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens,
     if (!ctx_lens || !new_lens || !block_table || !free_list || !free_count || !free_count_out || !cu_new || !kv_lens ||
         !status || (T > 0 && (!positions || !slots)))
         return paged_fail(GLC_ERR_INVALID_ARG, "null pointer");
-    if (B < 0 || T < 0 || max_pages <= 0 || capacity < 0)
+    if (B < 0 || T < 0 || max_pages <= 0 || capacity < 0 || (int64_t)max_pages * std::max(page_size, 1) > 0x7fffffff ||
+        capacity == 0x7fffffff)
         return paged_fail(GLC_ERR_INVALID_ARG, "page plan of %d requests, %d rows, %d pages a table row, %d pages", B, T,
                           max_pages, capacity);
     if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)

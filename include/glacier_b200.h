@@ -301,8 +301,9 @@ typedef struct glc_kv_pages {
  * requests (attention gives those zero rows); positions and slots [T] of
  * every new row (slot = page * page_size + row; slot -1, position 0 for the
  * rows of unserved requests and behind the last one); status = requests not
- * served.  kv_lens and free_count_out must not alias the inputs.  The same
- * inputs give the same outputs again, so a step can be planned twice. */
+ * served.  kv_lens and free_count_out must not alias the inputs, and
+ * max_pages * page_size must fit 31 bits.  The same inputs give the same outputs
+ * again, so a step can be planned twice. */
 int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens, int32_t B, int32_t page_size,
                     int32_t* block_table, int32_t max_pages, int32_t* free_list, int32_t capacity,
                     const int32_t* free_count, int32_t* free_count_out, int32_t T, int32_t* cu_new,
@@ -316,7 +317,7 @@ int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens, int32_t B,
  * q_out [T][n_heads][128] in q_out_type (GLC_GGUF_F32 or GLC_GGUF_F16; may be
  * q itself for dense fp32 rows; n_heads 0: keys and values only).  cache NULL:
  * nothing is stored; slots < 0 are skipped, slots past the cache are skipped
- * and recorded (glc_paged_poll_error).  k_out / v_out: the same fp16 rows
+ * and recorded (glc_paged_poll_error); two rows must not name one slot.  k_out / v_out: the same fp16 rows
  * packed [T][n_kv_heads][128], or NULL. */
 int glc_rope_append_dev(const float* q, int64_t q_stride, const float* k, const float* v, int64_t kv_stride,
                         int32_t T, int32_t n_heads, int32_t n_kv_heads, const int32_t* positions,
@@ -360,7 +361,9 @@ int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_stride, const gl
 /* Reads and clears the device error word of the paged entry points on the
  * current device (synchronises the device): GLC_ERR_INVALID_ARG when a page
  * id, slot or length on the device was out of range, GLC_ERR_TIMEOUT when a
- * bounded device-side wait gave up, else GLC_OK. */
+ * bounded device-side wait gave up (the outputs are unspecified then, and a
+ * workspace that captured calls use has to be cleared), else GLC_OK.  The first
+ * paged call on a device looks the word up: make one before any stream capture. */
 int glc_paged_poll_error(void);
 
 /* ---- router alone (for tests and for callers that route elsewhere) ---- */

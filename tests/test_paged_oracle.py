@@ -168,6 +168,14 @@ def test_workspace_bytes_refuses(glc):
     assert glc.attn_paged_workspace_bytes(40, 8, 64, 64, 1) > 0
 
 
+@pytest.mark.parametrize("kw", [dict(max_pages=1 << 27, page_size=16), dict(max_pages=1 << 23, page_size=256),
+                                dict(capacity=2**31 - 1)])
+def test_plan_refuses_positions_past_32_bits(glc, kw):
+    with pytest.raises(glc.GlcError, match="page plan") as e:
+        glc.kv_plan_dev(**plan_args(**kw))
+    assert e.value.status == -1
+
+
 @pytest.mark.parametrize("heads,kv", [(40, 8), (28, 4), (16, 1), (8, 8)])
 def test_workspace_of_the_largest_call_serves_smaller_ones(glc, heads, kv):
     sizes = [glc.attn_paged_workspace_bytes(heads, kv, B, T, T) for B, T in
