@@ -499,6 +499,83 @@ def test_two_calls_at_once(cuda, glc):
         p.check()
 
 
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("B,Hq,Hkv,ps", [(7, 28, 4, 32), (50, 8, 8, 16), (300, 6, 2, 16), (560, 16, 1, 64)])
+def test_paged_mixed_batches(cuda, glc, B, Hq, Hkv, ps, qt):
+    """Chunks next to decode tokens, idle sequences and sequences without keys:
+    both kernels in one call, also with more sequences than a CTA keeps lengths of."""
+    rng = np.random.default_rng(B)
+    new, kv = [], []
+    for b in range(B):
+        n = (1, 1, 2, 0, 1, 1)[b % 6] if b % 23 else int(rng.integers(17, 60))
+        new.append(n)
+        kv.append(0 if b % 29 == 5 else n + int(rng.integers(0, 700 if b % 50 else 2600)))
+    p = Paged(cuda, glc, rng, new, kv, Hq, Hkv, ps, qt, pad=3)
+    p.call()
+    glc.paged_poll_error()
+    skip = [b for b in range(B) if B > 60 and b % 7 and b % 23 and b % 29 != 5]   # the oracle is slow
+    p.check(skip=skip)
+    first = p.out.clone()
+    p.call()
+    glc.paged_poll_error()
+    assert cuda.equal(first, p.out)
+
+
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_paged_all_without_keys(cuda, glc, new, qt):
+    p = Paged(cuda, glc, np.random.default_rng(16), [new] * 3, [0] * 3, 8, 2, 16, qt, pad=2)
+    p.call()
+    glc.paged_poll_error()
+    assert cuda.all(p.out[:3 * new] == 0) and cuda.all(p.out[3 * new:] == 7)
+
+
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_prompt_of_single_rows(cuda, glc, qt):
+    """Few rows in all: sequences of one or two tokens among empty ones."""
+    rng = np.random.default_rng(17)
+    lens = [0, 1, 0, 2, 1, 0, 0, 3] + [0] * 300 + [1]
+    T, cu = sum(lens), np.concatenate([[0], np.cumsum(lens)])
+    q = rng.standard_normal((T, 4, 128)).astype(NP[qt])
+    k, v = (rng.standard_normal((T, 2, 128)).astype(np.float16) for _ in range(2))
+    got = run_prompt(cuda, glc, q, k, v, cu, qt).reshape(T, 4, 128)
+    for b in range(len(lens)):
+        s = slice(cu[b], cu[b + 1])
+        if lens[b]:
+            check_attention(got[s], q[s], k[s], v[s], 0, qt == F32)
+
+
+@pytest.mark.parametrize("new,kv", [([1, 1, 2], [5000, 40, 3100]), ([70, 90], [3500, 1800])])
+def test_graphs_that_share_a_workspace(cuda, glc, new, kv):
+    """Two captured calls on one workspace, replayed in turn with keys split over
+    CTAs and lengths that change between replays."""
+    torch = cuda
+    rng = np.random.default_rng(18)
+    ps = [Paged(torch, glc, rng, new, kv, 12, 2, 16, F16), Paged(torch, glc, rng, new[::-1], kv[::-1], 12, 2, 16, F32)]
+    ps[1].ws = ps[0].ws
+    graphs = []
+    for p in ps:
+        p.call()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            p.call(stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    full = [(p.k, p.v, p.kv) for p in ps]
+    for cut in (0, 129, 1300):
+        for p, (k, v, kv0) in zip(ps, full):
+            p.kv = [max(a - cut, n) for a, n in zip(kv0, p.new)]
+            p.k, p.v = [a[:n] for a, n in zip(k, p.kv)], [a[:n] for a, n in zip(v, p.kv)]
+            p.dkv.copy_(dev(torch, np.array(p.kv, np.int32)))
+            p.out.fill_(7.0)
+        for _ in range(3):
+            for g in graphs:
+                g.replay()
+        glc.paged_poll_error()
+        for p in ps:
+            p.check()
+
+
 def test_host_memory_is_refused(cuda, glc):
     torch = cuda
     a = np.zeros(1 << 16, np.uint8)
