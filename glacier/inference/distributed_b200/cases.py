@@ -36,6 +36,15 @@ CASES = {
     "dispatch": ("dispatch_plan_kernel x1", "histogram / scan / stable permute of P=8192 slot ids over E=64"),
     "attention": ("attn_decode_kernel x1 (a 16- or 8-CTA cluster per KV head)",
                   "40 query / 8 KV heads x 128, position 2047 of a 2048-row fp16 cache, 16 rotating layer caches"),
+    "kv_plan": ("kv_plan_flat_kernel x1", "page plan of 2048 requests over 16-row pages, a tenth of them chunks of prompts"),
+    "rope_append": ("rope_append_kernel x1",
+                    "RoPE and store of 8192 rows, 48 query / 8 KV heads x 128, fp16 queries out, 16-row pages"),
+    "attn_prompt": ("attn_tiles_kernel x1", "one prompt of 8192 tokens, 48 query / 8 KV heads x 128, fp16 queries"),
+    "attn_prompt_f32": ("attn_tiles_kernel x1", "one prompt of 4096 tokens, 40 query / 8 KV heads x 128, fp32 queries"),
+    "attn_chunk": ("attn_tiles_kernel x1 + attn_tiles_join_kernel x1",
+                   "512 new tokens of a 16384-row sequence, 40 query / 8 KV heads x 128, fp32 queries, 64-row pages"),
+    "attn_paged": ("attn_rows_kernel x1",
+                   "decode tokens of 64 sequences of 128 to 8192 rows, 48 query / 8 KV heads x 128, fp16 queries, 16-row pages"),
     "decode_fused": ("moe_decode_fused_kernel x1", "Mixtral-8x7B layer decode, T=1 (one launch)"),
     "decode_wide": ("moe_decode_wide_kernel x1", "Qwen2-57B-A14B layer decode with its shared expert, T=1 (one launch)"),
     "stage": ("per layer: attn_decode_kernel x1, q4k_gemv_chain_kernel x1",
@@ -157,6 +166,93 @@ def case_attention(torch, glc, reps):
     torch.cuda.synchronize()
 
 
+def case_kv_plan(torch, glc, reps):
+    B, ps, width, rng = 2048, 16, 544, np.random.default_rng(11)
+    ctx = rng.integers(0, 8193, B)
+    new = np.where(rng.random(B) < 0.1, rng.integers(1, 513, B), 1)
+    held, T = -(-ctx // ps), int(new.sum())
+    ids = rng.permutation(int(held.sum()) + T).astype(np.int32)
+    table = np.zeros((B, width), np.int32)
+    at = np.concatenate([[0], np.cumsum(held)])
+    for b in range(B):
+        table[b, :held[b]] = ids[at[b]:at[b + 1]]
+    pool = ids[at[-1]:]
+    d = [torch.from_numpy(a.astype(np.int32)).cuda() for a in (ctx, new, table, pool, np.array([len(pool)]))]
+    o = [torch.empty(n, dtype=torch.int32, device="cuda") for n in (1, B + 1, B, T, 1)]
+    slots = torch.empty(T, dtype=torch.int64, device="cuda")
+    st, s = _stream(torch)
+    with torch.cuda.stream(st):
+        for _ in range(3 + reps):
+            glc.kv_plan_dev(d[0].data_ptr(), d[1].data_ptr(), B, ps, d[2].data_ptr(), width, d[3].data_ptr(), len(pool),
+                            d[4].data_ptr(), o[0].data_ptr(), T, o[1].data_ptr(), o[2].data_ptr(), o[3].data_ptr(),
+                            slots.data_ptr(), o[4].data_ptr(), stream=s)
+    torch.cuda.synchronize()
+
+
+def _pages(torch, glc, lens, Hkv, ps):
+    """A cache of random rows in shuffled pages, and the sequences' page table."""
+    held = [-(-n // ps) for n in lens]
+    n_pages, width = sum(held), max(held)
+    kv = [torch.randn(n_pages, Hkv, ps, 128, device="cuda", dtype=torch.float16) for _ in range(2)]
+    ids = np.random.default_rng(12).permutation(n_pages).astype(np.int32)
+    table, at = np.zeros((len(lens), width), np.int32), 0
+    for b, n in enumerate(held):
+        table[b, :n] = ids[at:at + n]
+        at += n
+    return kv, glc.KvPages(kv[0].data_ptr(), kv[1].data_ptr(), n_pages, ps, Hkv), torch.from_numpy(table).cuda()
+
+
+def case_rope_append(torch, glc, reps):
+    T, Hq, Hkv, row = 8192, 48, 8, 64 * 128
+    x = torch.randn(T, row, device="cuda")                  # fused q, k, v rows: 268 MB
+    keep, cache, _ = _pages(torch, glc, [T], Hkv, 16)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    slots = torch.randperm(T, device="cuda")
+    q = torch.empty(T, Hq * 128, device="cuda", dtype=torch.float16)
+    p = x.data_ptr()
+    st, s = _stream(torch)
+    with torch.cuda.stream(st):
+        for _ in range(3 + reps):
+            glc.rope_append_dev(p, row, p + Hq * 512, p + (Hq + Hkv) * 512, row, T, Hq, Hkv, pos.data_ptr(),
+                                slots.data_ptr(), 1e6, cache, q.data_ptr(), glc.GGUF_F16, stream=s)
+    torch.cuda.synchronize()
+    glc.paged_poll_error()
+
+
+def case_attn_prompt(torch, glc, T, Hq, f32, reps):
+    Hkv = 8
+    q = torch.randn(T, Hq * 128, device="cuda", dtype=torch.float32 if f32 else torch.float16)
+    k, v = (torch.randn(T, Hkv * 128, device="cuda", dtype=torch.float16) for _ in range(2))
+    out = torch.empty_like(q)
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    st, s = _stream(torch)
+    with torch.cuda.stream(st):
+        for _ in range(3 + reps):
+            glc.attn_prompt_dev(q.data_ptr(), glc.GGUF_F32 if f32 else glc.GGUF_F16, Hq * 128, k.data_ptr(), v.data_ptr(),
+                                Hkv * 128, cu.data_ptr(), 1, T, Hq, Hkv, out.data_ptr(), Hq * 128, stream=s)
+    torch.cuda.synchronize()
+    glc.paged_poll_error()
+
+
+def case_attn_paged(torch, glc, new, lens, Hq, ps, f32, reps):
+    Hkv, B, T = 8, len(lens), sum(new)
+    keep, cache, table = _pages(torch, glc, lens, Hkv, ps)
+    q = torch.randn(T, Hq * 128, device="cuda", dtype=torch.float32 if f32 else torch.float16)
+    out = torch.empty_like(q)
+    cu = torch.from_numpy(np.concatenate([[0], np.cumsum(new)]).astype(np.int32)).cuda()
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    wb = glc.attn_paged_workspace_bytes(Hq, Hkv, B, T, max(new))
+    work = torch.empty(wb, dtype=torch.uint8, device="cuda")
+    st, s = _stream(torch)
+    with torch.cuda.stream(st):
+        for _ in range(3 + reps):
+            glc.attn_paged_dev(q.data_ptr(), glc.GGUF_F32 if f32 else glc.GGUF_F16, Hq * 128, cache, table.data_ptr(),
+                               table.shape[1], cu.data_ptr(), kv.data_ptr(), B, T, max(new), Hq, out.data_ptr(), Hq * 128,
+                               work.data_ptr(), wb, stream=s)
+    torch.cuda.synchronize()
+    glc.paged_poll_error()
+
+
 def case_decode(torch, glc, wide, reps):
     w = QWEN if wide else MIXTRAL
     worker = glc.GpuExpertStageWorker(w["D"], w["F"], w["E"], w["k"], shared_ffn_dim=w.get("Fs", 0),
@@ -233,6 +329,18 @@ def main(argv=None) -> int:
         case_dispatch(torch, glc, n)
     elif c == "attention":
         case_attention(torch, glc, n)
+    elif c == "kv_plan":
+        case_kv_plan(torch, glc, n)
+    elif c == "rope_append":
+        case_rope_append(torch, glc, n)
+    elif c == "attn_prompt":
+        case_attn_prompt(torch, glc, 8192, 48, False, n)
+    elif c == "attn_prompt_f32":
+        case_attn_prompt(torch, glc, 4096, 40, True, n)
+    elif c == "attn_chunk":
+        case_attn_paged(torch, glc, [512], [16384], 40, 64, True, n)
+    elif c == "attn_paged":
+        case_attn_paged(torch, glc, [1] * 64, [128 * (1 + 13 * i % 64) for i in range(64)], 48, 16, False, n)
     elif c in ("decode_fused", "decode_wide"):
         case_decode(torch, glc, c == "decode_wide", n)
     elif c == "stage":
