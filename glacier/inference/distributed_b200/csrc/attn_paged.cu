@@ -88,6 +88,11 @@ int attn_launch(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap&
     }
     if (!a.tiles) return GLC_OK;
     p.tokens_per_tile = kTileTokens(p.G);
+    // ceil(2^(31 + l) / d) with 2^(l - 1) < d <= 2^l: exact below 2^31 (d is 16 at least)
+    int l = 1;
+    while ((1 << l) < p.tokens_per_tile) ++l;
+    p.unit_mul = (unsigned)(((1ull << (31 + l)) + p.tokens_per_tile - 1) / p.tokens_per_tile);
+    p.unit_shift = l - 1;
     CUtensorMap tq = ttk;   // fp32 queries are not read through a descriptor
     if (!f32)
         if (int rc = query_map(&tq, p)) return rc;

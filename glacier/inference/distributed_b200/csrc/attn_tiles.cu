@@ -163,23 +163,33 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // Units of sequence b whose key tiles number up to x: the tiles a unit sees grow along
 // the sequence.
 struct SeqUnits {
-    int n, kv_len, per;           // new tokens, keys, tokens of a unit
-    __device__ __forceinline__ int upto(int x) const {
-        const int all = (n + per - 1) / per;
+    int n, kv_len, first;         // new tokens, keys, first row
+    __device__ __forceinline__ int upto(const AttnBatch& p, int x) const {
         if (x < 0) return 0;
-        if (kv_len <= x * (long long)kTile) return all;
-        const long long t = (long long)x * kTile - (kv_len - n);   // tokens whose keys fit x tiles
-        return t <= 0 ? 0 : (int)min((long long)all - 1, t / per);
+        if ((unsigned)kv_len <= (unsigned)x * kTile) return all(p);
+        const int t = (int)((unsigned)x * kTile) - kv_len + n;   // tokens whose keys fit x tiles
+        return t <= 0 ? 0 : min(all(p) - 1, div_unit(p, t));
+    }
+    __device__ __forceinline__ int all(const AttnBatch& p) const { return div_unit(p, n + p.tokens_per_tile - 1); }
+    __device__ __forceinline__ int tiles() const { return (int)(((unsigned)kv_len + kTile - 1) / kTile); }
+    // x / tokens_per_tile, 0 <= x < 2^31 (a division takes 200 cycles, and a CTA's first
+    // items wait for dozens of them)
+    static __device__ __forceinline__ int div_unit(const AttnBatch& p, int x) {
+        return (int)(__umulhi((unsigned)x, p.unit_mul) >> p.unit_shift);
     }
 };
-__device__ __forceinline__ SeqUnits seq_units(const AttnBatch& p, int b) {
-    SeqUnits u{0, 0, p.tokens_per_tile};
-    if (b < 0 || b >= p.B) return u;
-    int first;
-    seq_rows(p, b, first, u.n);
+__device__ __forceinline__ SeqUnits seq_units(const AttnBatch& p, int b, bool record = false) {
+    SeqUnits u{0, 0, 0};
+    if (b < 0) return u;
+    seq_rows(p, b, u.first, u.n);
     if (u.n * p.G <= p.rows_take) u.n = 0;   // none, or the row kernel's
-    const long long room = (long long)p.max_pages << p.ps_log2;
-    u.kv_len = p.kv_lens ? (int)min((long long)max(p.kv_lens[b], 0), room) : u.n;
+    u.kv_len = u.n;
+    if (p.kv_lens) {
+        const long long room = (long long)p.max_pages << p.ps_log2;
+        const int len = p.kv_lens[b];
+        u.kv_len = (int)min((long long)max(len, 0), room);
+        if (record && u.n > 0 && (len != u.kv_len || u.n > p.max_new)) atomicExch(p.err, kDevBadArg);
+    }
     return u;
 }
 
@@ -193,21 +203,40 @@ __device__ __forceinline__ SeqUnits seq_units(const AttnBatch& p, int b) {
 // an item's cost, in key tiles: its own, two for its prologue and epilogue, and a
 // third of one for each part that the join reads.
 constexpr int kBuckets = 16;
+static_assert(kMaxParts == 8, "a lane for each number of parts");
+constexpr int kSeqCache = 4;       // chunks of 32 sequences, from the last down, kept in registers
 struct ItemWalk {
+    int seq_first[kSeqCache], seq_n[kSeqCache], seq_kv[kSeqCache];   // of the lane's sequences
+    int first, n, kv_len;         // of the lane's sequence in the chunk at hand
     int L, most, total, cut;      // tiles of a part, of the longest unit; items in all, and those of cut units
     int bucket, b0, before, slots;   // class; chunk of 32 sequences (the one of lane 0); items and places before it
     int low, units, parts, count, split, end, send, chunk, schunk;   // of the lane's sequence; sums of the chunk
 
-    __device__ __forceinline__ int parts_of(int tiles) const { return max(1, (tiles - 1) / L + 1); }
+    __device__ __forceinline__ int parts_of(int tiles) const { return tiles <= L ? 1 : (int)((unsigned)(tiles - 1) / (unsigned)L) + 1; }
 
+    __device__ __forceinline__ SeqUnits seq(const AttnBatch& p, int chunk) const {
+        if (p.B > 32 * kSeqCache) return seq_units(p, p.B - 1 - 32 * chunk - (int)(threadIdx.x & 31));
+        SeqUnits u{0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < kSeqCache; ++k)
+            if (k == chunk) {
+                u.n = seq_n[k];
+                u.kv_len = seq_kv[k];
+                u.first = seq_first[k];
+            }
+        return u;
+    }
     __device__ __forceinline__ void load(const AttnBatch& p) {
         const int lane = threadIdx.x & 31;
-        const SeqUnits u = seq_units(p, b0 - lane);
+        const SeqUnits u = seq(p, (p.B - 1 - b0) >> 5);
+        first = u.first;
+        n = u.n;
+        kv_len = u.kv_len;
         // classes (lo, hi] of key tiles; the last one takes units without keys too
-        const int hi = (int)((long long)most * (bucket + 1) / kBuckets), lo = bucket ? (int)((long long)most * bucket / kBuckets) : -1;
-        low = u.upto(lo);
-        units = u.n > 0 ? u.upto(hi) - low : 0;
-        parts = parts_of((u.kv_len + kTile - 1) / kTile);
+        const int hi = most * (bucket + 1) / kBuckets, lo = bucket ? most * bucket / kBuckets : -1;   // (most < 2^24)
+        low = u.upto(p, lo);
+        units = u.n > 0 ? u.upto(p, hi) - low : 0;
+        parts = parts_of(u.tiles());
         count = units * p.n_kv * parts;
         split = parts > 1 ? count : 0;
         end = count;
@@ -229,12 +258,21 @@ struct ItemWalk {
         L = 0x7fffffff;
         most = total = cut = 0;
         long long rows = 0;
-        for (int c = 0; c < p.B; c += 32) {
-            const SeqUnits u = seq_units(p, c + lane);
+        const int chunks = (p.B + 31) >> 5;
+#pragma unroll
+        for (int k = 0; k < kSeqCache; ++k) {
+            const SeqUnits u = seq_units(p, p.B - 1 - 32 * k - lane, blockIdx.x == 0);
+            seq_first[k] = u.first;
+            seq_n[k] = u.n;
+            seq_kv[k] = u.kv_len;
+        }
+        for (int c = 0; c < chunks; ++c) {
+            const SeqUnits u = seq(p, c);
+            if (c >= kSeqCache && blockIdx.x == 0) seq_units(p, p.B - 1 - 32 * c - lane, true);
             if (u.n > 0) {
                 rows += u.n;
-                most = max(most, (u.kv_len + kTile - 1) / kTile);
-                total += (u.n + u.per - 1) / u.per * p.n_kv;
+                most = max(most, u.tiles());
+                total += u.all(p) * p.n_kv;
             }
         }
         total = __reduce_add_sync(0xffffffffu, total);
@@ -248,40 +286,40 @@ struct ItemWalk {
             return;
         }
         if (p.split && most > kMinPart) {
-            int len[kMaxParts], n[kMaxParts];
-#pragma unroll
-            for (int i = 0; i < kMaxParts; ++i) {
-                len[i] = max(kMinPart, (most + i) / (i + 1));
-                n[i] = 0;
-            }
-            for (int c = 0; c < p.B; c += 32) {
-                const SeqUnits u = seq_units(p, c + lane);
-                const int units = (u.n + u.per - 1) / u.per * p.n_kv, tiles = (u.kv_len + kTile - 1) / kTile;
-#pragma unroll
-                for (int i = 0; i < kMaxParts; ++i) n[i] += units * max(1, (tiles + len[i] - 1) / len[i]);
-            }
-            int c[kMaxParts] = {};        // items of the units that are cut
-            for (int b = 0; b < p.B; b += 32) {
-                const SeqUnits u = seq_units(p, b + lane);
-                const int units = (u.n + u.per - 1) / u.per * p.n_kv, tiles = (u.kv_len + kTile - 1) / kTile;
-#pragma unroll
-                for (int i = 0; i < kMaxParts; ++i)
-                    if (tiles > len[i]) c[i] += units * ((tiles + len[i] - 1) / len[i]);
-            }
-            float best = 3.4e38f;
-            const int ctas = gridDim.x, whole = total;
-#pragma unroll
-            for (int i = 0; i < kMaxParts; ++i) {
-                n[i] = __reduce_add_sync(0xffffffffu, n[i]);
-                c[i] = __reduce_add_sync(0xffffffffu, c[i]);
-                const float cost = (float)((n[i] + ctas - 1) / ctas) * ((float)len[i] + 2.f) + 0.33f * i;
-                if (cost < best && n[i] - whole <= kMaxExtra) {
-                    best = cost;
-                    L = len[i];
-                    total = n[i];
-                    cut = c[i];
+            // lane: choice lane & 7, of the sequences 4 k + lane / 8 (eight choices in a row are
+            // long code that runs once, from a cold instruction cache: 6,000 cycles)
+            const int i = lane % kMaxParts, len = max(kMinPart, (most + i) / (i + 1));
+            int items = 0, of_cut = 0;
+            L = len;
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                const SeqUnits u = seq(p, c);
+                const int units = u.all(p) * p.n_kv, tiles = u.tiles();
+                const unsigned some = __ballot_sync(0xffffffffu, units > 0);
+#pragma unroll 1
+                for (int k = 0; k < 32; k += 4) {
+                    if ((some >> k & 15u) == 0) continue;
+                    const int parts = parts_of(__shfl_sync(0xffffffffu, tiles, k + lane / kMaxParts));
+                    const int count = __shfl_sync(0xffffffffu, units, k + lane / kMaxParts) * parts;
+                    items += count;
+                    if (parts > 1) of_cut += count;
                 }
             }
+#pragma unroll
+            for (int off = 16; off >= kMaxParts; off >>= 1) {
+                items += __shfl_xor_sync(0xffffffffu, items, off);
+                of_cut += __shfl_xor_sync(0xffffffffu, of_cut, off);
+            }
+            const int ctas = gridDim.x;
+            float cost = (float)((items + ctas - 1) / ctas) * ((float)len + 2.f) + 0.33f * i;
+            if (items - total > kMaxExtra) cost = INFINITY;   // (never the first: no parts)
+            float best = cost;
+#pragma unroll
+            for (int off = kMaxParts / 2; off >= 1; off >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, off));
+            const int pick = __ffs(__ballot_sync(0xffffffffu, cost == best)) - 1;
+            L = __shfl_sync(0xffffffffu, len, pick);
+            total = __shfl_sync(0xffffffffu, items, pick);
+            cut = __shfl_sync(0xffffffffu, of_cut, pick);
         }
         bucket = kBuckets - 1;
         b0 = p.B - 1;
@@ -304,22 +342,16 @@ struct ItemWalk {
         const int l = __ffs(__ballot_sync(0xffffffffu, before + end > x)) - 1;
         const int np = __shfl_sync(0xffffffffu, parts, l), nu = __shfl_sync(0xffffffffu, units, l);
         const int in = x - before - __shfl_sync(0xffffffffu, end - count, l);
-        const int u = in / np, part = in - u * np;            // unit of the class's, from its end
+        const int u = np == 1 ? in : (int)((unsigned)in / (unsigned)np), part = in - u * np;   // unit of the class's, from its end
+        const int ul = (int)((unsigned)u / (unsigned)p.n_kv);
         const int slot = slots + __shfl_sync(0xffffffffu, send - split, l) + u * np;
         const int tpt = p.tokens_per_tile >> 1;
         it.seq = b0 - l;
-        it.g = u % p.n_kv;
-        const int tok0 = (__shfl_sync(0xffffffffu, low, l) + nu - 1 - u / p.n_kv) * p.tokens_per_tile;
-        int first, n;
-        seq_rows(p, it.seq, first, n);
-        it.kv_len = n;
+        it.g = u - ul * p.n_kv;
+        const int tok0 = (__shfl_sync(0xffffffffu, low, l) + nu - 1 - ul) * p.tokens_per_tile;
+        const int first = __shfl_sync(0xffffffffu, this->first, l), n = __shfl_sync(0xffffffffu, this->n, l);
+        it.kv_len = __shfl_sync(0xffffffffu, kv_len, l);
         it.kv_row0 = p.kv_lens ? 0 : first;
-        if (p.kv_lens) {
-            const long long room = (long long)p.max_pages << p.ps_log2;
-            const int len = p.kv_lens[it.seq];
-            it.kv_len = (int)min((long long)max(len, 0), room);
-            if ((len != it.kv_len || n > p.max_new) && (threadIdx.x & 31) == 0) atomicExch(p.err, kDevBadArg);
-        }
         it.row0 = first + tok0;
         it.see0 = it.kv_len - n + tok0 + 1;
         it.kv_end = 0;
@@ -340,8 +372,12 @@ struct ItemWalk {
             *tile_unit(p, slot + part) = TileUnit{part == 0 && it.parts > 1 ? it.parts : 0, it.g, it.row0, it.see0, it.kv_len,
                                                   {it.ntok[0], it.ntok[1]}};
         if (part >= it.parts) return false;
-        it.j0 = (int)((long long)all * part / it.parts);
-        it.ntiles = (int)((long long)all * (part + 1) / it.parts) - it.j0;
+        it.j0 = 0;
+        it.ntiles = all;
+        if (it.parts > 1) {   // (fewer than 2^24 tiles, eight parts)
+            it.j0 = (int)((unsigned)(all * part) / (unsigned)it.parts);
+            it.ntiles = (int)((unsigned)(all * (part + 1)) / (unsigned)it.parts) - it.j0;
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) it.nt[t] = max(0, min(nt[t], it.j0 + it.ntiles) - it.j0);
         return true;
@@ -380,6 +416,37 @@ __device__ __forceinline__ void store_f32(uint4* d, uint64_t a, uint64_t b, uint
             "l"(d),
         "l"(a), "l"(b), "l"(c)
         : "memory");
+}
+__device__ __forceinline__ uint4 mul_pairs(uint64_t a, uint64_t b, uint64_t c) {
+    uint4 u;
+    asm("{\n\t.reg .b64 t;\n\tmul.rn.f32x2 t, %4, %6;\n\tmov.b64 {%0, %1}, t;\n\tmul.rn.f32x2 t, %5, %6;\n\t"
+        "mov.b64 {%2, %3}, t;\n\t}"
+        : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+        : "l"(a), "l"(b), "l"(c));
+    return u;
+}
+// Four lanes' 16-byte pieces of their rows, turned: u[i] becomes piece `lane & 3` of
+// row i of the four, so that a store of the four covers 64 bytes of a row.  Stores of
+// one row a lane touch 32 lines each, and 256 rows of 256 bytes take 4,000 cycles.
+__device__ __forceinline__ uint4 shfl_xor4(const uint4& a, int x) {
+    return make_uint4(__shfl_xor_sync(0xffffffffu, a.x, x), __shfl_xor_sync(0xffffffffu, a.y, x),
+                      __shfl_xor_sync(0xffffffffu, a.z, x), __shfl_xor_sync(0xffffffffu, a.w, x));
+}
+__device__ __forceinline__ uint4 pick4(bool c, const uint4& a, const uint4& b) {
+    return make_uint4(c ? a.x : b.x, c ? a.y : b.y, c ? a.z : b.z, c ? a.w : b.w);
+}
+__device__ __forceinline__ void turn_pieces(uint4 (&u)[4]) {
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+        const bool up = threadIdx.x & x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (!(i & x)) {
+                const uint4 r = shfl_xor4(pick4(up, u[i], u[i + x]), x);
+                u[i] = pick4(up, r, u[i]);
+                u[i + x] = pick4(up, u[i + x], r);
+            }
+    }
 }
 // 2^((a, b) * f - mu)
 __device__ __forceinline__ void exp_pair(uint32_t a, uint32_t b, uint64_t f, uint64_t mu, float& x, float& y) {
@@ -748,6 +815,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         fence_mbar_init();
     }
+    if (warp == 8 && lane == 0) {
+        if (!F32) asm volatile("prefetch.tensormap [%0];" ::"l"(&tq) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
+    }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem)),
                      "r"(kTcCols)
@@ -996,6 +1068,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             auto out_off = [&] {
                 return ((int64_t)it.row0 + t * tpt + tok) * p.out_stride + (int64_t)(it.g * p.G + row - tok * p.G) * kHd;
             };
+            // rows of the thread's group of four lanes
+            auto four_rows = [&](int64_t (&off)[4], bool (&on)[4]) {
+                const int64_t mine = out_off();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    off[e] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + e);
+                    on[e] = wrow + (lane & ~3) + e < rows;
+                }
+            };
             auto part_out = [&] { return p.tile_work + (size_t)(it.slot + it.part) * kTilePartFloats; };
             float m = -INFINITY, l = 0.f;
             const int both = min(it.nt[0], it.nt[1]);
@@ -1038,25 +1119,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (lane == 0)
                         asm volatile("red.release.cta.shared::cta.add.s32 [%0], 1;" ::"r"(smem_u32(&S.reads[t])) : "memory");
                 }
-                if (ok && live) {
-                    if (it.parts > 1) {   // unnormalised, to the workspace
+                if (ok && it.parts > 1) {   // unnormalised, to the workspace
+                    if (live) {
                         float* x = part_out();
                         *reinterpret_cast<float2*>(x + 2 * kTcRows * kHd + 2 * (kTcRows * t + row)) = make_float2(m, l);
                         const uint64_t one = pair(1.f, 1.f);
 #pragma unroll
                         for (int e = 0; e < kHd / 2; e += 2)
                             store_f32(reinterpret_cast<uint4*>(part_at(x, t, e / 2, row)), o[e], o[e + 1], one);
-                    } else {
-                        uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + out_off());
-                        if (lim > 0) {
-                            const float rl = rcp(l);
-                            const uint64_t inv = pair(rl, rl);
+                    }
+                } else if (ok && rows > wrow) {
+                    int64_t off[4];
+                    bool on[4];
+                    four_rows(off, on);
+                    const bool some = lim > 0;   // no key seen: zeros
+                    const float rl = rcp(l);
+                    const uint64_t inv = pair(rl, rl);
 #pragma unroll
-                            for (int e = 0; e < kHd / 2; e += 2) store_f32(d + e / 2, o[e], o[e + 1], inv);
-                        } else {   // no key seen
+                    for (int e = 0; e < kHd / 2; e += 8) {
+                        uint4 u[4];
 #pragma unroll
-                            for (int e = 0; e < kHd / 4; ++e) d[e] = make_uint4(0u, 0u, 0u, 0u);
-                        }
+                        for (int k = 0; k < 4; ++k)
+                            u[k] = pick4(some, mul_pairs(o[e + 2 * k], o[e + 2 * k + 1], inv), make_uint4(0u, 0u, 0u, 0u));
+                        turn_pieces(u);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (on[k])
+                                *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + off[k] + 2 * e + 4 * (lane & 3)) = u[k];
                     }
                 }
             } else {
@@ -1084,7 +1173,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (it.parts > 1 && live)
                         *reinterpret_cast<float2*>(part_out() + 2 * kTcRows * kHd + 2 * (kTcRows * t + row)) = make_float2(m, l);
                     const float rl = rcp(l);
-                    uint4* d = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + out_off());
+                    int64_t off[4];
+                    bool on[4];
+                    four_rows(off, on);
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t r[32];
@@ -1100,18 +1191,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             __syncwarp();
                             continue;
                         }
+                        uint4 u[4];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                        for (int k = 0; k < 4; ++k) {
+                            u[k] = make_uint4(0u, 0u, 0u, 0u);
                             if (lim > 0) {
-                                u.x = pack2(__uint_as_float(r[e]) * rl, __uint_as_float(r[e + 1]) * rl);
-                                u.y = pack2(__uint_as_float(r[e + 2]) * rl, __uint_as_float(r[e + 3]) * rl);
-                                u.z = pack2(__uint_as_float(r[e + 4]) * rl, __uint_as_float(r[e + 5]) * rl);
-                                u.w = pack2(__uint_as_float(r[e + 6]) * rl, __uint_as_float(r[e + 7]) * rl);
+                                const uint32_t* v = r + 8 * k;
+                                u[k].x = pack2(__uint_as_float(v[0]) * rl, __uint_as_float(v[1]) * rl);
+                                u[k].y = pack2(__uint_as_float(v[2]) * rl, __uint_as_float(v[3]) * rl);
+                                u[k].z = pack2(__uint_as_float(v[4]) * rl, __uint_as_float(v[5]) * rl);
+                                u[k].w = pack2(__uint_as_float(v[6]) * rl, __uint_as_float(v[7]) * rl);
                             }
-                            if (live) d[4 * c + (e >> 3)] = u;
                         }
-                        __syncwarp();
+                        turn_pieces(u);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (on[k])
+                                *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + off[k] + 32 * c + 8 * (lane & 3)) = u[k];
                     }
                     tc_before();   // the next item's products may overwrite the outputs
                 }
