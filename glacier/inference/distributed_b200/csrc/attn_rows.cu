@@ -132,6 +132,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kConsumers = kRowWarps * 32;
 
+    // the tile kernel of the same call, where there is one, reads nothing that this one writes
+    if ((long long)p.max_new * p.G > kRows) grid_dep_launch_dependents();
     if (threadIdx.x == kConsumers) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");

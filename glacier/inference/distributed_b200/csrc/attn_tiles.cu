@@ -1218,6 +1218,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
     tc_before();
+    if (p.rows_take > 0 && threadIdx.x == 0) grid_dep_wait();   // what follows this launch waits for the row kernel too
     __syncthreads();
     if (warp == 9) {
         tc_after();
@@ -1231,19 +1232,24 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
     constexpr int smem = tiles_smem_bytes<F32>();
     static_assert(smem <= 232448, "shared memory of a CTA");
     cudaError_t e = cudaFuncSetAttribute(attn_tiles_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.stream = st;
+    cfg.attrs = attr;
     if (e == cudaSuccess) {
-        attn_tiles_kernel<F32><<<(unsigned)std::min<long long>(items, 148), kTcThreads, smem, st>>>(tq, tk, tv, p);
-        e = cudaGetLastError();
+        // behind the row kernel of the same call: CTAs start as its CTAs leave their SMs
+        cfg.gridDim = dim3((unsigned)std::min<long long>(items, 148));
+        cfg.blockDim = dim3(kTcThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.numAttrs = p.rows_take > 0 ? 1 : 0;
+        e = cudaLaunchKernelEx(&cfg, attn_tiles_kernel<F32>, tq, tk, tv, p);
     }
     if (e == cudaSuccess && p.split) {
-        cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(kJoinCtas);
         cfg.blockDim = dim3(256);
-        cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
+        cfg.dynamicSmemBytes = 0;
         cfg.numAttrs = 1;
         e = cudaLaunchKernelEx(&cfg, attn_tiles_join_kernel<F32>, p);
     }
