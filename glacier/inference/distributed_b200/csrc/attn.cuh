@@ -122,6 +122,10 @@ __device__ __forceinline__ void store_pair(void* out, int64_t off, float2 a, flo
 // ---- the kernels, and what a call needs of them
 constexpr int kTileRows = 256;                  // query rows of an item of the tile kernel
 constexpr int kTileParts = 8;                   // most parts of a unit's keys
+// From two units an SM on, whole units fill the SMs better than parts with their
+// join: 192 units of 130 key tiles take 456 us cut and 565 whole, 312 units of 65
+// take 490 cut and 430 whole (48 heads over 8, fp16 queries).
+constexpr int kCutUnits = 2 * 148;
 constexpr int kTileExtra = 3 * 148;             // most items that cutting units into parts adds
 constexpr int kTilePartFloats = kTileRows * (kHd + 2);
 constexpr int kTileUnitBytes = 32;              // a place's entry for the join

@@ -61,12 +61,16 @@ AttnPlan plan_attention(int n_heads, int n_kv, int B, int T, int max_new, bool w
     AttnPlan a{};
     // A sequence of up to 16 rows a KV head is the row kernel's.  With longer ones
     // in the batch the row kernel comes first where there may be several short
-    // ones; a batch of up to four is left to the tiles, the empty launch costs 3 us.
+    // ones; a batch of up to four is left to the tiles, where the short ones fill SMs
+    // that would idle.  300 tokens at 2,000 keys (48 heads over 8, fp16) next to k
+    // single ones at 4,000, both kernels against tiles alone: k = 1 64 against 72 us,
+    // 3 74 against 64, 4 78 against 87, 16 107 against 140.
     a.tiles = (long long)max_new * G > kRows;
     a.rows = !a.tiles || (workspace && B > 4);
     const long long units = ((long long)T / kTileTokens(G) + std::min(B, T)) * n_kv;
-    // Many units fill the SMs by themselves, and each CTA looks through all sequences
-    a.split = a.tiles && workspace && units <= 16 * 148;
+    // The kernel cuts up to kCutUnits units; the host, which does not know the lengths,
+    // leaves the joining launch out where there may be many more.
+    a.split = a.tiles && workspace && units <= 8 * kCutUnits;
     a.items = units + (a.split ? kTileExtra : 0);
     // (room for parts also where none are cut: a workspace serves every smaller call)
     a.slots = a.tiles && workspace ? (int)std::min<long long>(units * kTileParts, 2 * kTileExtra) : 0;

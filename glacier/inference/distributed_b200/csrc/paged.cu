@@ -658,7 +658,7 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
     // A warp's four angles (double reduction, sincosf: ~200 instructions) serve its
     // run of head pairs: long runs where there are warps enough, one pair a warp
     // where the call is short (8192 rows of 48 / 8 heads: 158 us with runs of one
-    // pair, 78 us with eight).
+    // pair, 76 us with eight: 5.8 TB/s).
     p.run = (int)std::min<long long>(8, std::max<long long>(1, (long long)T * pairs / (148 * 64)));
     const long long warps = (long long)T * ((pairs + p.run - 1) / p.run);
     const long long blocks = (warps + 7) / 8;
