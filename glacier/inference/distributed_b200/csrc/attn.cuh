@@ -29,6 +29,7 @@ struct AttnBatch {
     const int32_t* table;           // [B][max_pages]
     int max_pages, ps_log2, n_pages, box_rows;
     int B, T, max_new, n_heads, n_kv, G, tokens_per_tile;
+    int row_tile_tokens;            // tokens of a row tile of the tile kernel: one or two make a unit
     unsigned unit_mul;              // x / tokens_per_tile = (x * unit_mul >> 32) >> unit_shift, 0 <= x < 2^31
     int unit_shift;
     float scale_log2;               // softmax scale times log2(e)

@@ -35,15 +35,15 @@ unsigned long long next_nonce() {
     return ((z ^ (z >> 31)) & ~0xffull) | 0x100ull;
 }
 
-// Tokens of an item of the tile kernel: two row tiles of 128 rows.
-constexpr int kTileTokens(int G) { return 2 * (kTileRows / 2 / G); }
+// Tokens of a row tile of the tile kernel, 128 rows.
+constexpr int kRowTileTokens(int G) { return kTileRows / 2 / G; }
 
 // Descriptor of fp16 queries as [2 halves][tokens][heads][64]: a box is a row tile's
 // tokens times the heads of a KV head of one 64-element half, 128-byte swizzled.
 int query_map(CUtensorMap* map, const AttnBatch& p) {
     const cuuint64_t dims[4] = {64, (cuuint64_t)p.n_heads, (cuuint64_t)p.T, 2};
     const cuuint64_t strides[3] = {kHd * 2, (cuuint64_t)p.q_stride * 2, 128};
-    const cuuint32_t box[4] = {64, (cuuint32_t)p.G, (cuuint32_t)(p.tokens_per_tile / 2), 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)p.G, (cuuint32_t)p.row_tile_tokens, 1};
     return paged_encode(map, p.q, 4, dims, strides, box);
 }
 
@@ -51,6 +51,7 @@ int query_map(CUtensorMap* map, const AttnBatch& p) {
 struct AttnPlan {
     bool rows, tiles;     // kernels that are launched
     bool split;           // units of the tile kernel may be cut
+    int row_tiles;        // of a unit of the tile kernel
     long long items;      // most items of it
     int slots;            // and of their partials
     size_t work;          // workspace bytes
@@ -67,7 +68,16 @@ AttnPlan plan_attention(int n_heads, int n_kv, int B, int T, int max_new, bool w
     // 3 74 against 64, 4 78 against 87, 16 107 against 140.
     a.tiles = (long long)max_new * G > kRows;
     a.rows = !a.tiles || (workspace && B > 4);
-    const long long units = ((long long)T / kTileTokens(G) + std::min(B, T)) * n_kv;
+    const auto units_of = [&](int row_tiles) {   // at most
+        return ((long long)T / (row_tiles * kRowTileTokens(G)) + std::min(B, T)) * n_kv;
+    };
+    // Two row tiles share a CTA's keys and hide each other's chain; packed prompts that
+    // would leave half of the SMs without any take one a unit (40 heads over 8, fp32:
+    // 33 tokens 14.8 against 17.0 us, 300 21.6 against 25.3; at 450, 208 units, 24.7
+    // against 28.7, but at 600, 264 units, 36 against 32).  Over pages keys are cut
+    // instead (300 tokens at 8,000 keys: 102 us as pairs in parts, 165 singly).
+    a.row_tiles = !workspace && units_of(1) <= 148 ? 1 : 2;
+    const long long units = units_of(a.row_tiles);
     // The kernel cuts up to kCutUnits units; the host, which does not know the lengths,
     // leaves the joining launch out where there may be many more.
     a.split = a.tiles && workspace && units <= 8 * kCutUnits;
@@ -91,8 +101,9 @@ int attn_launch(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap&
         if (int rc = attn_rows_launch(f32, tk, tv, p, st)) return rc;
     }
     if (!a.tiles) return GLC_OK;
-    p.tokens_per_tile = kTileTokens(p.G);
-    // ceil(2^(31 + l) / d) with 2^(l - 1) < d <= 2^l: exact below 2^31 (d is 16 at least)
+    p.row_tile_tokens = kRowTileTokens(p.G);
+    p.tokens_per_tile = a.row_tiles * p.row_tile_tokens;
+    // ceil(2^(31 + l) / d) with 2^(l - 1) < d <= 2^l: exact below 2^31 (d is 8 at least)
     int l = 1;
     while ((1 << l) < p.tokens_per_tile) ++l;
     p.unit_mul = (unsigned)(((1ull << (31 + l)) + p.tokens_per_tile - 1) / p.tokens_per_tile);

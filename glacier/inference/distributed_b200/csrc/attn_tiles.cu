@@ -352,7 +352,7 @@ struct ItemWalk {
         const int u = np == 1 ? in : (int)((unsigned)in / (unsigned)np), part = in - u * np;   // unit of the class's, from its end
         const int ul = (int)((unsigned)u / (unsigned)p.n_kv);
         const int slot = slots + __shfl_sync(0xffffffffu, send - split, l) + u * np;
-        const int tpt = p.tokens_per_tile >> 1;
+        const int tpt = p.row_tile_tokens;
         it.seq = b0 - l;
         it.g = u - ul * p.n_kv;
         const int tok0 = (__shfl_sync(0xffffffffu, low, l) + nu - 1 - ul) * p.tokens_per_tile;
@@ -365,7 +365,7 @@ struct ItemWalk {
         int nt[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            it.ntok[t] = max(0, min(tpt, n - tok0 - t * tpt));
+            it.ntok[t] = max(0, min(tpt, min(n - tok0, p.tokens_per_tile) - t * tpt));
             const int see = it.ntok[t] ? max(0, min(it.kv_len, it.see0 - 1 + t * tpt + it.ntok[t])) : 0;
             nt[t] = (see + kTile - 1) / kTile;
             it.kv_end = max(it.kv_end, see);
@@ -749,7 +749,7 @@ constexpr int kJoinCtas = 4 * 148;
 template <bool F32>
 __global__ void __launch_bounds__(256, 4) attn_tiles_join_kernel(const __grid_constant__ AttnBatch p) {
     grid_dep_wait();
-    const int places = *tile_places(p), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tpt = p.tokens_per_tile >> 1;
+    const int places = *tile_places(p), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tpt = p.row_tile_tokens;
     for (int w = blockIdx.x; w < 8 * places; w += kJoinCtas) {
         const TileUnit u = *tile_unit(p, w >> 3);
         const int t = (w >> 2) & 1, row = 32 * (w & 3) + lane;
@@ -838,7 +838,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_after();
     const uint32_t tmem = S.tmem;
     grid_dep_launch_dependents();
-    const int tpt = p.tokens_per_tile >> 1;   // tokens per row tile
+    const int tpt = p.row_tile_tokens;   // tokens per row tile
 
     // the i-th item of the CTA, for a role (a whole warp): false at the end
     auto take = [&](int i, bool& ok) {
