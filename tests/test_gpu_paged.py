@@ -576,6 +576,47 @@ def test_graphs_that_share_a_workspace(cuda, glc, new, kv):
             p.check()
 
 
+def test_mixed_call_is_done_when_the_next_starts(cuda, glc):
+    """A copy right behind a call of both kernels sees all of its rows, live and
+    captured, while the queries and the outputs change between calls."""
+    torch = cuda
+    rng = np.random.default_rng(19)
+    p = Paged(torch, glc, rng, [1, 1, 40, 2, 1, 1, 1, 150], [900, 5000, 700, 64, 0, 3, 1700, 2000], 12, 2, 16, F16)
+    flip = -p.dq
+    p.call()
+    glc.paged_poll_error()
+    p.check()
+    want = p.out.clone()
+    p.dq.copy_(flip)
+    p.call()
+    want2 = p.out.clone()
+    glc.paged_poll_error()
+    assert not torch.equal(want, want2)
+    stream = torch.cuda.Stream()
+    copies = torch.empty(12, *p.out.shape, dtype=p.out.dtype, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for i in range(12):
+            p.dq.neg_()
+            p.out.fill_(7.0)
+            p.call(stream=stream.cuda_stream)
+            copies[i].copy_(p.out)
+    glc.paged_poll_error()
+    assert all(torch.equal(copies[i], want2 if i % 2 else want) for i in range(12))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for i in range(4):
+            p.dq.neg_()
+            p.out.fill_(7.0)
+            p.call(stream=torch.cuda.current_stream().cuda_stream)
+            copies[i].copy_(p.out)
+    for _ in range(3):
+        copies.zero_()
+        g.replay()
+        glc.paged_poll_error()
+        assert all(torch.equal(copies[i], want2 if i % 2 else want) for i in range(4))
+
+
 def test_host_memory_is_refused(cuda, glc):
     torch = cuda
     a = np.zeros(1 << 16, np.uint8)
