@@ -221,17 +221,21 @@ extern "C" int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_strid
     while ((1 << p.ps_log2) < cache->page_size) ++p.ps_log2;
     p.box_rows = std::min(cache->page_size, glc::kTile);
     const glc::AttnPlan a = glc::plan_attention(n_heads, cache->n_kv_heads, B, T, max_new, true);
-    CUtensorMap tk, tv, ttk, ttv;
+    CUtensorMap tk{}, tv{}, ttk{}, ttv{};   // of the row kernel, of the tile kernel
     const auto map = [&](CUtensorMap* m, const void* base, int halves) {
         return glc::paged_tensor_map(m, base, cache->page_size, cache->row_stride, cache->n_kv_heads, cache->head_stride,
                                      cache->n_pages, cache->page_stride, p.box_rows, halves);
     };
-    if (int rc = map(&tk, cache->k, 2)) return rc;
-    if (int rc = map(&tv, cache->v, 2)) return rc;
+    if (a.rows) {
+        if (int rc = map(&tk, cache->k, 2)) return rc;
+        if (int rc = map(&tv, cache->v, 2)) return rc;
+    }
     // the tile kernel's K and V lie as two blocks of 64 dims: a box that covers part
     // of a tile's keys is one block's, one that covers them all takes both
     const int halves = p.box_rows < glc::kTile ? 1 : 2;
-    if (int rc = map(&ttk, cache->k, halves)) return rc;
-    if (int rc = map(&ttv, cache->v, halves)) return rc;
+    if (a.tiles) {
+        if (int rc = map(&ttk, cache->k, halves)) return rc;
+        if (int rc = map(&ttv, cache->v, halves)) return rc;
+    }
     return glc::attn_launch(tk, tv, ttk, ttv, p, a, q_type == GLC_GGUF_F32, (cudaStream_t)stream);
 }
