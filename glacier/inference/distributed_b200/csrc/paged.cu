@@ -653,7 +653,14 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
     p.T = T;
     p.n_heads = n_heads;
     p.n_kv = n_kv_heads;
-    for (int i = 0; i < 64; ++i) p.inv_freq[i] = std::exp(-(double)(2 * i) / 128.0 * std::log((double)rope_theta));
+    // theta^(-i/64) as products of six powers: 64 exponentials take 1 us, as long as the
+    // launch; five roundings in double do not show in an fp32 angle
+    const double step = -std::log((double)rope_theta) / 64.0;
+    p.inv_freq[0] = 1.0;
+    for (int n = 1; n < 64; n *= 2) {
+        const double f = std::exp(n * step);
+        for (int i = 0; i < n; ++i) p.inv_freq[n + i] = p.inv_freq[i] * f;
+    }
     const long long pairs = (n_heads + 2LL * n_kv_heads + 1) / 2;
     // A warp's four angles (double reduction, sincosf: ~200 instructions) serve its
     // run of head pairs: long runs where there are warps enough, one pair a warp
