@@ -25,7 +25,8 @@
 // core works 2,500 (a product of 128 x 128 x 16 takes 87 cycles with both operands in
 // shared memory, 67 with A in tensor memory) and the exponentials 2,050, and 6,200
 // with fp32 ones (4,600 and 2,050).  16,384 tokens (48 heads over 8, fp16) take
-// 3.1 ms, 1,060 TFLOP/s; 512 tokens against 32,513 keys (40 over 8, fp32) 575 us.
+// 3.1 ms, 1,060 TFLOP/s; 512 tokens against 32,513 keys (40 over 8, fp32) 575 us
+// (3.5 ms and 670 us where the power limit holds the clock down).
 // An item costs 4,000 cycles more for its outputs, and fp32 queries 7,000 to load.
 #include <algorithm>
 #include <type_traits>
