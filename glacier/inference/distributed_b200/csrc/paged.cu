@@ -331,13 +331,13 @@ __device__ __forceinline__ int upper(const int* end, int n, int x) {
 // Sums past what they are compared with (T rows, the pages there are) are held
 // one above it, so 32 bits carry them.
 __global__ void __launch_bounds__(1024, 1) kv_plan_flat_kernel(const __grid_constant__ PlanParams p) {
-    extern __shared__ int plan_smem[];
-    int* row_end = plan_smem;         // [B] inclusive ends: rows, pages given back, pages taken
+    extern __shared__ long long plan_smem[];
+    long long* part = plan_smem;                            // [32]
+    int* row_end = reinterpret_cast<int*>(plan_smem + 32);  // [B] inclusive ends: rows, pages given back, pages taken
     int* back_end = row_end + p.B;
     int* page_end = back_end + p.B;
     int* s_ctx = page_end + p.B;
     int* s_held = s_ctx + p.B;        // pages held, -1 - held for a request that is not served
-    __shared__ long long part[32];
     const int tid = threadIdx.x, nt = blockDim.x, items = (p.B + nt - 1) / nt, i0 = tid * items;
     const int ps = 1 << p.ps_log2;
     const int n = max(0, min(items, p.B - i0));
@@ -578,7 +578,7 @@ extern "C" int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens,
         const int threads = B <= 256 ? 256 : 1024;
         const long long work = std::max<long long>(T, B);
         const int grid = (int)std::min<long long>(148, (work + threads - 1) / threads);
-        const int smem = 5 * (int)sizeof(int) * B;
+        const int smem = 32 * (int)sizeof(long long) + 5 * (int)sizeof(int) * B;   // all that the kernel has
         if (smem > 48 * 1024)
             e = cudaFuncSetAttribute(glc::kv_plan_flat_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e == cudaSuccess) {
