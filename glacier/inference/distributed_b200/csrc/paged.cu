@@ -328,6 +328,9 @@ __device__ __forceinline__ int upper(const int* end, int n, int x) {
     return lo;
 }
 
+// All of the shared memory of kv_plan_flat_kernel
+constexpr int plan_flat_smem(int B) { return 32 * (int)sizeof(long long) + 5 * (int)sizeof(int) * B; }
+
 // Sums past what they are compared with (T rows, the pages there are) are held
 // one above it, so 32 bits carry them.
 __global__ void __launch_bounds__(1024, 1) kv_plan_flat_kernel(const __grid_constant__ PlanParams p) {
@@ -578,9 +581,12 @@ extern "C" int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens,
         const int threads = B <= 256 ? 256 : 1024;
         const long long work = std::max<long long>(T, B);
         const int grid = (int)std::min<long long>(148, (work + threads - 1) / threads);
-        const int smem = 32 * (int)sizeof(long long) + 5 * (int)sizeof(int) * B;   // all that the kernel has
+        const int smem = glc::plan_flat_smem(B);
+        // the limit belongs to the kernel, not to the call: always that of the largest plan, so
+        // that no other host thread lowers it before this launch
         if (smem > 48 * 1024)
-            e = cudaFuncSetAttribute(glc::kv_plan_flat_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            e = cudaFuncSetAttribute(glc::kv_plan_flat_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     glc::plan_flat_smem(glc::kPlanFlat));
         if (e == cudaSuccess) {
             glc::kv_plan_flat_kernel<<<std::max(grid, 1), threads, smem, (cudaStream_t)stream>>>(p);
             e = cudaGetLastError();

@@ -2,6 +2,7 @@
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -30,3 +31,42 @@ def test_plan_of_every_size_in_a_fresh_process(cuda):
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([REPO, HERE, os.environ.get("PYTHONPATH", "")]))
     out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, out.stdout[-2000:] + out.stderr[-2000:]
+
+
+def test_plans_from_two_host_threads(cuda, glc):
+    """Calls of 2,500 and of 4,096 requests at once: neither changes what the other
+    may launch."""
+    torch = cuda
+    cases = [plan_case(np.random.default_rng(B), B, 16, 90, 3) for B in (2500, 4096)]
+    for c in cases:
+        run_plan(torch, glc, c[0], c[1], 16, *c[2:], 9000)
+    errors, stop = [], threading.Event()
+
+    def many(c, n):
+        ctx, new, table, pool, free = c
+        B, width = table.shape
+        s = torch.cuda.Stream()
+        d = [torch.from_numpy(a).cuda() for a in (ctx, new, table, pool, np.array([free], np.int32))]
+        o = [torch.zeros(k, dtype=torch.int32, device="cuda") for k in (1, B + 1, B, 9000, 1)]
+        slots = torch.zeros(9000, dtype=torch.int64, device="cuda")
+        torch.cuda.synchronize()
+        a = [t.data_ptr() for t in d + o + [slots]]
+        try:
+            for i in range(n):
+                if stop.is_set():
+                    break
+                glc.kv_plan_dev(a[0], a[1], B, 16, a[2], width, a[3], len(pool), a[4], a[5], 9000, a[6], a[7], a[8], a[10],
+                                a[9], stream=s.cuda_stream)
+                if i % 100 == 99:
+                    s.synchronize()
+        except glc.GlcError as e:
+            errors.append(e)
+            stop.set()
+        s.synchronize()
+
+    threads = [threading.Thread(target=many, args=(c, 6000)) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
