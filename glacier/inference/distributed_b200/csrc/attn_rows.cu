@@ -80,7 +80,7 @@ __device__ __forceinline__ RowsUnit load_unit(const AttnBatch& p, int b, bool re
     if (p.kv_lens) {
         const long long room = (long long)p.max_pages << p.ps_log2;
         u.kv_len = (int)min((long long)max(len, 0), room);
-        if (record && (len != u.kv_len || u.n > p.max_new)) atomicExch(p.err, kDevBadArg);
+        if (record && (len != u.kv_len || u.n > p.max_new)) record_bad_arg(p.err);
     }
     if (u.n * p.G > p.rows_take) u.n = 0;   // the tile kernel's
     u.tiles = u.n > 0 ? (u.kv_len + kTile - 1) / kTile : 0;
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
                     page = p.table[(long long)w.b * p.max_pages + (r0 >> p.ps_log2)];
                     row = r0 & (ps - 1);
                     if ((unsigned)page >= (unsigned)p.n_pages) {  // reads as zeros
-                        atomicExch(p.err, kDevBadArg);
+                        record_bad_arg(p.err);
                         page = p.n_pages;
                     }
                 }

@@ -197,7 +197,7 @@ __device__ __forceinline__ SeqUnits seq_units(const AttnBatch& p, int b, bool re
         const long long room = (long long)p.max_pages << p.ps_log2;
         const int len = p.kv_lens[b];
         u.kv_len = (int)min((long long)max(len, 0), room);
-        if (record && u.n > 0 && (len != u.kv_len || u.n > p.max_new)) atomicExch(p.err, kDevBadArg);
+        if (record && u.n > 0 && (len != u.kv_len || u.n > p.max_new)) record_bad_arg(p.err);
     }
     return u;
 }
@@ -290,7 +290,7 @@ struct ItemWalk {
         for (int off = 16; off >= 1; off >>= 1) rows += __shfl_xor_sync(0xffffffffu, rows, off);
         // first rows that do not ascend may name more units than there is room for: no items
         if (rows > p.T) {
-            if (lane == 0) atomicExch(p.err, kDevBadArg);
+            if (lane == 0) record_bad_arg(p.err);
             total = 0;
             return;
         }
@@ -900,7 +900,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         page = p.table[(long long)it.seq * p.max_pages + (r0 >> p.ps_log2)];
                         row = r0 & (ps - 1);
                         if ((unsigned)page >= (unsigned)p.n_pages) {  // reads as zeros
-                            atomicExch(p.err, kDevBadArg);
+                            record_bad_arg(p.err);
                             page = p.n_pages;
                         }
                     }

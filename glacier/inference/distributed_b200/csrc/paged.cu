@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
     const int pos = p.pos[t];
     const long long slot = p.slots ? p.slots[t] : -1;
     const bool store = p.kc != nullptr && slot >= 0 && slot < p.n_slots;
-    if (p.kc != nullptr && slot >= p.n_slots && lane == 0) atomicExch(p.err, kDevBadArg);
+    if (p.kc != nullptr && slot >= p.n_slots && lane == 0) record_bad_arg(p.err);
     const long long page = slot >> p.ps_log2;
     const long long row_off = store ? page * p.page_stride + (slot - (page << p.ps_log2)) * p.row_stride : 0;
     float c[4], s[4];

@@ -19,6 +19,11 @@ int paged_fail(int code, const char* fmt, ...);
 // of the failure).  A fixed device word of the library: nothing is allocated.
 int paged_error_word(int** err);
 
+// Records a bad page id, slot or length.  A wait that gave up is never hidden by one:
+// the caller has to clear the workspace of captured calls after it (and that code is
+// recorded over this one).
+__device__ __forceinline__ void record_bad_arg(int* err) { atomicCAS(err, kDevOk, kDevBadArg); }
+
 // GLC_OK when `device_ptr` is memory the current device owns or can be handed
 // without faulting (managed and pinned host memory included).
 int paged_check_device(const void* device_ptr, const char* what);

@@ -14,6 +14,7 @@ pytestmark = pytest.mark.gpu
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
+LIBDIR = os.path.join(REPO, "glacier", "inference", "distributed_b200")
 
 
 def plans_ascending(torch, glc):
@@ -70,3 +71,17 @@ def test_plans_from_two_host_threads(cuda, glc):
     for t in threads:
         t.join()
     assert not errors
+
+
+def built(tmp_path, name):
+    exe = str(tmp_path / name)
+    subprocess.check_call(["/usr/local/cuda/bin/nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O2",
+                           "--expt-relaxed-constexpr", "-I", os.path.join(REPO, "include"), "-I", os.path.join(LIBDIR, "csrc"),
+                           os.path.join(HERE, "cpp", name + ".cu"), "-o", exe, "-L", LIBDIR, "-lglacier_b200",
+                           "-Xlinker", f"-rpath={LIBDIR}"])
+    return exe
+
+
+def test_bad_argument_does_not_hide_a_timeout(cuda, tmp_path):
+    out = subprocess.run([built(tmp_path, "paged_error_check")], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stdout + out.stderr
