@@ -20,6 +20,11 @@
 namespace glc {
 
 static __device__ int g_paged_err;
+static __device__ int g_paged_seen;   // what a poll took from it
+
+// Read and cleared in one step: what another stream records meanwhile is in this
+// poll or in the next.
+static __global__ void take_error_kernel() { g_paged_seen = atomicExch(&g_paged_err, kDevOk); }
 
 int paged_fail(int code, const char* fmt, ...) {
     char buf[512];
@@ -686,14 +691,17 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
 }
 
 extern "C" int glc_paged_poll_error(void) {
-    int* err = nullptr;
-    if (int rc = glc::paged_error_word(&err)) return rc;
+    static std::mutex mu;   // one poll at a time has the word it was read to
+    std::lock_guard<std::mutex> lk(mu);
     int code = 0;
     cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaMemcpy(&code, err, sizeof(int), cudaMemcpyDeviceToHost);
-    if (e == cudaSuccess && code) e = cudaMemset(err, 0, sizeof(int));
+    if (e == cudaSuccess) {
+        glc::take_error_kernel<<<1, 1, 0, cudaStreamLegacy>>>();
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&code, glc::g_paged_seen, sizeof(int));
     if (e != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "device error word: %s", cudaGetErrorString(e));
-    if (code == 0) return GLC_OK;
+    if (code == glc::kDevOk) return GLC_OK;
     if (code == glc::kDevBadArg)
         return paged_fail(GLC_ERR_INVALID_ARG, "a page id, slot or length on the device was out of range");
     return paged_fail(GLC_ERR_TIMEOUT, "a device-side wait of the paged attention gave up (code %d)", code);
