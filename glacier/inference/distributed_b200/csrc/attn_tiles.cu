@@ -392,6 +392,37 @@ struct ItemWalk {
     }
 };
 
+// The scheduler warp: hands the CTA's items out, an end marker behind them.  After a
+// wait that gave up it hands out no more but walks on, as every place of the workspace
+// that the joining launch reads is written on this walk.
+__device__ __forceinline__ void hand_out_items(const AttnBatch& p, TilesSmem& S) {
+    const int lane = threadIdx.x & 31;
+    ItemWalk w;
+    w.init(p);
+    if (p.split && blockIdx.x == 0 && lane == 0) *tile_places(p) = min(w.cut, p.slots);
+    const int ctas = gridDim.x, c = blockIdx.x;
+    bool ok = true;
+    int i = 0;
+    for (int r = 0;; ++r) {
+        const int x = r * ctas + ((r & 1) ? ctas - 1 - c : c);
+        TileItem it;
+        if (r * ctas >= w.total) it.seq = -1;
+        else if (x >= w.total || !w.get(p, x, it)) continue;
+        if (ok) {
+            const int buf = i % kItemBufs;
+            ok = mbar_wait_backoff(&S.item_empty[buf], ((uint32_t)(i / kItemBufs) & 1u) ^ 1u, p.err, kDevTimeoutEmpty, 64);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok && lane == 0) {
+                S.item[buf] = it;
+                mbar_arrive(&S.item_full[buf]);
+            }
+            __syncwarp();
+            ++i;
+        }
+        if (it.seq < 0) break;
+    }
+}
+
 // Pairs of fp32 values in one 64-bit register: half the issue slots of scalar
 // arithmetic.  Volatile on purpose: the compiler otherwise sinks a chunk's
 // arithmetic below the next chunk's tensor-memory load, keeps several chunks
@@ -857,30 +888,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 11) {
             // ------------------------------------------------------- next items
-            ItemWalk w;
-            w.init(p);
-            if (p.split && blockIdx.x == 0 && lane == 0) *tile_places(p) = min(w.cut, p.slots);
-            const int ctas = gridDim.x, c = blockIdx.x;
-            bool ok = true;
-            int i = 0;
-            for (int r = 0; ok; ++r) {
-                const int x = r * ctas + ((r & 1) ? ctas - 1 - c : c);
-                TileItem it;
-                if (r * ctas >= w.total) it.seq = -1;
-                else if (x >= w.total || !w.get(p, x, it)) continue;
-                const int buf = i % kItemBufs;
-                ok = mbar_wait_backoff(&S.item_empty[buf], ((uint32_t)(i / kItemBufs) & 1u) ^ 1u, p.err, kDevTimeoutEmpty,
-                                       64);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) {
-                    S.item[buf] = it;
-                    mbar_arrive(&S.item_full[buf]);
-                }
-                __syncwarp();
-                ++i;
-                if (it.seq < 0) break;
-            }
+            hand_out_items(p, S);
         } else if (warp == 8) {
             // --------------------------------------------- Q (fp16), K and V tiles
             const int ps = 1 << p.ps_log2, nbox = kTile / p.box_rows, halves = nbox == 1 ? 1 : 2;

@@ -90,3 +90,8 @@ def test_bad_argument_does_not_hide_a_timeout(cuda, tmp_path):
 def test_no_error_is_lost_to_a_poll(cuda, tmp_path):
     out = subprocess.run([built(tmp_path, "paged_error_check"), "lost"], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0, out.stdout + out.stderr
+
+
+def test_places_of_the_join_are_written_after_a_timeout(cuda, tmp_path):
+    out = subprocess.run([built(tmp_path, "tiles_scheduler_check")], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stdout + out.stderr
