@@ -486,6 +486,8 @@ __device__ __forceinline__ void store4(__half* d, float4 a) {
 }
 __device__ __forceinline__ void store4(float* d, float4 a) { *reinterpret_cast<float4*>(d) = a; }
 
+constexpr int kRopeBatch = 4;   // heads a thread has in flight
+
 template <typename QO>
 __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeParams p) {
     const int lane = threadIdx.x & 31, sub = lane & 15;
@@ -501,42 +503,61 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
     if (p.kc != nullptr && slot >= p.n_slots && lane == 0) record_bad_arg(p.err);
     const long long page = slot >> p.ps_log2;
     const long long row_off = store ? page * p.page_stride + (slot - (page << p.ps_log2)) * p.row_stride : 0;
+    const int hend = min(heads, h0 + 2 * p.run);
+    // The loads of kRopeBatch heads, then their stores: coherent loads (in place the launch
+    // writes these rows too) that no store holds up, the first ones under way while the
+    // angles are formed.  A thread stores to an address only what it formed from the value
+    // there.
+    float4 a[kRopeBatch], b[kRopeBatch];
+    auto load = [&](int hb) {
+#pragma unroll
+        for (int i = 0; i < kRopeBatch; ++i) {
+            const int h = hb + 2 * i;
+            if (h >= hend) break;
+            const float* src = h < p.n_heads ? p.q + t * p.q_stride + (int64_t)h * 128
+                               : h < p.n_heads + p.n_kv ? p.k + t * p.kv_stride + (int64_t)(h - p.n_heads) * 128
+                                                        : p.v + t * p.kv_stride + (int64_t)(h - p.n_heads - p.n_kv) * 128;
+            a[i] = *(reinterpret_cast<const float4*>(src) + sub);
+            b[i] = *(reinterpret_cast<const float4*>(src + 64) + sub);
+        }
+    };
+    load(h0 + (lane >> 4));
     float c[4], s[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) rope_cs(pos, p.inv_freq[4 * sub + e], c[e], s[e]);
-    const int hend = min(heads, h0 + 2 * p.run);
-#pragma unroll 4
-    for (int h = h0 + (lane >> 4); h < hend; h += 2) {
-        const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv;
-        const int kh = h - p.n_heads - (is_k ? 0 : p.n_kv);
-        const float* src = is_q ? p.q + t * p.q_stride + (int64_t)h * 128
-                                : (is_k ? p.k : p.v) + t * p.kv_stride + (int64_t)kh * 128;
-        const float4 a = __ldg(reinterpret_cast<const float4*>(src) + sub);
-        const float4 b = __ldg(reinterpret_cast<const float4*>(src + 64) + sub);
-        float4 x = a, y = b;
-        if (is_q || is_k) {
-            x = make_float4(a.x * c[0] - b.x * s[0], a.y * c[1] - b.y * s[1], a.z * c[2] - b.z * s[2],
-                            a.w * c[3] - b.w * s[3]);
-            y = make_float4(b.x * c[0] + a.x * s[0], b.y * c[1] + a.y * s[1], b.z * c[2] + a.z * s[2],
-                            b.w * c[3] + a.w * s[3]);
-        }
-        if (is_q) {
-            QO* d = static_cast<QO*>(p.q_out) + ((int64_t)t * p.n_heads + h) * 128 + 4 * sub;
-            store4(d, x);
-            store4(d + 64, y);
-        } else {
-            if (store) {
-                __half* d = (is_k ? p.kc : p.vc) + row_off + (int64_t)kh * p.head_stride + 4 * sub;
+    for (int hb = h0 + (lane >> 4); hb < hend; hb += 2 * kRopeBatch) {
+#pragma unroll
+        for (int i = 0; i < kRopeBatch; ++i) {
+            const int h = hb + 2 * i;
+            if (h >= hend) break;
+            const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv;
+            const int kh = h - p.n_heads - (is_k ? 0 : p.n_kv);
+            float4 x = a[i], y = b[i];
+            if (is_q || is_k) {
+                x = make_float4(a[i].x * c[0] - b[i].x * s[0], a[i].y * c[1] - b[i].y * s[1], a[i].z * c[2] - b[i].z * s[2],
+                                a[i].w * c[3] - b[i].w * s[3]);
+                y = make_float4(b[i].x * c[0] + a[i].x * s[0], b[i].y * c[1] + a[i].y * s[1], b[i].z * c[2] + a[i].z * s[2],
+                                b[i].w * c[3] + a[i].w * s[3]);
+            }
+            if (is_q) {
+                QO* d = static_cast<QO*>(p.q_out) + ((int64_t)t * p.n_heads + h) * 128 + 4 * sub;
                 store4(d, x);
                 store4(d + 64, y);
-            }
-            __half* o = is_k ? p.k_out : p.v_out;
-            if (o) {
-                o += ((int64_t)t * p.n_kv + kh) * 128 + 4 * sub;
-                store4(o, x);
-                store4(o + 64, y);
+            } else {
+                if (store) {
+                    __half* d = (is_k ? p.kc : p.vc) + row_off + (int64_t)kh * p.head_stride + 4 * sub;
+                    store4(d, x);
+                    store4(d + 64, y);
+                }
+                __half* o = is_k ? p.k_out : p.v_out;
+                if (o) {
+                    o += ((int64_t)t * p.n_kv + kh) * 128 + 4 * sub;
+                    store4(o, x);
+                    store4(o + 64, y);
+                }
             }
         }
+        load(hb + 2 * kRopeBatch);
     }
 }
 
@@ -674,10 +695,11 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
     }
     const long long pairs = (n_heads + 2LL * n_kv_heads + 1) / 2;
     // A warp's four angles (double reduction, sincosf: ~200 instructions) serve its
-    // run of head pairs: long runs where there are warps enough, one pair a warp
-    // where the call is short (8192 rows of 48 / 8 heads: 158 us with runs of one
-    // pair, 76 us with eight: 5.8 TB/s).
-    p.run = (int)std::min<long long>(8, std::max<long long>(1, (long long)T * pairs / (148 * 64)));
+    // run of head pairs: the shortest run whose warps are resident at once (three CTAs an
+    // SM), up to eight pairs, and one pair a warp where the call is short (8192 rows of
+    // 48 / 8 heads, fp16 out: 234 us with runs of one pair, 68 us with eight: 5.8 TB/s;
+    // 300 rows of 28 / 4: 8.3 us with one, 6.3 with two).
+    p.run = (int)std::min<long long>(8, ((long long)T * pairs + 148 * 24 - 1) / (148 * 24));
     const long long warps = (long long)T * ((pairs + p.run - 1) / p.run);
     const long long blocks = (warps + 7) / 8;
     if (blocks > 0x7fffffffLL) return paged_fail(GLC_ERR_UNSUPPORTED, "%d rows are too many for one call", T);

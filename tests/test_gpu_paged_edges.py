@@ -73,6 +73,25 @@ def test_plans_from_two_host_threads(cuda, glc):
     assert not errors
 
 
+@pytest.mark.parametrize("T,Hq,Hkv", [(1, 40, 8), (700, 48, 8), (3000, 13, 1)])
+def test_rotary_store_in_place_gives_the_same_bits(cuda, glc, T, Hq, Hkv):
+    """Queries rotated where they lie, by warps that take one and several heads."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(T)
+    q, k, v = (torch.randn(T, h, 128, generator=g, device="cuda") for h in (Hq, Hkv, Hkv))
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") * 11
+    out = [torch.empty_like(q), torch.empty_like(q), q.clone()]
+    packed = [torch.zeros(2, T, Hkv, 128, dtype=torch.float16, device="cuda") for _ in range(3)]
+    for o, p in zip(out, packed):
+        src = o if o is out[2] else q
+        glc.rope_append_dev(src.data_ptr(), Hq * 128, k.data_ptr(), v.data_ptr(), Hkv * 128, T, Hq, Hkv, pos.data_ptr(), None,
+                            1e6, None, o.data_ptr(), glc.GGUF_F32, p[0].data_ptr(), p[1].data_ptr(),
+                            stream=glc.torch_stream_handle())
+    glc.paged_poll_error()
+    for o, p in zip(out[1:], packed[1:]):
+        assert torch.equal(o, out[0]) and torch.equal(p, packed[0])
+
+
 def built(tmp_path, name):
     exe = str(tmp_path / name)
     subprocess.check_call(["/usr/local/cuda/bin/nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O2",
