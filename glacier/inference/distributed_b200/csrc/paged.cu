@@ -13,6 +13,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
+#include <utility>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -561,6 +562,15 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
     }
 }
 
+// Whether any of T fp32 rows (`stride` elements apart, `row` long, row <= stride) meets
+// the bytes [at, end).
+bool rows_overlap(const float* base, int64_t stride, int64_t row, int T, uintptr_t at, uintptr_t end) {
+    if (row == 0 || at >= end) return false;
+    const uintptr_t b = (uintptr_t)base, len = (uintptr_t)row * 4, step = (uintptr_t)stride * 4;
+    const uintptr_t i = b + len > at ? 0 : (at - b - len) / step + 1;   // first row that ends behind `at`
+    return i < (uintptr_t)T && b + i * step < end;
+}
+
 }  // namespace
 
 }  // namespace glc
@@ -654,6 +664,14 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
         return paged_fail(GLC_ERR_INVALID_ARG, "row strides shorter than a row");
     if (q_out == q && n_heads > 0 && (q_out_type != GLC_GGUF_F32 || q_stride != (int64_t)n_heads * 128))
         return paged_fail(GLC_ERR_INVALID_ARG, "in place only as fp32 rows of n_heads x 128");
+    const int64_t q_row = (int64_t)n_heads * 128, kv_row = (int64_t)n_kv_heads * 128;
+    for (const auto& o : {std::make_pair(q_out, q_row * (q_out_type == GLC_GGUF_F32 ? 4 : 2)), std::make_pair(k_out, kv_row * 2),
+                          std::make_pair(v_out, kv_row * 2)}) {
+        const uintptr_t at = (uintptr_t)o.first, end = at + (uintptr_t)(T * o.second);
+        if (o.first && ((o.first != q && glc::rows_overlap(q, q_stride, q_row, T, at, end)) ||
+                        glc::rows_overlap(k, kv_stride, kv_row, T, at, end) || glc::rows_overlap(v, kv_stride, kv_row, T, at, end)))
+            return paged_fail(GLC_ERR_INVALID_ARG, "outputs overlap the rows of q, k or v");
+    }
     if (cache) {
         if (int rc = glc::paged_check_pages(cache)) return rc;
         if (cache->n_kv_heads != n_kv_heads)

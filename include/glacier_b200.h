@@ -317,8 +317,9 @@ int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens, int32_t B,
  * q_out [T][n_heads][128] in q_out_type (GLC_GGUF_F32 or GLC_GGUF_F16; may be
  * q itself for dense fp32 rows; n_heads 0: keys and values only).  cache NULL:
  * nothing is stored; slots < 0 are skipped, slots past the cache are skipped
- * and recorded (glc_paged_poll_error); two rows must not name one slot.  k_out / v_out: the same fp16 rows
- * packed [T][n_kv_heads][128], or NULL. */
+ * and recorded (glc_paged_poll_error); two rows must not name one slot.
+ * k_out / v_out: the same fp16 rows packed [T][n_kv_heads][128], or NULL.
+ * Outputs that overlap rows of q, k or v in any other way are refused. */
 int glc_rope_append_dev(const float* q, int64_t q_stride, const float* k, const float* v, int64_t kv_stride,
                         int32_t T, int32_t n_heads, int32_t n_kv_heads, const int32_t* positions,
                         const int64_t* slots, float rope_theta, const glc_kv_pages* cache, void* q_out,
