@@ -591,8 +591,16 @@ extern "C" int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens,
     if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
         return paged_fail(GLC_ERR_UNSUPPORTED, "page_size %d (16, 32, 64, 128 or 256)", page_size);
     // the CTAs of a launch read the inputs while others write the outputs
-    if (kv_lens == ctx_lens || kv_lens == new_lens || free_count_out == free_count)
-        return paged_fail(GLC_ERR_INVALID_ARG, "kv_lens and free_count_out must not alias the inputs");
+    struct Range {
+        const void* p;
+        int64_t bytes;
+    };
+    for (const Range& i : {Range{ctx_lens, 4LL * B}, Range{new_lens, 4LL * B}, Range{free_count, 4}})
+        for (const Range& o : {Range{block_table, 4LL * B * max_pages}, Range{free_list, 4LL * capacity}, Range{free_count_out, 4},
+                               Range{cu_new, 4LL * B + 4}, Range{kv_lens, 4LL * B}, Range{positions, 4LL * T},
+                               Range{slots, 8LL * T}, Range{status, 4}})
+            if ((uintptr_t)i.p < (uintptr_t)o.p + o.bytes && (uintptr_t)o.p < (uintptr_t)i.p + i.bytes)
+                return paged_fail(GLC_ERR_INVALID_ARG, "outputs must not alias ctx_lens, new_lens or free_count");
     if (int rc = glc::paged_check_device(status, "status")) return rc;
     glc::PlanParams p{};
     p.ctx = ctx_lens;

@@ -301,7 +301,7 @@ typedef struct glc_kv_pages {
  * requests (attention gives those zero rows); positions and slots [T] of
  * every new row (slot = page * page_size + row; slot -1, position 0 for the
  * rows of unserved requests and behind the last one); status = requests not
- * served.  kv_lens and free_count_out must not alias the inputs, and
+ * served.  No output may alias ctx_lens, new_lens or free_count, and
  * max_pages * page_size must fit 31 bits.  The same inputs give the same outputs
  * again, so a step can be planned twice. */
 int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens, int32_t B, int32_t page_size,

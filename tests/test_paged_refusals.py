@@ -2,7 +2,7 @@
 (decided on the host: no GPU is touched)."""
 import pytest
 
-from test_paged_oracle import F16, F32, P, append_args
+from test_paged_oracle import F16, F32, P, append_args, plan_args
 
 
 @pytest.mark.parametrize("kw", [
@@ -31,3 +31,31 @@ def test_append_takes_outputs_beside_inputs(glc, kw):
         a.update(k_ptr=8 * P, v_ptr=8 * P, q_out_type=F32)
     with pytest.raises(glc.GlcError, match="device|CUDA"):
         glc.rope_append_dev(**a)
+
+
+def apart(**kw):
+    """A plan of 100 requests and 100 rows whose arrays lie side by side."""
+    a = plan_args(B=100, T=100, capacity=40, max_pages=4)
+    at = P
+    for name, n in (("ctx_lens", 400), ("new_lens", 400), ("free_count", 4), ("free_count_out", 4), ("block_table", 1600),
+                    ("free_list", 160), ("cu_new", 404), ("kv_lens", 400), ("positions", 400), ("slots", 800), ("status", 4)):
+        a[name + "_ptr"] = at
+        at += n
+    a.update({k: a[v[0]] + v[1] for k, v in kw.items()})
+    return a
+
+
+@pytest.mark.parametrize("out", ["block_table_ptr", "free_list_ptr", "free_count_out_ptr", "cu_new_ptr", "kv_lens_ptr",
+                                 "positions_ptr", "slots_ptr", "status_ptr"])
+@pytest.mark.parametrize("over,offset", [("ctx_lens_ptr", 0), ("ctx_lens_ptr", 396), ("new_lens_ptr", 200),
+                                         ("free_count_ptr", 0)])
+def test_plan_refuses_outputs_over_inputs(glc, out, over, offset):
+    with pytest.raises(glc.GlcError, match="alias") as e:
+        glc.kv_plan_dev(**apart(**{out: (over, offset)}))
+    assert e.value.status == -1
+
+
+def test_plan_takes_arrays_side_by_side(glc):
+    """Goes on to the check of the memory, which fails for a made-up pointer."""
+    with pytest.raises(glc.GlcError, match="device|CUDA"):
+        glc.kv_plan_dev(**apart())
