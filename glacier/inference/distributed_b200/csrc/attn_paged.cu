@@ -168,7 +168,7 @@ extern "C" int glc_attn_prompt_dev(const void* q, int32_t q_type, int64_t q_stri
         kv_stride >= ((int64_t)1 << 38))
         return paged_fail(GLC_ERR_INVALID_ARG, "key and value rows must be 16-byte aligned and a row apart");
     if (B == 0 || T == 0) return GLC_OK;
-    if (int rc = glc::paged_check_device(k, "k")) return rc;
+    if (int rc = glc::paged_check_devices({{q, "q"}, {k, "k"}, {v, "v"}, {cu_seqlens, "cu_seqlens"}, {out, "out"}})) return rc;
     glc::AttnBatch p = glc::make_batch(q, q_stride, out, out_stride, cu_seqlens, B, T, n_heads, n_kv_heads, scale);
     if (int rc = glc::paged_error_word(&p.err)) return rc;
     p.box_rows = glc::kTile;  // the packed rows are one page of T rows
@@ -209,7 +209,10 @@ extern "C" int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_strid
         return paged_fail(GLC_ERR_INVALID_ARG, "workspace of %llu bytes is too small or not 16-byte aligned",
                           (unsigned long long)workspace_bytes);
     if (B == 0 || T == 0) return GLC_OK;
-    if (int rc = glc::paged_check_device(cache->k, "the cache")) return rc;
+    if (int rc = glc::paged_check_devices({{q, "q"}, {cache->k, "the cache's k"}, {cache->v, "the cache's v"},
+                                           {block_table, "block_table"}, {cu_new, "cu_new"}, {kv_lens, "kv_lens"},
+                                           {out, "out"}, {workspace, "workspace"}}))
+        return rc;
     glc::AttnBatch p = glc::make_batch(q, q_stride, out, out_stride, cu_new, B, T, n_heads, cache->n_kv_heads, scale);
     if (int rc = glc::paged_error_word(&p.err)) return rc;
     p.work = static_cast<float*>(workspace);

@@ -54,18 +54,35 @@ int paged_error_word(int** err) {
     return GLC_OK;
 }
 
-int paged_check_device(const void* device_ptr, const char* what) {
+// Driver function by name, looked up once.
+template <typename F>
+static F driver_fn(const char* name) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint(name, &ptr, cudaEnableDefault, &qr) != cudaSuccess || qr != cudaDriverEntryPointSuccess)
+        ptr = nullptr;
+    return (F)ptr;
+}
+
+int paged_check_devices(std::initializer_list<DevicePtr> ptrs) {
+    // (30 ns a pointer; 60 for the runtime's question, asked where this one does not settle it)
+    static const auto attribute = driver_fn<CUresult (*)(void*, CUpointer_attribute, CUdeviceptr)>("cuPointerGetAttribute");
     int dev = 0;
-    cudaPointerAttributes at{};
     if (cudaGetDevice(&dev) != cudaSuccess) return paged_fail(GLC_ERR_CUDA, "no CUDA device");
-    if (cudaPointerGetAttributes(&at, device_ptr) != cudaSuccess) {
-        cudaGetLastError();
-        return paged_fail(GLC_ERR_INVALID_ARG, "%s is not memory known to CUDA", what);
+    for (const DevicePtr& d : ptrs) {
+        int on = -1;
+        if (!d.p || (attribute && attribute(&on, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, (CUdeviceptr)d.p) == CUDA_SUCCESS && on == dev))
+            continue;
+        cudaPointerAttributes at{};
+        if (cudaPointerGetAttributes(&at, d.p) != cudaSuccess) {
+            cudaGetLastError();
+            return paged_fail(GLC_ERR_INVALID_ARG, "%s is not memory known to CUDA", d.what);
+        }
+        if (at.type == cudaMemoryTypeUnregistered)
+            return paged_fail(GLC_ERR_INVALID_ARG, "%s is not device memory", d.what);
+        if (at.type == cudaMemoryTypeDevice && at.device != dev)
+            return paged_fail(GLC_ERR_INVALID_ARG, "%s is on device %d, the current device is %d", d.what, at.device, dev);
     }
-    if (at.type == cudaMemoryTypeUnregistered)
-        return paged_fail(GLC_ERR_INVALID_ARG, "%s is not device memory", what);
-    if (at.type == cudaMemoryTypeDevice && at.device != dev)
-        return paged_fail(GLC_ERR_INVALID_ARG, "%s is on device %d, the current device is %d", what, at.device, dev);
     return GLC_OK;
 }
 
@@ -91,14 +108,7 @@ typedef CUresult (*PFN_encodeTiledKv)(CUtensorMap*, CUtensorMapDataType, cuuint3
 
 int paged_encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                  const cuuint32_t* box) {
-    static PFN_encodeTiledKv fn = [] {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult qr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qr) != cudaSuccess ||
-            qr != cudaDriverEntryPointSuccess)
-            ptr = nullptr;
-        return (PFN_encodeTiledKv)ptr;
-    }();
+    static const auto fn = driver_fn<PFN_encodeTiledKv>("cuTensorMapEncodeTiled");
     if (!fn) return paged_fail(GLC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box,
@@ -601,7 +611,13 @@ extern "C" int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens,
                                Range{slots, 8LL * T}, Range{status, 4}})
             if ((uintptr_t)i.p < (uintptr_t)o.p + o.bytes && (uintptr_t)o.p < (uintptr_t)i.p + i.bytes)
                 return paged_fail(GLC_ERR_INVALID_ARG, "outputs must not alias ctx_lens, new_lens or free_count");
-    if (int rc = glc::paged_check_device(status, "status")) return rc;
+    const auto used = [](const void* ptr, int n) { return n ? ptr : nullptr; };   // arrays without elements may be anything
+    if (int rc = glc::paged_check_devices({{used(ctx_lens, B), "ctx_lens"}, {used(new_lens, B), "new_lens"},
+                                           {used(block_table, B), "block_table"}, {used(free_list, capacity), "free_list"},
+                                           {free_count, "free_count"}, {free_count_out, "free_count_out"}, {cu_new, "cu_new"},
+                                           {used(kv_lens, B), "kv_lens"}, {used(positions, T), "positions"},
+                                           {used(slots, T), "slots"}, {status, "status"}}))
+        return rc;
     glc::PlanParams p{};
     p.ctx = ctx_lens;
     p.nw = new_lens;
@@ -686,7 +702,11 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
             return paged_fail(GLC_ERR_INVALID_ARG, "%d KV heads for a cache of %d", n_kv_heads, cache->n_kv_heads);
     }
     if (T == 0) return GLC_OK;
-    if (int rc = glc::paged_check_device(k, "k")) return rc;
+    if (int rc = glc::paged_check_devices({{n_heads ? q : nullptr, "q"}, {k, "k"}, {v, "v"}, {positions, "positions"},
+                                           {slots, "slots"}, {cache ? cache->k : nullptr, "the cache's k"},
+                                           {cache ? cache->v : nullptr, "the cache's v"},
+                                           {n_heads ? q_out : nullptr, "q_out"}, {k_out, "k_out"}, {v_out, "v_out"}}))
+        return rc;
     glc::RopeParams p{};
     if (int rc = glc::paged_error_word(&p.err)) return rc;
     p.q = q;

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../../../include/glacier_b200.h"
 #include "kernels.h"
 
@@ -24,9 +26,13 @@ int paged_error_word(int** err);
 // recorded over this one).
 __device__ __forceinline__ void record_bad_arg(int* err) { atomicCAS(err, kDevOk, kDevBadArg); }
 
-// GLC_OK when `device_ptr` is memory the current device owns or can be handed
-// without faulting (managed and pinned host memory included).
-int paged_check_device(const void* device_ptr, const char* what);
+// GLC_OK when every pointer that is not null is memory the current device owns or can
+// be handed without faulting (managed and pinned host memory included).
+struct DevicePtr {
+    const void* p;
+    const char* what;
+};
+int paged_check_devices(std::initializer_list<DevicePtr> ptrs);
 
 // The shape, strides and alignment rules of a page set.
 int paged_check_pages(const glc_kv_pages* c);

@@ -114,3 +114,61 @@ def test_no_error_is_lost_to_a_poll(cuda, tmp_path):
 def test_places_of_the_join_are_written_after_a_timeout(cuda, tmp_path):
     out = subprocess.run([built(tmp_path, "tiles_scheduler_check")], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0, out.stdout + out.stderr
+
+
+def test_every_array_in_host_memory_is_refused(cuda, glc):
+    """Each device array of each call, replaced by ordinary host memory."""
+    torch = cuda
+    Hq, Hkv, T, B, ps = 4, 2, 20, 2, 16
+    g = lambda *s, t=torch.int32: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    host = np.zeros(1 << 16, np.uint8)
+    bad = (host.ctypes.data + 63) & ~63
+    f16, f32, i64 = torch.float16, torch.float32, torch.int64
+    kc, vc = g(4, Hkv, ps, 128, t=f16), g(4, Hkv, ps, 128, t=f16)
+    q, k, v, o = g(T, Hq, 128, t=f32), g(T, Hkv, 128, t=f32), g(T, Hkv, 128, t=f32), g(T, Hq, 128, t=f32)
+    ko, vo = g(T, Hkv, 128, t=f16), g(T, Hkv, 128, t=f16)
+    cu = torch.tensor([0, 10, 20], dtype=torch.int32, device="cuda")
+    kv = torch.tensor([10, 10], dtype=torch.int32, device="cuda")
+    slots = torch.arange(T, device="cuda")
+    ws = g(glc.attn_paged_workspace_bytes(Hq, Hkv, B, T, T), t=torch.uint8)
+    held = []                                     # arrays whose pointers are in use
+
+    def p(t):
+        held.append(t)
+        return t.data_ptr()
+
+    def pages(k_ptr, v_ptr):
+        return glc.KvPages(k_ptr, v_ptr, 4, ps, Hkv)
+    st = glc.torch_stream_handle()
+    plan = dict(ctx_lens_ptr=p(g(B)), new_lens_ptr=p(g(B)), block_table_ptr=p(g(B, 4)), free_list_ptr=p(g(8)),
+                free_count_ptr=p(g(1)), free_count_out_ptr=p(g(1)), cu_new_ptr=p(g(B + 1)), kv_lens_ptr=p(g(B)),
+                positions_ptr=p(g(T)), slots_ptr=p(g(T, t=i64)), status_ptr=p(g(1)))
+    append = dict(q_ptr=p(q), k_ptr=p(k), v_ptr=p(v), positions_ptr=p(g(T)), slots_ptr=p(slots), q_out_ptr=p(o),
+                  k_out_ptr=p(ko), v_out_ptr=p(vo), cache_k=p(kc), cache_v=p(vc))
+    prompt = dict(q_ptr=p(q), k_ptr=p(ko), v_ptr=p(vo), cu_seqlens_ptr=p(cu), out_ptr=p(o))
+    paged = dict(q_ptr=p(q), block_table_ptr=p(g(B, 4)), cu_new_ptr=p(cu), kv_lens_ptr=p(kv), out_ptr=p(o), work_ptr=p(ws),
+                 cache_k=p(kc), cache_v=p(vc))
+
+    def call_append(a):
+        a = dict(a)
+        cache = pages(a.pop("cache_k"), a.pop("cache_v"))
+        glc.rope_append_dev(**a, cache=cache, q_stride=Hq * 128, kv_stride=Hkv * 128, T=T, n_heads=Hq, n_kv_heads=Hkv,
+                            rope_theta=1e6, stream=st)
+
+    def call_paged(a):
+        a = dict(a)
+        cache = pages(a.pop("cache_k"), a.pop("cache_v"))
+        glc.attn_paged_dev(**a, cache=cache, q_type=glc.GGUF_F32, q_stride=Hq * 128, max_pages=4, B=B, T=T, max_new=10,
+                           n_heads=Hq, out_stride=Hq * 128, work_bytes=ws.numel(), stream=st)
+    calls = [(plan, lambda a: glc.kv_plan_dev(**a, B=B, page_size=ps, max_pages=4, capacity=8, T=T, stream=st)),
+             (append, call_append),
+             (prompt, lambda a: glc.attn_prompt_dev(**a, q_type=glc.GGUF_F32, q_stride=Hq * 128, kv_stride=Hkv * 128, B=B, T=T,
+                                                    n_heads=Hq, n_kv_heads=Hkv, out_stride=Hq * 128, stream=st)),
+             (paged, call_paged)]
+    for args, call in calls:
+        call(args)
+        for name in args:
+            with pytest.raises(glc.GlcError, match="device memory|known to CUDA") as e:
+                call({**args, name: bad})
+            assert e.value.status == -1 and name.replace("_ptr", "").split("_")[-1][:3] in str(e.value), name
+    glc.paged_poll_error()
