@@ -201,7 +201,8 @@ extern "C" int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_strid
     if (int rc = glc::check_rows(q, q_type, q_stride, out, out_stride, n_heads, cache->n_kv_heads, cache->head_dim,
                                  scale, B, T))
         return rc;
-    if (max_pages <= 0 || max_new < 0 || (int64_t)max_pages * cache->page_size > 0x7fffffff)
+    // (the kernels round key counts up to whole tiles in 32 bits)
+    if (max_pages <= 0 || max_new < 0 || (int64_t)max_pages * cache->page_size > 0x80000000ll - glc::kTile)
         return paged_fail(GLC_ERR_INVALID_ARG, "tables of %d pages, up to %d new tokens", max_pages, max_new);
     uint64_t need = 0;
     if (int rc = glc_attn_paged_workspace_bytes(n_heads, cache->n_kv_heads, B, T, max_new, &need)) return rc;

@@ -344,7 +344,8 @@ int glc_attn_prompt_dev(const void* q, int32_t q_type, int64_t q_stride, const v
  * holds them (a chunk of a prompt, or one decode token): sequence b's n new
  * rows are cu_new[b] .. cu_new[b+1], its cache holds kv_lens[b] rows in pages
  * block_table[b][0 ..], and its query i sees keys j <= kv_len - n + i (a query
- * that sees none gets zeros).  max_new: the most new tokens of any sequence.
+ * that sees none gets zeros).  max_new: the most new tokens of any sequence;
+ * max_pages * page_size is at most 2^31 - 128.
  * The rest as glc_attn_prompt_dev; rows of a page past kv_len are not read as
  * numbers.  A page id outside the cache, a kv_len past the table or a sequence
  * longer than max_new is recorded (glc_paged_poll_error) and that sequence's

@@ -172,3 +172,46 @@ def test_every_array_in_host_memory_is_refused(cuda, glc):
                 call({**args, name: bad})
             assert e.value.status == -1 and name.replace("_ptr", "").split("_")[-1][:3] in str(e.value), name
     glc.paged_poll_error()
+
+
+@pytest.mark.parametrize("qt", [0, 1])
+def test_decode_of_the_longest_tables(cuda, glc, qt):
+    """Two sequences of 2^31 - 128 rows, the most a table may name, over two pages: one
+    that is repeated, with keys of zero, and one behind it whose 64 keys score 20.  The
+    sums of the weights are exact (multiples of 2^12, at most 2^18 of them); what rounds
+    is the exponential (2^-20) and the join of 148 parts, in fp32, of numerator and
+    denominator: 2 x 150 x 2^-24 < 2^-15 of the weighted values.  fp32 queries add their
+    16-key products up exactly too (multiples of 2^11 below 2^35).  fp16 queries leave
+    them in the tensor core's accumulator, which may cut a unit of the last place, 2^-23
+    of the running sum, at each of a CTA's n tiles: equal products, so the sum after i
+    tiles is i / n of the last, and the cuts together at most (n + 1) / 2 x 2^-23 of the
+    repeated page's share; n is 2 (2^24 - 1 + 2) / 148 + 1."""
+    torch = cuda
+    ps, kv = 64, 2**31 - 128
+    width = kv // ps
+    rng = np.random.default_rng(21)
+    val = rng.integers(-32, 33, (2, 128)) / 8
+    kc, vc = (torch.zeros(2, 1, ps, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    kc[1, 0, :, 0] = 20
+    vc[:, 0] = torch.from_numpy(val).cuda()[:, None, :]
+    table = torch.zeros(2, width, dtype=torch.int32, device="cuda")
+    table[:, -1] = 1
+    dt = torch.float32 if qt == 0 else torch.float16
+    q, out = torch.zeros(2, 1, 128, dtype=dt, device="cuda"), torch.zeros(2, 1, 128, dtype=dt, device="cuda")
+    q[:, 0, 0] = 1
+    cu = torch.arange(3, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([kv, kv - 64], dtype=torch.int32, device="cuda")     # the second ends before the last page
+    ws = torch.empty(glc.attn_paged_workspace_bytes(1, 1, 2, 2, 1), dtype=torch.uint8, device="cuda")
+    glc.attn_paged_dev(q.data_ptr(), qt, 128, glc.KvPages(kc.data_ptr(), vc.data_ptr(), 2, ps, 1), table.data_ptr(), width,
+                       cu.data_ptr(), lens.data_ptr(), 2, 2, 1, 1, out.data_ptr(), 128, ws.data_ptr(), ws.numel(), scale=1.0,
+                       stream=glc.torch_stream_handle())
+    glc.paged_poll_error()
+    w = np.array([kv - 64, 64 * np.exp(20.0)])
+    w /= w.sum()
+    got = out[:, 0].double().cpu().numpy()
+    final = 2.0**-24 if qt == 0 else 2.0**-11
+    cut = 0.0 if qt == 0 else (2 * (2**24 + 1) / 148 + 2) / 2 * 2.0**-23
+    for g, wt in zip(got, (w, np.array([1.0, 0.0]))):
+        want = wt @ val
+        tol = (wt @ np.abs(val)) * 2.0**-15 + wt[0] * np.abs(val[0]) * cut + np.abs(want) * final + 1e-30
+        assert (np.abs(g - want) <= tol).all()

@@ -2,7 +2,7 @@
 (decided on the host: no GPU is touched)."""
 import pytest
 
-from test_paged_oracle import F16, F32, P, append_args, plan_args
+from test_paged_oracle import F16, F32, P, append_args, paged_args, pages, plan_args
 
 
 @pytest.mark.parametrize("kw", [
@@ -59,3 +59,15 @@ def test_plan_takes_arrays_side_by_side(glc):
     """Goes on to the check of the memory, which fails for a made-up pointer."""
     with pytest.raises(glc.GlcError, match="device|CUDA"):
         glc.kv_plan_dev(**apart())
+
+
+@pytest.mark.parametrize("ps", [16, 32, 64, 128, 256])
+def test_paged_refuses_tables_whose_tiles_pass_31_bits(glc, ps):
+    """The kernels round a key count up to tiles of 128 in 32 bits."""
+    most = (2**31 - 128) // ps
+    for n in (most + 1, (2**31 - 1) // ps + 1):
+        with pytest.raises(glc.GlcError, match="tables") as e:
+            glc.attn_paged_dev(**paged_args(glc, cache=pages(glc, page_size=ps), max_pages=n))
+        assert e.value.status == -1
+    with pytest.raises(glc.GlcError, match="device|CUDA"):     # goes on to the check of the memory
+        glc.attn_paged_dev(**paged_args(glc, cache=pages(glc, page_size=ps), max_pages=most))
