@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from oracle import paged as ref
-from test_gpu_paged import plan_case, run_plan, same_plan
+from test_gpu_paged import Paged, dev, plan_case, run_plan, same_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -215,3 +215,24 @@ def test_decode_of_the_longest_tables(cuda, glc, qt):
         want = wt @ val
         tol = (wt @ np.abs(val)) * 2.0**-15 + wt[0] * np.abs(val[0]) * cut + np.abs(want) * final + 1e-30
         assert (np.abs(g - want) <= tol).all()
+
+
+@pytest.mark.parametrize("qt", [0, 1])
+@pytest.mark.parametrize("new,kv", [([4, 4], [50, 60]), ([30, 50], [900, 60]), ([4, 40, 1, 2, 1, 3], [50, 600, 9, 70, 1, 400])])
+def test_first_rows_outside_are_held_inside(cuda, glc, new, kv, qt):
+    """A first row below 0 counts as 0, a last one past T as T: the rows that are left
+    are right, nothing is recorded and nothing beside the outputs is written."""
+    torch = cuda
+    p = Paged(torch, glc, np.random.default_rng(22), new, kv, 8, 2, 16, qt)
+    guard = torch.full((p.out.numel() + 4096,), 7.0, dtype=p.out.dtype, device="cuda")
+    p.out = guard[2048:-2048].view(p.out.shape)
+    around = torch.full((p.dq.numel() + 4096,), float("nan"), dtype=p.dq.dtype, device="cuda")
+    around[2048:-2048] = p.dq.flatten()
+    p.dq = around[2048:-2048].view(p.dq.shape)
+    cu = p.cu.copy()
+    cu[0], cu[-1] = -10, 10**9
+    p.dc.copy_(dev(torch, cu))
+    p.call()
+    glc.paged_poll_error()
+    p.check()
+    assert torch.all(guard[:2048] == 7) and torch.all(guard[-2048:] == 7)
