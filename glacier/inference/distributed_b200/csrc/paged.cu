@@ -145,7 +145,7 @@ namespace {
 // nothing waits.  More requests (kv_plan_kernel) go 1024 at a time through one
 // cluster of 8 CTAs, with a cluster barrier between the pages given back and the
 // pages taken.
-constexpr int kPlanMaxCluster = 8;
+constexpr int kPlanCluster = 8;
 constexpr int kPlanFlat = 4096;
 
 struct PlanParams {
@@ -187,7 +187,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long* part, lo
 }
 
 // First index in [0, n) whose inclusive end is above x (ends ascending).
-__device__ __forceinline__ int upper(const long long* end, int n, long long x) {
+template <typename T>
+__device__ __forceinline__ int upper(const T* end, int n, T x) {
     int lo = 0, hi = n;
     while (lo < hi) {
         const int m = (lo + hi) >> 1;
@@ -234,11 +235,7 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
     }
     const long long avail = min(free0 + back, (long long)p.capacity);
     // every push is visible to the cluster before any page is taken
-    if (size > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    } else {
-        __syncthreads();
-    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     long long rows = 0, need_sum = 0, used = 0;
     int bad = 0;
@@ -326,22 +323,10 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
                 used = max(used, part[w]);
                 bad += s_ok[w];
             }
-            if (p.B == 0) p.cu[0] = 0;
             *p.free_out = (int)(avail - used);
             *p.status = bad;
         }
     }
-}
-
-// First index in [0, n) whose inclusive end is above x (ends ascending).
-__device__ __forceinline__ int upper(const int* end, int n, int x) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int m = (lo + hi) >> 1;
-        if (end[m] > x) hi = m;
-        else lo = m + 1;
-    }
-    return lo;
 }
 
 // All of the shared memory of kv_plan_flat_kernel
@@ -653,12 +638,12 @@ extern "C" int glc_kv_plan_dev(const int32_t* ctx_lens, const int32_t* new_lens,
         }
     } else {
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(glc::kPlanMaxCluster);
+        cfg.gridDim = dim3(glc::kPlanCluster);
         cfg.blockDim = dim3(1024);
         cfg.stream = (cudaStream_t)stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = glc::kPlanMaxCluster;
+        attr[0].val.clusterDim.x = glc::kPlanCluster;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
