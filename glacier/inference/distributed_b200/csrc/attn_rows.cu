@@ -84,7 +84,7 @@ __device__ __forceinline__ RowsUnit load_unit(const AttnBatch& p, int b, bool re
     if (p.kv_lens) {
         const long long room = (long long)p.max_pages << p.ps_log2;
         u.kv_len = (int)min((long long)max(len, 0), room);
-        if (record && (len != u.kv_len || u.n > p.max_new)) record_bad_arg(p.err);
+        if (record && u.n > 0 && (len != u.kv_len || u.n > p.max_new)) record_bad_arg(p.err);
     }
     if (u.n * p.G > p.rows_take) u.n = 0;   // the tile kernel's
     u.tiles = u.n > 0 ? (u.kv_len + kTile - 1) / kTile : 0;

@@ -349,8 +349,9 @@ int glc_attn_prompt_dev(const void* q, int32_t q_type, int64_t q_stride, const v
  * The rest as glc_attn_prompt_dev; rows of a page past kv_len are not read as
  * numbers.  A page id outside the cache, a kv_len past the table or a sequence
  * longer than max_new is recorded (glc_paged_poll_error) and that sequence's
- * rows are unspecified; first rows that do not ascend may be recorded, and all
- * rows are unspecified then.  workspace: glc_attn_paged_workspace_bytes device
+ * rows are unspecified; what stands for a sequence without new tokens is not
+ * used.  First rows that do not ascend may be recorded, and all rows are
+ * unspecified then.  workspace: glc_attn_paged_workspace_bytes device
  * bytes, 16-byte aligned, any contents; those of the largest B, T and max_new
  * serve all smaller calls; calls that may overlap need their own. */
 int glc_attn_paged_workspace_bytes(int32_t n_heads, int32_t n_kv_heads, int32_t B, int32_t T, int32_t max_new,

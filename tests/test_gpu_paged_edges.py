@@ -236,3 +236,18 @@ def test_first_rows_outside_are_held_inside(cuda, glc, new, kv, qt):
     glc.paged_poll_error()
     p.check()
     assert torch.all(guard[:2048] == 7) and torch.all(guard[-2048:] == 7)
+
+
+@pytest.mark.parametrize("new", [[1, 0, 2], [1, 0, 2, 0, 1, 1], [40, 0, 2], [40, 0, 2, 0, 1, 1]])
+def test_idle_sequences_may_have_any_length(cuda, glc, new):
+    """A padded batch: what stands in kv_lens for a sequence without new tokens is not
+    used and not an error, whichever kernels run."""
+    torch = cuda
+    kv = [n + 30 * b for b, n in enumerate(new)]
+    p = Paged(torch, glc, np.random.default_rng(23), new, kv, 8, 2, 16, 1)
+    for garbage in (-1, 10**9, 2**31 - 1):
+        p.dkv[1] = garbage
+        p.out.fill_(7.0)
+        p.call()
+        glc.paged_poll_error()
+        p.check()
