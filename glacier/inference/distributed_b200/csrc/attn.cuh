@@ -13,12 +13,17 @@ constexpr int kHd = 128;
 constexpr int kTile = 128;                     // keys per tile
 constexpr int kTileBytes = kTile * kHd * 2;    // K or V of a tile
 constexpr int kRows = 16;                      // most query rows of a KV head in the row kernel
-constexpr float kPShift = 10.f;                // exponentials are stored as 2^10 e^(s - m): see below
+constexpr float kPShift = 10.f;                // exponentials are stored as 2^10 2^(s - m): see below
 
 constexpr float kMinFactor = 1.2e-38f;         // a factor of zero would turn a masked -inf into NaN
 
-// p = 2^(s - m) lies in [0, 1]; stored as 2^10 p its fp16 form stays normal down
-// to 2^-24 of the row's largest weight.  The factor cancels in o / l.
+// p = 2^(s - m) lies in [0, 1]; stored as 2^10 p its fp16 form (or the high one of two
+// halves) stays normal down to 2^-24 of the row's largest weight.  The factor cancels in
+// o / l.  Both kernels do so but for fp16 queries on tiles: there m may lag behind the
+// row's maximum by 11 powers of two, so 2^4 p is stored, normal down to 2^-18 of the
+// largest (see kShift16).  One fp16 weight is off by half a step, 2^-11: with the outputs'
+// own rounding rows of fp16 queries come out 2.5e-4 to 2.8e-4 off (2-norm), 2.1e-4 of it
+// from the outputs.
 
 struct AttnBatch {
     const void* q;
@@ -123,9 +128,12 @@ __device__ __forceinline__ void store_pair(void* out, int64_t off, float2 a, flo
 // ---- the kernels, and what a call needs of them
 constexpr int kTileRows = 256;                  // query rows of an item of the tile kernel
 constexpr int kTileParts = 8;                   // most parts of a unit's keys
-// From two units an SM on, whole units fill the SMs better than parts with their
-// join: 192 units of 130 key tiles take 456 us cut and 565 whole, 312 units of 65
-// take 490 cut and 430 whole (48 heads over 8, fp16 queries).
+// From two units an SM on, whole units of about the same length fill the SMs better than
+// parts with their join: 192 units of 130 key tiles take 456 us cut and 565 whole, 312
+// units of 65 take 490 cut and 430 whole (48 heads over 8, fp16 queries).  The rule counts
+// units whatever their length, so one long chunk among many short sequences is not cut: 64
+// fp32 tokens against 32,000 keys take 140 us alone, 202 next to 100 single tokens against
+// 500 keys, 915 next to 300 of them and 817 next to 40 sequences of four tokens.
 constexpr int kCutUnits = 2 * 148;
 constexpr int kTileExtra = 3 * 148;             // most items that cutting units into parts adds
 constexpr int kTilePartFloats = kTileRows * (kHd + 2);

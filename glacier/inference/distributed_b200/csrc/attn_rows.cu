@@ -14,9 +14,10 @@
 // of it over a CTA's n tiles: 2^-13 at 2,048 tiles (262,144 keys), a quarter of the
 // fp16 output's own half step.
 // Bound by the bytes of K and V: 64 sequences of 100 to 16,000 rows (48 heads over
-// 8, fp16 queries) take 141 us, 93 % of the copy rate.  One sequence of 2,048 rows
-// (40 heads over 8, fp32 queries) takes 9.5 us: the chain of lengths, page table,
-// keys, merge of the warps and join of the CTAs, not the 8.4 MB.
+// 8) take 140 to 145 us, 90 to 94 % of the copy rate, with fp16 queries and with fp32
+// ones.  One sequence of 2,048 rows (40 heads over 8, fp32 queries) takes 11 us a call,
+// 9.5 in a replayed graph: the chain of lengths, page table, keys, merge of the warps and
+// join of the CTAs, not the 8.4 MB.
 #include <type_traits>
 
 #include "attn.cuh"

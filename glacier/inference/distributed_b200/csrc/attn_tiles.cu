@@ -24,9 +24,10 @@
 // S): a key tile of a pair takes 3,600 cycles with fp16 queries, of which the tensor
 // core works 2,500 (a product of 128 x 128 x 16 takes 87 cycles with both operands in
 // shared memory, 67 with A in tensor memory) and the exponentials 2,050, and 6,200
-// with fp32 ones (4,600 and 2,050).  16,384 tokens (48 heads over 8, fp16) take
-// 3.1 ms, 1,060 TFLOP/s; 512 tokens against 32,513 keys (40 over 8, fp32) 575 us
-// (3.5 ms and 670 us where the power limit holds the clock down).
+// with fp32 ones (4,600 and 2,050).  Calls one after another, where the power limit holds
+// the clock down: 16,384 tokens (48 heads over 8, fp16) take 3.44 ms, 958 TFLOP/s; 512
+// tokens against 32,513 keys (40 over 8, fp32) 672 us, two products each.  At the full
+// clock 3.1 ms and 575 us.
 // An item costs 4,000 cycles more for its outputs, and fp32 queries 7,000 to load.
 #include <algorithm>
 #include <type_traits>
@@ -566,7 +567,8 @@ __device__ __forceinline__ void weights_ready(uint64_t* bar) {
 // scores in tensor memory (a row's 128 scores next to its 128 outputs would not
 // fit the registers): the maximum, then the exponentials.  Both loop over 32
 // scores as two loads of 16, the next in flight while one is worked on, and stay
-// rolled: unrolled, all the loads move to the top and their values spill.  MASK:
+// rolled: unrolled, all the loads move to the top and their values spill (the kernel as
+// it is still stores 40 bytes a thread and loads 64, by ptxas' count).  MASK:
 // keys at or past lim count as -inf.  Returns the rescale of what came before.
 template <bool MASK>
 __device__ __forceinline__ float softmax_row(uint32_t trow, int lim, float f, float& m, float& l, uint64_t* p_full) {

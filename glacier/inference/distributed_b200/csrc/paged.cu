@@ -728,7 +728,7 @@ extern "C" int glc_rope_append_dev(const float* q, int64_t q_stride, const float
     // A warp's four angles (double reduction, sincosf: ~200 instructions) serve its
     // run of head pairs: the shortest run whose warps are resident at once (three CTAs an
     // SM), up to eight pairs, and one pair a warp where the call is short (8192 rows of
-    // 48 / 8 heads, fp16 out: 234 us with runs of one pair, 68 us with eight: 5.8 TB/s;
+    // 48 / 8 heads, fp16 out: 234 us with runs of one pair, 68 us with eight: 5.9 TB/s;
     // 300 rows of 28 / 4: 8.3 us with one, 6.3 with two).
     p.run = (int)std::min<long long>(8, ((long long)T * pairs + 148 * 24 - 1) / (148 * 24));
     const long long warps = (long long)T * ((pairs + p.run - 1) / p.run);

@@ -269,7 +269,7 @@ int glc_attn_decode_dev(const float* q, const float* k_new, const float* v_new, 
  *      the calls run on the current device and the stream as given, allocate
  *      nothing and can be captured into a graph (the first call on a device
  *      looks up the error word's address: make it before a capture).  Pointers
- *      of another device are refused.  Lengths live on the device; what
+ *      of another device, or that CUDA does not know, are refused.  Lengths live on the device; what
  *      the host passes are row counts and bounds. ---- */
 
 /* Pages of one layer: row r of KV head h of page p is the 128 halves at
@@ -364,9 +364,11 @@ int glc_attn_paged_dev(const void* q, int32_t q_type, int64_t q_stride, const gl
 /* Reads and clears the device error word of the paged entry points on the
  * current device (synchronises the device): GLC_ERR_INVALID_ARG when a page
  * id, slot or length on the device was out of range, GLC_ERR_TIMEOUT when a
- * bounded device-side wait gave up (the outputs are unspecified then, and a
- * workspace that captured calls use has to be cleared), else GLC_OK.  The first
- * paged call on a device looks the word up: make one before any stream capture. */
+ * bounded device-side wait gave up (also where a bad argument came after it; the
+ * outputs are unspecified then, and a workspace that captured calls use has to be
+ * cleared), else GLC_OK.  What another stream or host thread records meanwhile is
+ * in this poll or in the next.  The first paged call on a device looks the word
+ * up: make one before any stream capture. */
 int glc_paged_poll_error(void);
 
 /* ---- router alone (for tests and for callers that route elsewhere) ---- */
